@@ -400,6 +400,89 @@ int tyr_hip_gemm_fp8_ws(const void* aq, const void* bq, void* c,
                         int trans_b, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Root-mean-square norm with the residual's addition.
+ *
+ * The norm of the decoder models (`RMSNorm` before attention, before the MLP and, without a residual, of the query and key heads),
+ * as tyr_hip_layernorm_residual is the LayerNorm:
+ *   out_resid = bf16(x + residual)                        (without a residual: x itself, nothing is written)
+ *   y         = out_resid * weight * rsqrt(mean(out_resid^2) + eps)
+ *   out       = bf16(y)                                   out_dtype = TYR_HIP_OUT_BF16
+ *   out       = e4m3(y / row_scale), row_scale = max |y| of the row / 448     out_dtype = TYR_HIP_OUT_E4M3
+ * The e4m3 output and its row scales are the `aq` and `row_scale` of tyr_hip_gemm_fp8_ex.  A row whose largest |y| is below 2^-100
+ * (a zero row among them) takes the scale 1.  Statistics are f32 over the whole row of the rounded out_resid.
+ *
+ *   x, residual, out_resid : bf16 [rows, d_model]; residual and out_resid both given or both NULL; outputs overlap no input
+ *   weight : bf16 [d_model]     out : bf16 or e4m3 [rows, d_model]     row_scale : f32 [rows] (e4m3), not looked at for bf16
+ * Supported: d_model % 8 == 0 up to 16384.
+ */
+int tyr_hip_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* out, void* out_resid,
+                             float* row_scale, uint64_t rows, uint64_t d_model, float eps, int out_dtype, void* stream);
+
+/* Gradients of the bf16 form.  With rho = rsqrt(mean(resid^2) + eps), g = d_out * weight:
+ *   dx      = bf16(rho g - (rho^3 / d_model) (sum g resid) resid + d_resid)     the gradient of x and of residual alike
+ *   dweight = bf16(sum over rows of d_out resid rho)
+ *   resid   : the forward's out_resid (its x where there was no residual), bf16 [rows, d_model]
+ *   d_out   : gradient of out, bf16 [rows, d_model]
+ *   d_resid : gradient that reaches out_resid by other ways, bf16 [rows, d_model], or NULL
+ *   dx      : bf16 [rows, d_model]      dweight : bf16 [d_model]      (they overlap no input)
+ *   workspace : tyr_hip_rmsnorm_residual_bwd_workspace_bytes(rows, d_model) bytes, 16-byte aligned, contents arbitrary
+ * The result is deterministic (no atomic accumulation).  Shapes as the forward. */
+size_t tyr_hip_rmsnorm_residual_bwd_workspace_bytes(uint64_t rows, uint64_t d_model);
+int tyr_hip_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const void* resid, const void* weight, void* dx,
+                                 void* dweight, uint64_t rows, uint64_t d_model, float eps, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Key-value cache in pages.
+ *
+ * No counterpart in the reference, whose cache is [batch, kv_heads, maxLen, head_dim] (Tyr/Model/Qwen/Attention.lean:54-68) and
+ * reserves maxLen rows for every sequence; tyr_hip_decode_rope_append and tyr_hip_gqa_decode are the same two calls on that one.
+ *
+ *   k_pages, v_pages : [num_pages, Hkv, page_size, D], bf16 (TYR_HIP_CACHE_BF16) or e4m3 (TYR_HIP_CACHE_E4M3)
+ *   page_table       : device int32 [B, table_width]; row j of sequence b is row j % page_size of page
+ *                      page_table[b * table_width + j / page_size].  An entry outside [0, num_pages) is a page that is not there:
+ *                      nothing is written to it, and its rows are not seen.
+ *   k_scale, v_scale : device f32 [Hkv], positive: a cached K is k_scale[kv head] * the stored value, V alike; NULL = all ones.
+ *                      Only with e4m3 pages.
+ * Supported: D in {64, 128}; page_size a multiple of 16; num_pages * Hkv * page_size / 16 < 2^31; table_width * page_size < 2^31.
+ *
+ * tyr_hip_paged_rope_append: rotary embedding of T new tokens a sequence and their way into the pages.
+ *   q : bf16 [B, T, Hq, D]     k_new, v_new : bf16 [B, T, Hkv, D]     q_out : bf16 [B, T, Hq, D] (rotated; may alias q)
+ *   cos, sin  : f32 [rope_rows, D/2], the whole rotary table
+ *   positions : device int32 [B], position of each sequence's first new token; negative = the sequence has none (a free place of the batch)
+ *   new_lens  : device int32 [B] or NULL (= T): new tokens of each sequence, the rest of its T are padding
+ *   Token t of sequence b stands at positions[b] + t: its q is rotated, its k (rotated) and v become that row of the cache.  Padding is
+ *   not written, nor is a token beyond the rotary table or the page table.  q_out of a token without a place in the rotary table is 0.
+ *   e4m3 pages take k / k_scale and v / v_scale, rounded to nearest even, saturating at +-448.
+ *   Two tokens of one call that stand in the same row of the same page race.
+ *   Supported: B * T * (Hq + 2 Hkv) * D / 16 < 2^32 - 256.
+ */
+enum tyr_hip_cache_dtype { TYR_HIP_CACHE_BF16 = 0, TYR_HIP_CACHE_E4M3 = 1 };
+int tyr_hip_paged_rope_append(const void* q, const void* k_new, const void* v_new, const float* cos, const float* sin, void* q_out,
+                              void* k_pages, void* v_pages, const int32_t* page_table, const int32_t* positions,
+                              const int32_t* new_lens, const float* k_scale, const float* v_scale, uint64_t B, uint64_t T,
+                              uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t num_pages, uint64_t page_size, uint64_t table_width,
+                              uint64_t rope_rows, int cache_dtype, void* stream);
+
+/* Attention of one new token of each sequence over its pages.
+ *   q, o    : bf16 [B, Hq, 1, D], query head h reads kv head h / (Hq/Hkv), any Hq/Hkv      lse : f32 [B, Hq] (may be NULL)
+ *   kv_lens : device int32 [B], rows of each sequence (the new token's among them), clamped to [0, table_width * page_size]
+ *   window  : 0 = every row is visible; > 0: row j of n is visible iff j >= n - window or j < sinks
+ *   sinks   : first rows that stay visible outside the window (without a window: no effect)
+ * Pages without a visible row are not looked at, and their table entries may hold anything.  A sequence that sees no row gets O = 0,
+ * LSE = -inf.  What the rows that are not visible hold, NaN included, does not matter.
+ * The batch is cut into pieces on the device, by the lengths that are there: a captured call follows lengths and tables that change
+ * between replays.  Results are reproducible for the same lengths.
+ *   workspace : tyr_hip_paged_decode_workspace_bytes(...) bytes, 16-byte aligned, contents arbitrary; calls that overlap in time need
+ *               one each (may be NULL where that is 0)
+ */
+size_t tyr_hip_paged_decode_workspace_bytes(uint64_t B, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t page_size, uint64_t table_width);
+int tyr_hip_paged_decode(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table, const int32_t* kv_lens,
+                         const float* k_scale, const float* v_scale, void* o, float* lse, uint64_t B, uint64_t Hq, uint64_t Hkv,
+                         uint64_t D, uint64_t num_pages, uint64_t page_size, uint64_t table_width, uint64_t window, uint64_t sinks,
+                         int cache_dtype, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
  * The element-wise half of the attention train step, fused.
  *
  * The reference's `oneKernelTrainStep` (Examples/GPU/RunMhaH100Train.lean:77-93) surrounds its forward

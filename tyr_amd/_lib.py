@@ -18,6 +18,8 @@ SYMBOLS = (
     "tyr_hip_gqa_decode_workspace_bytes", "tyr_hip_gqa_decode_auto_splits",
     "tyr_hip_gqa_decode", "tyr_hip_gqa_decode_varlen", "tyr_hip_gqa_decode_static", "tyr_hip_gemm_bf16", "tyr_hip_gemm_bf16_batched", "tyr_hip_gemm_bf16_batched_ws", "tyr_hip_gemm_workspace_bytes", "tyr_hip_gemm_force_general", "tyr_hip_flash_attn_fwd_persistent", "tyr_hip_gemm_fp8", "tyr_hip_gemm_fp8_ex", "tyr_hip_gemm_fp8_ws",
     "tyr_hip_decode_rope_append", "tyr_hip_rope_fwd", "tyr_hip_layernorm_residual", "tyr_hip_copy", "tyr_hip_mfma_sustain", "tyr_hip_mse_loss_grad_workspace_bytes", "tyr_hip_mse_loss_grad", "tyr_hip_sgd_step",
+    "tyr_hip_rmsnorm_residual", "tyr_hip_rmsnorm_residual_bwd_workspace_bytes", "tyr_hip_rmsnorm_residual_bwd", "tyr_hip_paged_rope_append",
+    "tyr_hip_paged_decode_workspace_bytes", "tyr_hip_paged_decode",
 )
 
 BINDING_PATH = os.path.join(_HERE, "lib", "_tyr_torch.so")
@@ -128,5 +130,17 @@ def load() -> ctypes.CDLL:
     L.tyr_hip_mse_loss_grad.restype = ci
     L.tyr_hip_sgd_step.argtypes = [vp, vp, f32, vp, vp, u64, vp]
     L.tyr_hip_sgd_step.restype = ci
+    L.tyr_hip_rmsnorm_residual.argtypes = [vp] * 6 + [u64, u64, f32, ci, vp]
+    L.tyr_hip_rmsnorm_residual.restype = ci
+    L.tyr_hip_rmsnorm_residual_bwd_workspace_bytes.argtypes = [u64, u64]
+    L.tyr_hip_rmsnorm_residual_bwd_workspace_bytes.restype = sz
+    L.tyr_hip_rmsnorm_residual_bwd.argtypes = [vp] * 6 + [u64, u64, f32, vp, sz, vp]
+    L.tyr_hip_rmsnorm_residual_bwd.restype = ci
+    L.tyr_hip_paged_rope_append.argtypes = [vp] * 13 + [u64] * 9 + [ci, vp]
+    L.tyr_hip_paged_rope_append.restype = ci
+    L.tyr_hip_paged_decode_workspace_bytes.argtypes = [u64] * 6
+    L.tyr_hip_paged_decode_workspace_bytes.restype = sz
+    L.tyr_hip_paged_decode.argtypes = [vp] * 9 + [u64] * 9 + [ci, f32, vp, sz, vp]
+    L.tyr_hip_paged_decode.restype = ci
     _lib = L
     return L

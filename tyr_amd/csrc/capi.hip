@@ -18,6 +18,7 @@
 namespace {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 inline bool fits_int(uint64_t v) { return v <= (uint64_t)INT_MAX; }
 // A window of all `rows` hides nothing that a larger one does not, and leaves the sums that plans and kernels make with it in 32 bits.
 inline int window_rows(uint64_t window, uint64_t rows) { return (int)std::min(window, rows); }
@@ -408,6 +409,116 @@ int tyr_hip_layernorm_residual(const void* x, const void* residual, const void* 
         return TYR_HIP_ERR_MISALIGNED;
     const int rc = tyr::launch_layernorm_residual(x, residual, weight, bias, out, out_resid, (size_t)rows,
                                                   (int)d_model, eps, static_cast<hipStream_t>(stream));
+    return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
+}
+
+static bool norm_extents(uint64_t rows, uint64_t d_model, int* rc) {
+    if (rows == 0 || d_model == 0) *rc = TYR_HIP_ERR_BAD_SHAPE;
+    else if (d_model % 8 != 0 || d_model > 16384) *rc = TYR_HIP_ERR_UNSUPPORTED;
+    else if (rows > (uint64_t)INT_MAX) *rc = TYR_HIP_ERR_BAD_SHAPE;
+    else return true;
+    return false;
+}
+
+int tyr_hip_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* out, void* out_resid, float* row_scale,
+                             uint64_t rows, uint64_t d_model, float eps, int out_dtype, void* stream) {
+    if (!x || !weight || !out || (residual != nullptr) != (out_resid != nullptr)) return TYR_HIP_ERR_NULL_POINTER;
+    int rc;
+    if (!norm_extents(rows, d_model, &rc)) return rc;
+    if ((out_dtype != TYR_HIP_OUT_BF16 && out_dtype != TYR_HIP_OUT_E4M3) || !(eps >= 0.0f)) return TYR_HIP_ERR_UNSUPPORTED;
+    if (out_dtype == TYR_HIP_OUT_E4M3 && !row_scale) return TYR_HIP_ERR_NULL_POINTER;
+    if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(out) || !aligned16(out_resid) || !aligned4(row_scale))
+        return TYR_HIP_ERR_MISALIGNED;
+    rc = tyr::launch_rmsnorm_residual(x, residual, weight, out, out_resid, row_scale, (size_t)rows, (int)d_model, eps,
+                                      out_dtype == TYR_HIP_OUT_E4M3, static_cast<hipStream_t>(stream));
+    return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
+}
+
+size_t tyr_hip_rmsnorm_residual_bwd_workspace_bytes(uint64_t rows, uint64_t d_model) {
+    int rc;
+    return norm_extents(rows, d_model, &rc) ? tyr::rmsnorm_residual_bwd_workspace_bytes((size_t)rows, (int)d_model) : 0;
+}
+
+int tyr_hip_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const void* resid, const void* weight, void* dx, void* dweight,
+                                 uint64_t rows, uint64_t d_model, float eps, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!d_out || !resid || !weight || !dx || !dweight) return TYR_HIP_ERR_NULL_POINTER;
+    int rc;
+    if (!norm_extents(rows, d_model, &rc)) return rc;
+    if (!(eps >= 0.0f)) return TYR_HIP_ERR_UNSUPPORTED;
+    if (!aligned16(d_out) || !aligned16(d_resid) || !aligned16(resid) || !aligned16(weight) || !aligned16(dx) || !aligned16(dweight))
+        return TYR_HIP_ERR_MISALIGNED;
+    if (!workspace || workspace_bytes < tyr::rmsnorm_residual_bwd_workspace_bytes((size_t)rows, (int)d_model)) return TYR_HIP_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return TYR_HIP_ERR_MISALIGNED;
+    rc = tyr::launch_rmsnorm_residual_bwd(d_out, d_resid, resid, weight, dx, dweight, (size_t)rows, (int)d_model, eps, workspace,
+                                          static_cast<hipStream_t>(stream));
+    return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
+}
+
+// what both calls on a cache in pages ask of it
+static int page_extents(uint64_t B, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t num_pages, uint64_t page_size, uint64_t table_width) {
+    if (B == 0 || Hq == 0 || Hkv == 0 || D == 0 || num_pages == 0 || page_size == 0 || table_width == 0) return TYR_HIP_ERR_BAD_SHAPE;
+    if (Hq % Hkv != 0) return TYR_HIP_ERR_BAD_SHAPE;
+    if ((D != 64 && D != 128) || page_size % 16 != 0) return TYR_HIP_ERR_UNSUPPORTED;
+    if (!fits_int(B) || !fits_int(Hq) || !fits_int(num_pages) || !fits_int(page_size) || !fits_int(table_width)) return TYR_HIP_ERR_BAD_SHAPE;
+    if (!fits_int(B * Hq) || !fits_int(table_width * page_size) || !fits_int(Hkv * (page_size / 16)) ||
+        num_pages > (uint64_t)INT_MAX / (Hkv * (page_size / 16)))
+        return TYR_HIP_ERR_BAD_SHAPE;
+    return TYR_HIP_OK;
+}
+// page scales belong to e4m3 pages
+static int page_format(int cache_dtype, const float* k_scale, const float* v_scale) {
+    if (cache_dtype != TYR_HIP_CACHE_BF16 && cache_dtype != TYR_HIP_CACHE_E4M3) return TYR_HIP_ERR_UNSUPPORTED;
+    if (cache_dtype == TYR_HIP_CACHE_BF16 && (k_scale || v_scale)) return TYR_HIP_ERR_UNSUPPORTED;
+    return aligned4(k_scale) && aligned4(v_scale) ? TYR_HIP_OK : TYR_HIP_ERR_MISALIGNED;
+}
+
+int tyr_hip_paged_rope_append(const void* q, const void* k_new, const void* v_new, const float* cos, const float* sin, void* q_out,
+                              void* k_pages, void* v_pages, const int32_t* page_table, const int32_t* positions,
+                              const int32_t* new_lens, const float* k_scale, const float* v_scale, uint64_t B, uint64_t T, uint64_t Hq,
+                              uint64_t Hkv, uint64_t D, uint64_t num_pages, uint64_t page_size, uint64_t table_width, uint64_t rope_rows,
+                              int cache_dtype, void* stream) {
+    if (!q || !k_new || !v_new || !cos || !sin || !q_out || !k_pages || !v_pages || !page_table || !positions) return TYR_HIP_ERR_NULL_POINTER;
+    int rc = page_extents(B, Hq, Hkv, D, num_pages, page_size, table_width);
+    if (rc != TYR_HIP_OK) return rc;
+    if (T == 0 || rope_rows == 0 || !fits_int(T) || !fits_int(rope_rows) || !fits_int(B * T)) return TYR_HIP_ERR_BAD_SHAPE;
+    if (Hq + 2 * Hkv > ((uint64_t)UINT32_MAX - 256) / (D / 16) / (B * T)) return TYR_HIP_ERR_BAD_SHAPE;     // threads of the launch
+    rc = page_format(cache_dtype, k_scale, v_scale);
+    if (rc != TYR_HIP_OK) return rc;
+    if (!aligned16(q) || !aligned16(k_new) || !aligned16(v_new) || !aligned16(cos) || !aligned16(sin) || !aligned16(q_out) ||
+        !aligned16(k_pages) || !aligned16(v_pages) || !aligned4(page_table) || !aligned4(positions) || !aligned4(new_lens))
+        return TYR_HIP_ERR_MISALIGNED;
+    rc = tyr::launch_paged_rope_append(q, k_new, v_new, cos, sin, q_out, k_pages, v_pages, page_table, positions, new_lens, k_scale,
+                                       v_scale, (int)B, (int)T, (int)Hq, (int)Hkv, (int)D, (int)num_pages, (int)page_size,
+                                       (int)table_width, (int)rope_rows, cache_dtype == TYR_HIP_CACHE_E4M3,
+                                       static_cast<hipStream_t>(stream));
+    return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
+}
+
+size_t tyr_hip_paged_decode_workspace_bytes(uint64_t B, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t page_size, uint64_t table_width) {
+    if (page_extents(B, Hq, Hkv, D, 1, page_size, table_width) != TYR_HIP_OK) return 0;
+    return tyr::paged_decode_workspace_bytes((int)B, (int)Hq, (int)Hkv, (int)D, (int64_t)(table_width * page_size));
+}
+
+int tyr_hip_paged_decode(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table, const int32_t* kv_lens,
+                         const float* k_scale, const float* v_scale, void* o, float* lse, uint64_t B, uint64_t Hq, uint64_t Hkv,
+                         uint64_t D, uint64_t num_pages, uint64_t page_size, uint64_t table_width, uint64_t window, uint64_t sinks,
+                         int cache_dtype, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!q || !k_pages || !v_pages || !page_table || !kv_lens || !o) return TYR_HIP_ERR_NULL_POINTER;
+    int rc = page_extents(B, Hq, Hkv, D, num_pages, page_size, table_width);
+    if (rc != TYR_HIP_OK) return rc;
+    rc = page_format(cache_dtype, k_scale, v_scale);
+    if (rc != TYR_HIP_OK) return rc;
+    if (!(scale > 0.0f) || scale > 3.0e38f) return TYR_HIP_ERR_UNSUPPORTED;
+    const uint64_t cap = table_width * page_size;
+    if (!fits_int(tyr::paged_decode_workgroups((int)B, (int)Hq, (int)Hkv, (int64_t)cap))) return TYR_HIP_ERR_BAD_SHAPE;
+    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o) || !aligned4(page_table) || !aligned4(kv_lens) || !aligned4(lse))
+        return TYR_HIP_ERR_MISALIGNED;
+    const size_t need = tyr_hip_paged_decode_workspace_bytes(B, Hq, Hkv, D, page_size, table_width);
+    if (need && (!workspace || workspace_bytes < need)) return TYR_HIP_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return TYR_HIP_ERR_MISALIGNED;
+    rc = tyr::launch_paged_decode(q, k_pages, v_pages, page_table, kv_lens, k_scale, v_scale, o, lse, (int)B, (int)Hq, (int)Hkv, (int)D,
+                                  (int)num_pages, (int)page_size, (int)table_width, window_rows(window, cap), window_rows(sinks, cap),
+                                  cache_dtype == TYR_HIP_CACHE_E4M3, scale, workspace, static_cast<hipStream_t>(stream));
     return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
 }
 

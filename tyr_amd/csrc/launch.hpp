@@ -50,5 +50,22 @@ int launch_decode_rope_append(const void* q, const void* k_new, const void* v_ne
                               int D, size_t kv_stride, size_t pos, hipStream_t stream);
 int launch_layernorm_residual(const void* x, const void* residual, const void* weight, const void* bias, void* out,
                               void* out_resid, size_t rows, int d_model, float eps, hipStream_t stream);
+// residual and out_resid: both or neither; row_scale [rows] with e4m3
+int launch_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* out, void* out_resid, float* row_scale,
+                            size_t rows, int d_model, float eps, int e4m3, hipStream_t stream);
+size_t rmsnorm_residual_bwd_workspace_bytes(size_t rows, int d_model);
+int launch_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const void* resid, const void* weight, void* dx, void* dweight,
+                                size_t rows, int d_model, float eps, void* workspace, hipStream_t stream);
+
+// The cache in pages; cap = rows that a table row can name.  k_scale / v_scale [Hkv] may be null.
+uint64_t paged_decode_workgroups(int B, int Hq, int Hkv, int64_t cap);
+size_t paged_decode_workspace_bytes(int B, int Hq, int Hkv, int D, int64_t cap);
+int launch_paged_decode(const void* q, const void* k_pages, const void* v_pages, const int* page_table, const int* kv_lens,
+                        const float* k_scale, const float* v_scale, void* o, float* lse, int B, int Hq, int Hkv, int D, int pages,
+                        int page_size, int width, int window, int sinks, int e4m3, float scale, void* workspace, hipStream_t stream);
+int launch_paged_rope_append(const void* q, const void* k_new, const void* v_new, const float* cosp, const float* sinp, void* q_out,
+                             void* k_pages, void* v_pages, const int* page_table, const int* positions, const int* new_lens,
+                             const float* k_scale, const float* v_scale, int B, int T, int Hq, int Hkv, int D, int pages, int page_size,
+                             int width, int rope_rows, int e4m3, hipStream_t stream);
 
 }  // namespace tyr

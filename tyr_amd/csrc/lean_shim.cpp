@@ -656,5 +656,223 @@ lean_object* lean_tyr_gpu_sgd_step(lean_obj_arg /*shape*/, b_lean_obj_arg param,
     }
 }
 
+// ---- RMS norm
+
+static lean_object* triple_result(torch::Tensor a, torch::Tensor b, torch::Tensor c) {      // a x (b x c)
+    lean_object* inner = lean_alloc_ctor(0, 2, 0);
+    lean_ctor_set(inner, 0, giveTensor(std::move(b)));
+    lean_ctor_set(inner, 1, giveTensor(std::move(c)));
+    lean_object* outer = lean_alloc_ctor(0, 2, 0);
+    lean_ctor_set(outer, 0, giveTensor(std::move(a)));
+    lean_ctor_set(outer, 1, inner);
+    return lean_io_result_mk_ok(outer);
+}
+
+// rmsNorm {rows d} x weight eps stream : IO (T #[rows,d])
+lean_object* lean_tyr_gpu_rmsnorm(uint64_t rows, uint64_t d, b_lean_obj_arg x, b_lean_obj_arg weight, double eps, uint64_t stream,
+                                  lean_object* /*world*/) {
+    try {
+        auto x_ = borrowTensor(x), w_ = borrowTensor(weight);
+        std::string err;
+        if (!check(x_, "x", torch::kBFloat16, err) || !check(w_, "weight", torch::kBFloat16, err)) return io_error(err);
+        LaunchStreamScope on_stream(stream, x_);   // outputs and scratch belong to the launch stream
+        auto out = torch::empty_like(x_);
+        const int rc = tyr_hip_rmsnorm_residual(x_.data_ptr(), nullptr, w_.data_ptr(), out.data_ptr(), nullptr, nullptr, rows, d,
+                                                (float)eps, TYR_HIP_OUT_BF16, reinterpret_cast<void*>(stream));
+        if (rc != TYR_HIP_OK) return status_error("rmsNorm", rc);
+        return lean_io_result_mk_ok(giveTensor(std::move(out)));
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+// rmsNormResidual {rows d} x residual weight eps stream : IO (out x outResid)
+lean_object* lean_tyr_gpu_rmsnorm_residual(uint64_t rows, uint64_t d, b_lean_obj_arg x, b_lean_obj_arg residual, b_lean_obj_arg weight,
+                                           double eps, uint64_t stream, lean_object* /*world*/) {
+    try {
+        auto x_ = borrowTensor(x), r_ = borrowTensor(residual), w_ = borrowTensor(weight);
+        std::string err;
+        if (!check(x_, "x", torch::kBFloat16, err) || !check(r_, "residual", torch::kBFloat16, err) ||
+            !check(w_, "weight", torch::kBFloat16, err))
+            return io_error(err);
+        LaunchStreamScope on_stream(stream, x_);   // outputs and scratch belong to the launch stream
+        auto out = torch::empty_like(x_), out_resid = torch::empty_like(x_);
+        const int rc = tyr_hip_rmsnorm_residual(x_.data_ptr(), r_.data_ptr(), w_.data_ptr(), out.data_ptr(), out_resid.data_ptr(),
+                                                nullptr, rows, d, (float)eps, TYR_HIP_OUT_BF16, reinterpret_cast<void*>(stream));
+        if (rc != TYR_HIP_OK) return status_error("rmsNormResidual", rc);
+        return pair_result(std::move(out), std::move(out_resid));
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+// rmsNormResidualE4M3 {rows d} x residual weight eps stream : IO (out x rowScale x outResid)
+lean_object* lean_tyr_gpu_rmsnorm_residual_e4m3(uint64_t rows, uint64_t d, b_lean_obj_arg x, b_lean_obj_arg residual,
+                                                b_lean_obj_arg weight, double eps, uint64_t stream, lean_object* /*world*/) {
+    try {
+        auto x_ = borrowTensor(x), r_ = borrowTensor(residual), w_ = borrowTensor(weight);
+        std::string err;
+        if (!check(x_, "x", torch::kBFloat16, err) || !check(r_, "residual", torch::kBFloat16, err) ||
+            !check(w_, "weight", torch::kBFloat16, err))
+            return io_error(err);
+        LaunchStreamScope on_stream(stream, x_);   // outputs and scratch belong to the launch stream
+        auto out = torch::empty_like(x_, x_.options().dtype(torch::kFloat8_e4m3fn)), out_resid = torch::empty_like(x_);
+        auto scale = torch::empty({(int64_t)rows}, x_.options().dtype(torch::kFloat32));
+        const int rc = tyr_hip_rmsnorm_residual(x_.data_ptr(), r_.data_ptr(), w_.data_ptr(), out.data_ptr(), out_resid.data_ptr(),
+                                                scale.data_ptr<float>(), rows, d, (float)eps, TYR_HIP_OUT_E4M3,
+                                                reinterpret_cast<void*>(stream));
+        if (rc != TYR_HIP_OK) return status_error("rmsNormResidualE4M3", rc);
+        return triple_result(std::move(out), std::move(scale), std::move(out_resid));
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+static lean_object* rmsnorm_bwd(const char* what, uint64_t rows, uint64_t d, const torch::Tensor& g, const torch::Tensor* dr,
+                                const torch::Tensor& h, const torch::Tensor& w, double eps, uint64_t stream) {
+    std::string err;
+    if (!check(g, "dOut", torch::kBFloat16, err) || !check(h, "resid", torch::kBFloat16, err) || !check(w, "weight", torch::kBFloat16, err) ||
+        (dr && !check(*dr, "dResid", torch::kBFloat16, err)))
+        return io_error(err);
+    LaunchStreamScope on_stream(stream, h);   // outputs and scratch belong to the launch stream
+    auto dx = torch::empty_like(h), dw = torch::empty_like(w);
+    const size_t ws_bytes = tyr_hip_rmsnorm_residual_bwd_workspace_bytes(rows, d);
+    auto ws = torch::empty({(int64_t)(ws_bytes ? ws_bytes : 16)}, h.options().dtype(torch::kUInt8));
+    const int rc = tyr_hip_rmsnorm_residual_bwd(g.data_ptr(), dr ? dr->data_ptr() : nullptr, h.data_ptr(), w.data_ptr(), dx.data_ptr(),
+                                                dw.data_ptr(), rows, d, (float)eps, ws.data_ptr(), ws_bytes, reinterpret_cast<void*>(stream));
+    if (rc != TYR_HIP_OK) return status_error(what, rc);
+    return pair_result(std::move(dx), std::move(dw));
+}
+
+// rmsNormBwd {rows d} dOut x weight eps stream : IO (dX x dWeight)
+lean_object* lean_tyr_gpu_rmsnorm_bwd(uint64_t rows, uint64_t d, b_lean_obj_arg d_out, b_lean_obj_arg x, b_lean_obj_arg weight, double eps,
+                                      uint64_t stream, lean_object* /*world*/) {
+    try {
+        return rmsnorm_bwd("rmsNormBwd", rows, d, borrowTensor(d_out), nullptr, borrowTensor(x), borrowTensor(weight), eps, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+// rmsNormResidualBwd {rows d} dOut dResid resid weight eps stream : IO (dX x dWeight)
+lean_object* lean_tyr_gpu_rmsnorm_residual_bwd(uint64_t rows, uint64_t d, b_lean_obj_arg d_out, b_lean_obj_arg d_resid,
+                                               b_lean_obj_arg resid, b_lean_obj_arg weight, double eps, uint64_t stream,
+                                               lean_object* /*world*/) {
+    try {
+        const auto dr = borrowTensor(d_resid);
+        return rmsnorm_bwd("rmsNormResidualBwd", rows, d, borrowTensor(d_out), &dr, borrowTensor(resid), borrowTensor(weight), eps, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+// ---- the cache in pages: bf16, or e4m3 with a factor per kv head
+
+static lean_object* paged_append(const char* what, uint64_t B, uint64_t T, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t P, uint64_t ps,
+                                 uint64_t W, uint64_t S, const torch::Tensor& q, const torch::Tensor& kn, const torch::Tensor& vn,
+                                 const torch::Tensor& cos, const torch::Tensor& sin, const torch::Tensor& k, const torch::Tensor& v,
+                                 const torch::Tensor& table, const torch::Tensor& pos, const torch::Tensor& lens, const torch::Tensor* ks,
+                                 const torch::Tensor* vs, uint64_t stream) {
+    std::string err;
+    const auto pages = ks ? torch::kFloat8_e4m3fn : torch::kBFloat16;
+    if (!check(q, "q", torch::kBFloat16, err) || !check(kn, "kNew", torch::kBFloat16, err) || !check(vn, "vNew", torch::kBFloat16, err) ||
+        !check(cos, "cos", torch::kFloat32, err) || !check(sin, "sin", torch::kFloat32, err) || !check(k, "kPages", pages, err) ||
+        !check(v, "vPages", pages, err) || !check(table, "pageTable", torch::kInt32, err) || !check(pos, "positions", torch::kInt32, err) ||
+        !check(lens, "newLens", torch::kInt32, err) || (ks && !check(*ks, "kScale", torch::kFloat32, err)) ||
+        (vs && !check(*vs, "vScale", torch::kFloat32, err)))
+        return io_error(err);
+    LaunchStreamScope on_stream(stream, q);   // outputs and scratch belong to the launch stream
+    auto q_out = torch::empty_like(q);
+    const int rc = tyr_hip_paged_rope_append(q.data_ptr(), kn.data_ptr(), vn.data_ptr(), cos.data_ptr<float>(), sin.data_ptr<float>(),
+                                             q_out.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr<int32_t>(),
+                                             pos.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), ks ? ks->data_ptr<float>() : nullptr,
+                                             vs ? vs->data_ptr<float>() : nullptr, B, T, Hq, Hkv, D, P, ps, W, S,
+                                             ks ? TYR_HIP_CACHE_E4M3 : TYR_HIP_CACHE_BF16, reinterpret_cast<void*>(stream));
+    if (rc != TYR_HIP_OK) return status_error(what, rc);
+    return lean_io_result_mk_ok(giveTensor(std::move(q_out)));
+}
+
+// pagedRopeAppend {B T Hq Hkv D P ps W S} q kNew vNew cos sin kPages vPages pageTable positions newLens stream : IO (T #[B,T,Hq,D])
+lean_object* lean_tyr_gpu_paged_rope_append(uint64_t B, uint64_t T, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t P, uint64_t ps,
+                                            uint64_t W, uint64_t S, b_lean_obj_arg q, b_lean_obj_arg k_new, b_lean_obj_arg v_new,
+                                            b_lean_obj_arg cos, b_lean_obj_arg sin, b_lean_obj_arg k_pages, b_lean_obj_arg v_pages,
+                                            b_lean_obj_arg table, b_lean_obj_arg positions, b_lean_obj_arg new_lens, uint64_t stream,
+                                            lean_object* /*world*/) {
+    try {
+        return paged_append("pagedRopeAppend", B, T, Hq, Hkv, D, P, ps, W, S, borrowTensor(q), borrowTensor(k_new), borrowTensor(v_new),
+                            borrowTensor(cos), borrowTensor(sin), borrowTensor(k_pages), borrowTensor(v_pages), borrowTensor(table),
+                            borrowTensor(positions), borrowTensor(new_lens), nullptr, nullptr, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+// pagedRopeAppendE4M3: the same with kScale vScale behind newLens
+lean_object* lean_tyr_gpu_paged_rope_append_e4m3(uint64_t B, uint64_t T, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t P, uint64_t ps,
+                                                 uint64_t W, uint64_t S, b_lean_obj_arg q, b_lean_obj_arg k_new, b_lean_obj_arg v_new,
+                                                 b_lean_obj_arg cos, b_lean_obj_arg sin, b_lean_obj_arg k_pages, b_lean_obj_arg v_pages,
+                                                 b_lean_obj_arg table, b_lean_obj_arg positions, b_lean_obj_arg new_lens,
+                                                 b_lean_obj_arg k_scale, b_lean_obj_arg v_scale, uint64_t stream, lean_object* /*world*/) {
+    try {
+        const auto ks = borrowTensor(k_scale), vs = borrowTensor(v_scale);
+        return paged_append("pagedRopeAppendE4M3", B, T, Hq, Hkv, D, P, ps, W, S, borrowTensor(q), borrowTensor(k_new), borrowTensor(v_new),
+                            borrowTensor(cos), borrowTensor(sin), borrowTensor(k_pages), borrowTensor(v_pages), borrowTensor(table),
+                            borrowTensor(positions), borrowTensor(new_lens), &ks, &vs, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+static lean_object* paged_attention(const char* what, uint64_t B, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t P, uint64_t ps, uint64_t W,
+                                    const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& table,
+                                    const torch::Tensor& lens, const torch::Tensor* ks, const torch::Tensor* vs, uint64_t window,
+                                    uint64_t sinks, double scale, uint64_t stream) {
+    std::string err;
+    const auto pages = ks ? torch::kFloat8_e4m3fn : torch::kBFloat16;
+    if (!check(q, "q", torch::kBFloat16, err) || !check(k, "kPages", pages, err) || !check(v, "vPages", pages, err) ||
+        !check(table, "pageTable", torch::kInt32, err) || !check(lens, "kvLens", torch::kInt32, err) ||
+        (ks && !check(*ks, "kScale", torch::kFloat32, err)) || (vs && !check(*vs, "vScale", torch::kFloat32, err)))
+        return io_error(err);
+    LaunchStreamScope on_stream(stream, q);   // outputs and scratch belong to the launch stream
+    auto o = torch::empty_like(q);
+    auto lse = torch::empty({(int64_t)B, (int64_t)Hq}, q.options().dtype(torch::kFloat32));
+    const size_t ws_bytes = tyr_hip_paged_decode_workspace_bytes(B, Hq, Hkv, D, ps, W);
+    auto ws = torch::empty({(int64_t)(ws_bytes ? ws_bytes : 16)}, q.options().dtype(torch::kUInt8));
+    const int rc = tyr_hip_paged_decode(q.data_ptr(), k.data_ptr(), v.data_ptr(), table.data_ptr<int32_t>(), lens.data_ptr<int32_t>(),
+                                        ks ? ks->data_ptr<float>() : nullptr, vs ? vs->data_ptr<float>() : nullptr, o.data_ptr(),
+                                        lse.data_ptr<float>(), B, Hq, Hkv, D, P, ps, W, window, sinks,
+                                        ks ? TYR_HIP_CACHE_E4M3 : TYR_HIP_CACHE_BF16, (float)scale, ws.data_ptr(), ws_bytes,
+                                        reinterpret_cast<void*>(stream));
+    if (rc != TYR_HIP_OK) return status_error(what, rc);
+    return pair_result(std::move(o), std::move(lse));
+}
+
+// pagedDecode {B Hq Hkv D P ps W} q kPages vPages pageTable kvLens window sinks scale stream : IO (T #[B,Hq,1,D] x T #[B,Hq])
+lean_object* lean_tyr_gpu_paged_decode(uint64_t B, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t P, uint64_t ps, uint64_t W,
+                                       b_lean_obj_arg q, b_lean_obj_arg k_pages, b_lean_obj_arg v_pages, b_lean_obj_arg table,
+                                       b_lean_obj_arg kv_lens, uint64_t window, uint64_t sinks, double scale, uint64_t stream,
+                                       lean_object* /*world*/) {
+    try {
+        return paged_attention("pagedDecode", B, Hq, Hkv, D, P, ps, W, borrowTensor(q), borrowTensor(k_pages), borrowTensor(v_pages),
+                               borrowTensor(table), borrowTensor(kv_lens), nullptr, nullptr, window, sinks, scale, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+// pagedDecodeE4M3: the same with kScale vScale behind kvLens
+lean_object* lean_tyr_gpu_paged_decode_e4m3(uint64_t B, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t P, uint64_t ps, uint64_t W,
+                                            b_lean_obj_arg q, b_lean_obj_arg k_pages, b_lean_obj_arg v_pages, b_lean_obj_arg table,
+                                            b_lean_obj_arg kv_lens, b_lean_obj_arg k_scale, b_lean_obj_arg v_scale, uint64_t window,
+                                            uint64_t sinks, double scale, uint64_t stream, lean_object* /*world*/) {
+    try {
+        const auto ks = borrowTensor(k_scale), vs = borrowTensor(v_scale);
+        return paged_attention("pagedDecodeE4M3", B, Hq, Hkv, D, P, ps, W, borrowTensor(q), borrowTensor(k_pages), borrowTensor(v_pages),
+                               borrowTensor(table), borrowTensor(kv_lens), &ks, &vs, window, sinks, scale, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
 }  // extern "C"
 #endif  // TYR_HAVE_LEAN

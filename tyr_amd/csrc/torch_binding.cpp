@@ -13,6 +13,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
@@ -68,7 +69,9 @@ public:
     X(tyr_hip_flash_attn_bwd_gqa) X(tyr_hip_flash_attn_bwd_mask) X(tyr_hip_gqa_decode_workspace_bytes)                        \
     X(tyr_hip_gqa_decode_varlen) X(tyr_hip_decode_rope_append) X(tyr_hip_rope_fwd) X(tyr_hip_layernorm_residual)             \
     X(tyr_hip_copy) X(tyr_hip_gemm_workspace_bytes) X(tyr_hip_gemm_bf16_batched_ws) X(tyr_hip_gemm_fp8_ws)                    \
-    X(tyr_hip_mse_loss_grad_workspace_bytes) X(tyr_hip_mse_loss_grad) X(tyr_hip_sgd_step)
+    X(tyr_hip_mse_loss_grad_workspace_bytes) X(tyr_hip_mse_loss_grad) X(tyr_hip_sgd_step)                                    \
+    X(tyr_hip_rmsnorm_residual) X(tyr_hip_rmsnorm_residual_bwd_workspace_bytes) X(tyr_hip_rmsnorm_residual_bwd)              \
+    X(tyr_hip_paged_rope_append) X(tyr_hip_paged_decode_workspace_bytes) X(tyr_hip_paged_decode)
 const struct Api {
 #define X(f) Symbol<decltype(&::f)> f{#f};
     TYR_ENTRY_POINTS(X)
@@ -344,6 +347,169 @@ PyObject* copy(PyObject* const* a) {
     return wrap(std::move(dst));
 }
 
+// The tensors of a call are on one device.  Without a stream given, that device is made current for the call, and the call goes to its
+// current stream; a stream given belongs to the current device, and so have the tensors to.
+struct OnDevice {
+    c10::DeviceIndex before, device;
+    OnDevice(const at::Tensor& first, std::initializer_list<const at::Tensor*> others, bool stream_given)
+        : before(c10::hip::current_device()), device(first.device().index()) {
+        for (const at::Tensor* t : others)
+            if (t && t->device() != first.device()) fail("all tensors must be on one device");
+        if (device == before) return;
+        if (stream_given) fail("the tensors must be on the stream's device");
+        c10::hip::set_device(device);
+    }
+    OnDevice(const OnDevice&) = delete;
+    ~OnDevice() {
+        if (device != before) (void)hipSetDevice(before);
+    }
+};
+// an empty tensor has no memory: say what is wrong with it rather than that its pointer is null
+void not_empty(std::initializer_list<const at::Tensor*> ts, const char* what) {
+    for (const at::Tensor* t : ts)
+        if (t->numel() == 0) check_status(TYR_HIP_ERR_BAD_SHAPE, what);
+}
+const at::Tensor* optional(PyObject* o, const char* name, at::ScalarType dtype, int ndim = -1) {
+    return o == Py_None ? nullptr : &checked(o, name, dtype, ndim);
+}
+void* pointer(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+
+// (x, residual, weight, eps, e4m3, stream_given) -> (out, out_resid) or (out, row_scale, out_resid)
+PyObject* rmsnorm_residual(PyObject* const* a) {
+    const at::Tensor &x = checked(a[0], "x", at::kBFloat16), &w = checked(a[2], "weight", at::kBFloat16, 1);
+    const at::Tensor* res = optional(a[1], "residual", at::kBFloat16);
+    const float eps = (float)real(a[3]);
+    const bool fp8 = truth(a[4]);
+    if (x.dim() == 0) fail("x must have dim >= 1");
+    const int64_t d = x.size(-1);
+    if ((res && res->sizes() != x.sizes()) || w.size(0) != d) fail("residual must match x, weight must be [d_model]");
+    not_empty({&x}, fp8 ? "rmsNormResidualE4M3" : "rmsNormResidual");
+    const OnDevice on(x, {res, &w}, truth(a[5]));
+    at::Tensor out, out_resid, scale;
+    int rc;
+    {
+        NoGil nogil;
+        out = empty(x.sizes(), fp8 ? at::kFloat8_e4m3fn : at::kBFloat16, x);
+        out_resid = res ? empty_like(x) : x;
+        if (fp8) scale = empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, x);
+        rc = api.tyr_hip_rmsnorm_residual(x.data_ptr(), pointer(res), w.data_ptr(), out.data_ptr(), res ? out_resid.data_ptr() : nullptr,
+                                          fp8 ? (float*)scale.data_ptr() : nullptr, d ? x.numel() / d : 0, d, eps,
+                                          fp8 ? TYR_HIP_OUT_E4M3 : TYR_HIP_OUT_BF16, stream());
+    }
+    check_status(rc, fp8 ? "rmsNormResidualE4M3" : "rmsNormResidual");
+    return fp8 ? wrap_tuple(std::move(out), std::move(scale), std::move(out_resid)) : wrap_tuple(std::move(out), std::move(out_resid));
+}
+
+// (d_out, resid, weight, eps, d_resid, stream_given)
+PyObject* rmsnorm_residual_bwd(PyObject* const* a) {
+    const at::Tensor &g = checked(a[0], "dOut", at::kBFloat16), &h = checked(a[1], "resid", at::kBFloat16),
+                     &w = checked(a[2], "weight", at::kBFloat16, 1);
+    const float eps = (float)real(a[3]);
+    const at::Tensor* dr = optional(a[4], "dResid", at::kBFloat16);
+    if (h.dim() == 0) fail("resid must have dim >= 1");
+    const int64_t d = h.size(-1);
+    if (g.sizes() != h.sizes() || (dr && dr->sizes() != h.sizes()) || w.size(0) != d)
+        fail("dOut and dResid must match resid, weight must be [d_model]");
+    not_empty({&h}, "rmsNormResidualBwd");
+    const OnDevice on(h, {&g, &w, dr}, truth(a[5]));
+    at::Tensor dx, dw;
+    int rc;
+    {
+        NoGil nogil;
+        dx = empty_like(h);
+        dw = empty_like(w);
+        const int64_t rows = d ? h.numel() / d : 0;
+        const at::Tensor ws = scratch(api.tyr_hip_rmsnorm_residual_bwd_workspace_bytes(rows, d), h);
+        rc = api.tyr_hip_rmsnorm_residual_bwd(g.data_ptr(), pointer(dr), h.data_ptr(), w.data_ptr(), dx.data_ptr(), dw.data_ptr(), rows, d,
+                                              eps, ws.data_ptr(), ws.numel(), stream());
+    }
+    check_status(rc, "rmsNormResidualBwd");
+    return wrap_tuple(std::move(dx), std::move(dw));
+}
+
+// ---- the cache in pages
+struct Pages {
+    const at::Tensor &k, &v, &table;
+    const at::Tensor *k_scale, *v_scale;
+    int64_t pages, Hkv, size, D, width;
+    int dtype;
+    Pages(PyObject* pk, PyObject* pv, PyObject* pt, PyObject* ks, PyObject* vs, int64_t B, int64_t D_)
+        : k(tensor(pk, "kPages")), v(tensor(pv, "vPages")), table(checked(pt, "pageTable", at::kInt, 2)),
+          k_scale(optional(ks, "kScale", at::kFloat, 1)), v_scale(optional(vs, "vScale", at::kFloat, 1)) {
+        if (k.scalar_type() != at::kBFloat16 && k.scalar_type() != at::kFloat8_e4m3fn) fail("kPages must have dtype torch.bfloat16 or torch.float8_e4m3fn");
+        check(k, "kPages", k.scalar_type(), 4);
+        check(v, "vPages", k.scalar_type(), 4);
+        pages = k.size(0), Hkv = k.size(1), size = k.size(2), D = k.size(3), width = table.size(1);
+        if (v.sizes() != k.sizes() || D != D_) fail("kPages and vPages must have the same shape [pages, Hkv, pageSize, D]");
+        if (table.size(0) != B) fail("pageTable must hold one row per sequence");
+        dtype = k.scalar_type() == at::kBFloat16 ? TYR_HIP_CACHE_BF16 : TYR_HIP_CACHE_E4M3;
+        if (dtype == TYR_HIP_CACHE_BF16 && (k_scale || v_scale)) fail("kScale and vScale belong to float8_e4m3fn pages");
+        if ((k_scale && k_scale->numel() != Hkv) || (v_scale && v_scale->numel() != Hkv)) fail("kScale and vScale must hold one factor per kv head");
+    }
+};
+const at::Tensor& one_each(PyObject* o, const char* name, int64_t B) {
+    const at::Tensor& t = checked(o, name, at::kInt, 1);
+    if (t.numel() != B) fail(std::string(name) + " must hold one value per sequence");
+    return t;
+}
+
+// (q, k_new, v_new, cos, sin, k_pages, v_pages, page_table, positions, new_lens, k_scale, v_scale, stream_given)
+PyObject* paged_rope_append(PyObject* const* a) {
+    const at::Tensor &q = checked(a[0], "q", at::kBFloat16, 4), &kn = checked(a[1], "kNew", at::kBFloat16, 4),
+                     &vn = checked(a[2], "vNew", at::kBFloat16, 4), &cos = checked(a[3], "cos", at::kFloat, 2),
+                     &sin = checked(a[4], "sin", at::kFloat, 2);
+    const int64_t B = q.size(0), T = q.size(1), Hq = q.size(2), D = q.size(3);
+    const Pages c(a[5], a[6], a[7], a[10], a[11], B, D);
+    const at::Tensor& pos = one_each(a[8], "positions", B);
+    const at::Tensor* lens = a[9] == Py_None ? nullptr : &one_each(a[9], "newLens", B);
+    for (const at::Tensor* t : {&kn, &vn})
+        if (t->size(0) != B || t->size(1) != T || t->size(2) != c.Hkv || t->size(3) != D) fail("kNew and vNew must have shape [B, T, Hkv, D]");
+    if (cos.sizes() != sin.sizes() || cos.size(1) != D / 2) fail("cos and sin must have shape [S, D/2]");
+    not_empty({&q, &kn, &cos, &c.k, &c.table}, "pagedRopeAppend");
+    const OnDevice on(q, {&kn, &vn, &cos, &sin, &c.k, &c.v, &c.table, c.k_scale, c.v_scale, &pos, lens}, truth(a[12]));
+    at::Tensor q_out;
+    int rc;
+    {
+        NoGil nogil;
+        q_out = empty_like(q);
+        rc = api.tyr_hip_paged_rope_append(q.data_ptr(), kn.data_ptr(), vn.data_ptr(), (const float*)cos.data_ptr(), (const float*)sin.data_ptr(),
+                                           q_out.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), (const int32_t*)c.table.data_ptr(),
+                                           (const int32_t*)pos.data_ptr(), (const int32_t*)pointer(lens), (const float*)pointer(c.k_scale),
+                                           (const float*)pointer(c.v_scale), B, T, Hq, c.Hkv, D, c.pages, c.size, c.width, cos.size(0), c.dtype,
+                                           stream());
+    }
+    check_status(rc, "pagedRopeAppend");
+    return wrap(std::move(q_out));
+}
+
+// (q, k_pages, v_pages, page_table, kv_lens, scale, window, sinks, k_scale, v_scale, stream_given)
+PyObject* paged_decode(PyObject* const* a) {
+    const at::Tensor& q = checked(a[0], "q", at::kBFloat16, 4);
+    const int64_t B = q.size(0), Hq = q.size(1), D = q.size(3);
+    if (q.size(2) != 1) fail("q must have shape [B, Hq, 1, D]");
+    const Pages c(a[1], a[2], a[3], a[8], a[9], B, D);
+    const at::Tensor& lens = one_each(a[4], "kvLens", B);
+    const float scale = attn_scale(a[5], D);
+    const int64_t window = integer(a[6]), sinks = integer(a[7]);
+    if (window < 0 || sinks < 0) fail("window and sinks must not be negative");
+    not_empty({&q, &c.k, &c.table}, "pagedDecode");
+    const OnDevice on(q, {&c.k, &c.v, &c.table, &lens, c.k_scale, c.v_scale}, truth(a[10]));
+    at::Tensor o, lse;
+    int rc;
+    {
+        NoGil nogil;
+        o = empty_like(q);
+        lse = empty({B, Hq}, at::kFloat, q);
+        const at::Tensor ws = scratch(api.tyr_hip_paged_decode_workspace_bytes(B, Hq, c.Hkv, D, c.size, c.width), q);
+        rc = api.tyr_hip_paged_decode(q.data_ptr(), c.k.data_ptr(), c.v.data_ptr(), (const int32_t*)c.table.data_ptr(),
+                                      (const int32_t*)lens.data_ptr(), (const float*)pointer(c.k_scale), (const float*)pointer(c.v_scale),
+                                      o.data_ptr(), (float*)lse.data_ptr(), B, Hq, c.Hkv, D, c.pages, c.size, c.width, window, sinks, c.dtype,
+                                      scale, ws.data_ptr(), ws.numel(), stream());
+    }
+    check_status(rc, "pagedDecode");
+    return wrap_tuple(std::move(o), std::move(lse));
+}
+
 // ---- products
 // B is [..., K, N], or [..., N, K] when transposed
 struct Extents { int64_t M, N, K; };
@@ -519,7 +685,8 @@ PyMethodDef methods[] = {
     TYR_METHOD(flash_attn_fwd, 8), TYR_METHOD(flash_attn_bwd, 11), TYR_METHOD(gqa_decode, 8), TYR_METHOD(decode_rope_append, 8),
     TYR_METHOD(rope_fwd, 3), TYR_METHOD(layernorm_residual, 5), TYR_METHOD(copy, 1), TYR_METHOD(gemm_bf16, 3),
     TYR_METHOD(matmul_bf16, 3), TYR_METHOD(gemm_fp8, 5), TYR_METHOD(gemm_fp8_scaled, 7), TYR_METHOD(mse_loss_grad, 2),
-    TYR_METHOD(sgd_step, 4), {nullptr, nullptr, 0, nullptr}};
+    TYR_METHOD(sgd_step, 4), TYR_METHOD(rmsnorm_residual, 6), TYR_METHOD(rmsnorm_residual_bwd, 6), TYR_METHOD(paged_rope_append, 13),
+    TYR_METHOD(paged_decode, 11), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tyr_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -29,6 +29,7 @@ _n = _lib.load_binding(TyrGpuError)
 _flash_attn_fwd, _flash_attn_bwd, _gqa_decode, _decode_rope_append = _n.flash_attn_fwd, _n.flash_attn_bwd, _n.gqa_decode, _n.decode_rope_append
 _rope_fwd, _layernorm_residual, _copy, _matmul_bf16, _gemm_bf16 = _n.rope_fwd, _n.layernorm_residual, _n.copy, _n.matmul_bf16, _n.gemm_bf16
 _gemm_fp8, _gemm_fp8_scaled, _mse_loss_grad, _sgd_step = _n.gemm_fp8, _n.gemm_fp8_scaled, _n.mse_loss_grad, _n.sgd_step
+_rmsnorm_residual, _rmsnorm_residual_bwd, _paged_rope_append, _paged_decode = _n.rmsnorm_residual, _n.rmsnorm_residual_bwd, _n.paged_rope_append, _n.paged_decode
 
 
 def library_path() -> str:
@@ -132,6 +133,62 @@ def layernorm_residual(x, residual, weight, bias, eps: float = 1e-5, stream=None
     if stream is None:
         return _layernorm_residual(x, residual, weight, bias, eps)
     return _on_stream(stream, _layernorm_residual, x, residual, weight, bias, eps)
+
+
+def rmsnorm_residual(x, residual, weight, eps: float = 1e-6, stream=None):
+    """(out, outResid) = rmsNormResidual x residual weight: outResid = x + residual, out = outResid * weight /
+    sqrt(mean(outResid^2) + eps) over the last axis.  bf16; x, residual [..., d]; weight [d].  Without a residual (None)
+    outResid is x itself."""
+    if stream is None:
+        return _rmsnorm_residual(x, residual, weight, eps, False, False)
+    return _on_stream(stream, _rmsnorm_residual, x, residual, weight, eps, False, True)
+
+
+def rmsnorm_residual_fp8(x, residual, weight, eps: float = 1e-6, stream=None):
+    """(out, rowScale, outResid) = rmsNormResidualE4M3 x residual weight: as rmsnorm_residual, with out as e4m3 [..., d] and
+    an f32 scale per row [...], out * rowScale being the norm: the ``aq`` and ``row_scale`` of gemm_fp8_scaled.  The
+    largest value of a row is +-448."""
+    if stream is None:
+        return _rmsnorm_residual(x, residual, weight, eps, True, False)
+    return _on_stream(stream, _rmsnorm_residual, x, residual, weight, eps, True, True)
+
+
+def rmsnorm_residual_bwd(d_out, resid, weight, eps: float = 1e-6, d_resid=None, stream=None):
+    """(dX, dWeight) = rmsNormResidualBwd dOut resid weight: gradients of rmsnorm_residual, bf16.  resid [..., d] is the
+    outResid that the forward returned, d_out the gradient of its out and d_resid (or None) the one that reaches outResid
+    from the layers behind.  dX [..., d] is the gradient of x and of the residual alike; dWeight [d]."""
+    if stream is None:
+        return _rmsnorm_residual_bwd(d_out, resid, weight, eps, d_resid, False)
+    return _on_stream(stream, _rmsnorm_residual_bwd, d_out, resid, weight, eps, d_resid, True)
+
+
+def paged_rope_append(q, k_new, v_new, cos, sin, k_pages, v_pages, page_table, positions, new_lens=None, k_scale=None, v_scale=None,
+                      stream=None):
+    """qRot = pagedRopeAppend q kNew vNew cos sin kPages vPages pageTable positions: rotates T new tokens of every sequence
+    and writes their k (rotated) and v into the pages, in place.
+
+    q bf16 [B,T,Hq,D]; k_new, v_new bf16 [B,T,Hkv,D]; cos, sin f32 [S,D/2], the whole rotary table; k_pages, v_pages
+    [pages,Hkv,page_size,D] bf16, or e4m3 with the factors k_scale, v_scale (f32 [Hkv], None = ones) that a stored value is
+    multiplied with; page_table int32 [B,width]; positions int32 [B], where each sequence's first new token stands (negative:
+    it has none); new_lens int32 [B], how many of the T tokens are real (None = all).  Row j of a sequence is row
+    j % page_size of page page_table[b, j / page_size].  Padding, tokens beyond the tables, and tokens on a page outside the
+    pool are not written.  Returns the rotated q [B,T,Hq,D] (0 where a token has no place in the rotary table)."""
+    if stream is None:
+        return _paged_rope_append(q, k_new, v_new, cos, sin, k_pages, v_pages, page_table, positions, new_lens, k_scale, v_scale, False)
+    return _on_stream(stream, _paged_rope_append, q, k_new, v_new, cos, sin, k_pages, v_pages, page_table, positions, new_lens, k_scale,
+                      v_scale, True)
+
+
+def paged_decode(q, k_pages, v_pages, page_table, kv_lens, scale: float | None = None, window: int = 0, sinks: int = 0, k_scale=None,
+                 v_scale=None, stream=None):
+    """O, LSE = pagedDecode q kPages vPages pageTable kvLens scale window sinks: attention of one new token over its pages.
+
+    q bf16 [B,Hq,1,D]; pages, page_table and scales as for paged_rope_append; kv_lens int32 [B], rows of each sequence, the new
+    token's among them (0: O = 0, LSE = -inf).  ``window`` > 0 restricts a sequence to its last ``window`` rows and its first
+    ``sinks``; table entries of pages without a visible row may hold anything.  -> (bf16 [B,Hq,1,D], f32 [B,Hq])."""
+    if stream is None:
+        return _paged_decode(q, k_pages, v_pages, page_table, kv_lens, scale, window, sinks, k_scale, v_scale, False)
+    return _on_stream(stream, _paged_decode, q, k_pages, v_pages, page_table, kv_lens, scale, window, sinks, k_scale, v_scale, True)
 
 
 def copy(src, stream=None):

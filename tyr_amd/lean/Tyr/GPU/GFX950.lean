@@ -199,4 +199,62 @@ opaque lossAndGradOut {s : Shape} (out target : @& T s) (stream : CudaStream) : 
 @[extern "lean_tyr_gpu_sgd_step"]
 opaque sgdUpdate {s : Shape} (param grad : @& T s) (lr : Float) (stream : CudaStream) : IO (T s × T s)
 
+/-- RMS norm over the last axis, bf16: `x · weight / √(mean(x²) + eps)`, `d % 8 = 0`, `d ≤ 16384` (also the norm of query
+    and key heads: `rows = B·S·H`, `d` = head dimension). -/
+@[extern "lean_tyr_gpu_rmsnorm"]
+opaque rmsNorm {rows d : UInt64} (x : @& T #[rows, d]) (weight : @& T #[d]) (eps : Float) (stream : CudaStream)
+    : IO (T #[rows, d])
+
+/-- Fused residual add + RMS norm, bf16: returns `(out, outResid)` with `outResid = x + residual` and
+    `out = outResid · weight / √(mean(outResid²) + eps)`. -/
+@[extern "lean_tyr_gpu_rmsnorm_residual"]
+opaque rmsNormResidual {rows d : UInt64} (x residual : @& T #[rows, d]) (weight : @& T #[d]) (eps : Float)
+    (stream : CudaStream) : IO (T #[rows, d] × T #[rows, d])
+
+/-- `rmsNormResidual` with an E4M3 output and its f32 scale per row: `(out, rowScale, outResid)`; `out` and `rowScale` are the
+    `a` and `rowScale` of `gemmFp8Scaled`. -/
+@[extern "lean_tyr_gpu_rmsnorm_residual_e4m3"]
+opaque rmsNormResidualE4M3 {rows d : UInt64} (x residual : @& T #[rows, d]) (weight : @& T #[d]) (eps : Float)
+    (stream : CudaStream) : IO (T #[rows, d] × T #[rows] × T #[rows, d])
+
+/-- Gradients of `rmsNorm`: `(dX, dWeight)`, bf16. -/
+@[extern "lean_tyr_gpu_rmsnorm_bwd"]
+opaque rmsNormBwd {rows d : UInt64} (dOut x : @& T #[rows, d]) (weight : @& T #[d]) (eps : Float) (stream : CudaStream)
+    : IO (T #[rows, d] × T #[d])
+
+/-- Gradients of `rmsNormResidual`: `resid` is the forward's `outResid`, `dResid` the gradient that reaches it from the layers
+    behind. Returns `(dX, dWeight)`; `dX` is the gradient of `x` and of `residual` alike. -/
+@[extern "lean_tyr_gpu_rmsnorm_residual_bwd"]
+opaque rmsNormResidualBwd {rows d : UInt64} (dOut dResid resid : @& T #[rows, d]) (weight : @& T #[d]) (eps : Float)
+    (stream : CudaStream) : IO (T #[rows, d] × T #[d])
+
+/-- `decodeRopeAppend` for a cache in pages, and for any number `Tn` of new tokens a sequence. `kPages vPages : bf16
+    [P, Hkv, ps, D]` are written **in place**; row `j` of sequence `b` is row `j % ps` of page `pageTable[b, j / ps]` (int32).
+    `cos sin : f32 [S, D/2]` is the whole rotary table, `positions : int32 [B]` where each sequence's first new token stands
+    (negative: it has none), `newLens : int32 [B]` how many of its `Tn` tokens are real. Returns the rotated `q`. -/
+@[extern "lean_tyr_gpu_paged_rope_append"]
+opaque pagedRopeAppend {B Tn Hq Hkv D P ps W S : UInt64} (q : @& T #[B, Tn, Hq, D]) (kNew vNew : @& T #[B, Tn, Hkv, D])
+    (cos sin : @& T #[S, D / 2]) (kPages vPages : @& T #[P, Hkv, ps, D]) (pageTable : @& T #[B, W])
+    (positions newLens : @& T #[B]) (stream : CudaStream) : IO (T #[B, Tn, Hq, D])
+
+/-- `pagedRopeAppend` into E4M3 pages: a cached value is `kScale[kvHead]` (`vScale`) times the stored one. -/
+@[extern "lean_tyr_gpu_paged_rope_append_e4m3"]
+opaque pagedRopeAppendE4M3 {B Tn Hq Hkv D P ps W S : UInt64} (q : @& T #[B, Tn, Hq, D]) (kNew vNew : @& T #[B, Tn, Hkv, D])
+    (cos sin : @& T #[S, D / 2]) (kPages vPages : @& T #[P, Hkv, ps, D]) (pageTable : @& T #[B, W])
+    (positions newLens : @& T #[B]) (kScale vScale : @& T #[Hkv]) (stream : CudaStream) : IO (T #[B, Tn, Hq, D])
+
+/-- `gqaDecodeVarlen` over a cache in pages. `kvLens : int32 [B]`, the new token's row among them; `window = 0` shows every
+    row, otherwise the last `window` and the first `sinks` (whose pages alone have to be in the table). A sequence that sees no
+    row gets `O = 0`, `LSE = -∞`. -/
+@[extern "lean_tyr_gpu_paged_decode"]
+opaque pagedDecode {B Hq Hkv D P ps W : UInt64} (q : @& T #[B, Hq, 1, D]) (kPages vPages : @& T #[P, Hkv, ps, D])
+    (pageTable : @& T #[B, W]) (kvLens : @& T #[B]) (window sinks : UInt64) (scale : Float) (stream : CudaStream)
+    : IO (T #[B, Hq, 1, D] × T #[B, Hq])
+
+/-- `pagedDecode` over E4M3 pages. -/
+@[extern "lean_tyr_gpu_paged_decode_e4m3"]
+opaque pagedDecodeE4M3 {B Hq Hkv D P ps W : UInt64} (q : @& T #[B, Hq, 1, D]) (kPages vPages : @& T #[P, Hkv, ps, D])
+    (pageTable : @& T #[B, W]) (kvLens : @& T #[B]) (kScale vScale : @& T #[Hkv]) (window sinks : UInt64) (scale : Float)
+    (stream : CudaStream) : IO (T #[B, Hq, 1, D] × T #[B, Hq])
+
 end Tyr.GPU.GFX950
