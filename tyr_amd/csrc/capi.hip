@@ -510,7 +510,7 @@ int tyr_hip_paged_decode(const void* q, const void* k_pages, const void* v_pages
     if (rc != TYR_HIP_OK) return rc;
     if (!(scale > 0.0f) || scale > 3.0e38f) return TYR_HIP_ERR_UNSUPPORTED;
     const uint64_t cap = table_width * page_size;
-    if (!fits_int(tyr::paged_decode_workgroups((int)B, (int)Hq, (int)Hkv, (int64_t)cap))) return TYR_HIP_ERR_BAD_SHAPE;
+    if (B * Hkv * ((Hq / Hkv + 15) / 16) > (uint64_t)INT_MAX / (cap / 32 + 8)) return TYR_HIP_ERR_BAD_SHAPE;      // steps of all heads
     if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o) || !aligned4(page_table) || !aligned4(kv_lens) || !aligned4(lse))
         return TYR_HIP_ERR_MISALIGNED;
     const size_t need = tyr_hip_paged_decode_workspace_bytes(B, Hq, Hkv, D, page_size, table_width);

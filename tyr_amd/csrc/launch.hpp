@@ -58,7 +58,6 @@ int launch_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const vo
                                 size_t rows, int d_model, float eps, void* workspace, hipStream_t stream);
 
 // The cache in pages; cap = rows that a table row can name.  k_scale / v_scale [Hkv] may be null.
-uint64_t paged_decode_workgroups(int B, int Hq, int Hkv, int64_t cap);
 size_t paged_decode_workspace_bytes(int B, int Hq, int Hkv, int D, int64_t cap);
 int launch_paged_decode(const void* q, const void* k_pages, const void* v_pages, const int* page_table, const int* kv_lens,
                         const float* k_scale, const float* v_scale, void* o, float* lse, int B, int Hq, int Hkv, int D, int pages,

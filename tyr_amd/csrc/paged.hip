@@ -5,12 +5,14 @@
 // 16 rows of an MFMA tile lie in one page; an entry outside [0, num_pages) is a page that is not there.
 //
 // Attention.  Row j of a sequence of n rows is visible iff j < n and (no window, or j >= n - window, or j < sinks).  The visible
-// rows are walked as a list of 16-row tiles, the sinks' first; pages without a visible row are never looked at.
-//   grid: one workgroup per (piece of a sequence, kv head, block of 16 of its query heads).  How a batch is cut into pieces is
-//   decided on the device from the lengths that are there, by every workgroup for itself: pieces of `chunk` tiles, so that there are
-//   about `target` workgroups however the lengths are spread and however wide the table is, and a captured launch follows lengths
-//   that change between replays.  The host only bounds the grid, (B + target / heads) pieces a head.
-//   Partial results (O, m, l) of sequences of several pieces are joined by a second launch, as
+// rows are walked as a list of 16-row tiles, the sinks' first, two tiles a step; pages without a visible row are never looked at.
+//   All steps of all heads (a head: one kv head of one sequence, and at most 16 of its query heads) stand in one row, sequence by
+//   sequence, and are dealt out evenly to as many waves as the device holds, one a SIMD: each works out its share from the lengths
+//   that are there, so neither unequal lengths nor a table much wider than they are leave CUs idle, and a captured launch follows
+//   lengths that change between replays.  A wave goes through its share without a pause between heads.  (Workgroups of four waves on
+//   one piece of a sequence, joined through LDS, 512 and more of them: 64 sequences of 37 to 32768 e4m3 rows took 160-190 us, so 117;
+//   32 sequences of 8192 bf16 rows 182, so 173.)
+//   Heads that several waves have a part of are joined by a second launch from partial results (O, m, l), as
 //     m = max m_s ; l = sum l_s 2^(m_s-m) ; O = sum O_s 2^(m_s-m) / l ; LSE = ln l + m ln 2.
 // HBM-bound: each visible row of K and V is read once a block of query heads, straight into MFMA operand registers (16x16x32 bf16):
 //   S^T (16 rows x 16 q) = K x Q^T and O^T_j (16 d x 16 q) += V^T x P^T, j = 0..7, the layouts of the contiguous decode:
@@ -21,12 +23,16 @@
 #include "common.hpp"
 #include "launch.hpp"
 
+#include <algorithm>
+
 namespace tyr {
 
 namespace paged {
-constexpr int TILE = 16, WAVES = 4, THREADS = 64 * WAVES, QPAD = 16;
-constexpr int MIN_CHUNK = 8;                // tiles of a piece at least
-constexpr int TARGET = 512;                 // pieces times heads that a launch aims at
+constexpr int TILE = 16, STEP = 2 * TILE, WAVES = 4, THREADS = 64 * WAVES;
+constexpr int SHARES = 1024;                // waves that share a launch's steps: one on every SIMD of 256 CUs
+constexpr int MIN_SHARE = 2;                // steps of a wave at least
+constexpr int WHOLE = 4;                    // sequences of so many steps at most are not cut
+constexpr int TURN = 3;                     // steps that going from one head to the next is counted as
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -49,39 +55,19 @@ struct Rows {
         auto below = [t](int row) { return (1u << max(0, min(TILE, row - t * TILE))) - 1u; };
         return below(n) & (~below(lo) | below(sinks));
     }
+    // of 32 rows; a sequence without rows has one, in which nothing is visible, and so gets its zeros written
+    __device__ __forceinline__ int steps() const { return max(1, (count + 1) / 2); }
 };
-__device__ __forceinline__ int rows_of(const int* kv_lens, int b, int cap) { return max(0, min(kv_lens[b], cap)); }
 
-struct Piece { int b, split, splits, first; };   // sequence; which of its pieces; pieces of sequences before it; b < 0: none
-
-// Piece j of the batch.  Every wave works it out for itself, 64 sequences at a time.
-__device__ __forceinline__ Piece find_piece(const int* kv_lens, int B, int cap, int window, int sinks, int heads, int target, int j, int lane) {
-    uint64_t tiles = 0;
-    for (int b = lane; b < B; b += 64) tiles += Rows(rows_of(kv_lens, b, cap), window, sinks).count;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) tiles += __shfl_xor(tiles, o, 64);
-    const uint64_t even = (tiles * heads + target - 1) / target;
-    const int chunk = (int)max((uint64_t)MIN_CHUNK, min(even, (uint64_t)1 << 28));       // a sequence has less than 2^27 tiles
-    int before = 0;
-    for (int b0 = 0; b0 < B; b0 += 64) {
-        const int b = b0 + lane;
-        const int mine = b < B ? max(1, (Rows(rows_of(kv_lens, b, cap), window, sinks).count + chunk - 1) / chunk) : 0;
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int left = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += left;
-        }
-        const int first = before + upto - mine;
-        const uint64_t here = __builtin_amdgcn_ballot_w64(j >= first && j < first + mine);
-        if (here) {
-            const int at = __builtin_ctzll(here);
-            const int start = __builtin_amdgcn_readlane(first, at);
-            return {b0 + at, j - start, __builtin_amdgcn_readlane(mine, at), start};
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
-    }
-    return {-1, 0, 0, 0};
+// Sum of x over this lane and those before it, by moves of the vector unit.
+__device__ __forceinline__ int sum_upto(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);      // 1, 2, 4, 8 lanes to the left in rows of 16
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);      // lane 15 of a row to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);      // lane 31 to rows 2 and 3
+    return x;
 }
 
 struct Args {
@@ -91,11 +77,24 @@ struct Args {
     const float *k_scale, *v_scale;
     uint16_t* o;
     float *lse, *part_o, *part_m, *part_l;
-    int2* plan;                             // [B] first piece and pieces of each sequence
+    int2* plan;                             // [B] first step of each sequence's first head, steps of a head; [B]: steps of a wave
     int B, Hq, Hkv, G, blocks;              // G = query heads of a kv head; blocks of 16 of them
     int width, page_tiles, pages;           // pages of a table row; tiles of a page; pages of the pool
-    int cap, window, sinks, target;
+    int cap, window, sinks, shares;         // shares = 0: every wave takes one head of one sequence, nothing is cut
     float scale_log2;
+};
+
+// The sequences in rounds of 64, one a lane.
+struct Round {
+    int b0, n, steps, upto;                 // its first sequence; this lane's rows, steps of a head, and those (and turns) up to it in the round
+    __device__ __forceinline__ void read(const Args& a, int b0_, int lane) {
+        b0 = b0_;
+        const int b = b0 + lane;
+        n = b < a.B ? max(0, min(a.kv_lens[b], a.cap)) : 0;
+        steps = b < a.B ? Rows(n, a.window, a.sinks).steps() : 0;
+        upto = sum_upto(b < a.B ? steps + TURN : 0);
+    }
+    __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(upto, 63); }
 };
 
 // What a lane holds of 32 rows.
@@ -108,6 +107,19 @@ template <int D> struct Buf<D, true> {
     u32x2 v[8];
 };
 
+// A tile of a pool as a buffer of `bytes` bytes.  Of one of no bytes loads give 0 and read nothing, so every step loads alike,
+// also behind the last one: a load that may or may not have been made is one that the compiler waits for together with all later ones.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* pool, size_t at, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(pool) + at), 0, bytes, 0x00020000);
+}
+constexpr int NT = 2;                       // cache policy: not kept
+__device__ __forceinline__ u32x4 load_tile_16(__amdgpu_buffer_rsrc_t t, int at) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(t, at, 0, NT));
+}
+__device__ __forceinline__ u32x2 load_tile_8(__amdgpu_buffer_rsrc_t t, int at) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(t, at, 0, NT));
+}
+
 __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t four, bool upper) {
     const bf16x2 r = upper ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, 1.0f, false);
     return __builtin_bit_cast(uint32_t, r);
@@ -118,111 +130,217 @@ __device__ __forceinline__ u32x4 bf16_of_e4m3(uint32_t lo, uint32_t hi) {
 }  // namespace paged
 
 template <int D, bool FP8>
-__global__ __launch_bounds__(paged::THREADS) void paged_decode_kernel(const paged::Args a) {
+__global__ __launch_bounds__(paged::THREADS, 1) void paged_decode_kernel(const paged::Args a) {
     using namespace paged;
-    extern __shared__ __attribute__((aligned(16))) float smem[];   // [WAVES][heads][D] O, then [WAVES][QPAD] m, l
-    const int t = threadIdx.x, lane = t & 63, w = __builtin_amdgcn_readfirstlane(t >> 6), x = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * WAVES + threadIdx.x / 64));
     const int heads = a.Hkv * a.blocks;
-    const int hb = (int)(blockIdx.x % (unsigned)heads), j = (int)(blockIdx.x / (unsigned)heads);
-    const int kvh = hb / a.blocks, q0 = (hb % a.blocks) * 16, nq = min(16, a.G - q0);     // query heads q0 .. q0 + nq of kv head kvh
-    Piece piece{j, 0, 1, j};
-    if (a.target) {
-        piece = find_piece(a.kv_lens, a.B, a.cap, a.window, a.sinks, heads, a.target, j, lane);
-        if (piece.b < 0) return;
-        if (hb == 0 && piece.split == 0 && t == 0) a.plan[piece.b] = int2{piece.first, piece.splits};
-    }
-    const int b = piece.b;
-    const Rows rows(rows_of(a.kv_lens, b, a.cap), a.window, a.sinks);
-    const int c0 = (int)((int64_t)rows.count * piece.split / piece.splits), c1 = (int)((int64_t)rows.count * (piece.split + 1) / piece.splits);
+    constexpr int KI = D / 32, TILE_BYTES = TILE * D * (FP8 ? 1 : 2);
 
-    // Q^T operand: column x = query head q0 + x (zero beyond the block's heads)
-    constexpr int KI = D / 32, ES = FP8 ? 1 : 2;
-    const size_t head0 = (size_t)b * a.Hq + (size_t)kvh * a.G + q0;
-    bf16x8 qf[KI];
-    {
+    // ---- this wave's steps [at, end) of all, and the head of the sequence in which they begin
+    Round round;
+    int at, end, b, hb, first;                       // first = the sequence's (head's) first step
+    if (a.shares == 0) {
+        if (wave >= a.B * heads) return;
+        b = wave / heads;
+        hb = wave - b * heads;
+        round.read(a, b & ~63, lane);
+        at = first = 0;
+        end = __builtin_amdgcn_readlane(round.steps, b & 63);
+    } else {
+        round.read(a, 0, lane);
+        int all = round.total();
+        for (int b0 = 64; b0 < a.B; b0 += 64) {
+            Round r;
+            r.read(a, b0, lane);
+            all += r.total();
+        }
+        all *= heads;
+        const int share = max(MIN_SHARE, (all + a.shares - 1) / a.shares);
+        if (wave == 0 && lane == 0) a.plan[a.B] = int2{share, 0};
+        at = min((int64_t)wave * share, (int64_t)all);
+        end = min(at + share, all);
+        // the round in which step `at` lies; the first wave goes through all of them and writes down the plan
+        int before = 0, base = 0;
+        Round r = round;
+        for (int b0 = 0;;) {
+            const int upto = before + r.total() * heads;
+            if (wave == 0 && b0 + lane < a.B) a.plan[b0 + lane] = int2{before + (r.upto - r.steps - TURN) * heads, r.steps};
+            if (before <= at && at < upto) {
+                round = r;
+                base = before;
+            }
+            if (wave != 0 && at < upto) break;
+            before = upto;
+            b0 += 64;
+            if (b0 >= a.B) break;
+            r.read(a, b0, lane);
+        }
+        if (at >= end) return;
+        // the first lane whose sequence ends behind `at`
+        const int i = __builtin_ctzll(__builtin_amdgcn_ballot_w64(at < base + round.upto * heads));
+        const int each = __builtin_amdgcn_readlane(round.steps, i) + TURN;
+        const int start = base + (__builtin_amdgcn_readlane(round.upto, i) - each) * heads;
+        b = round.b0 + i;
+        hb = (at - start) / each;
+        first = start + hb * each;
+    }
+
+    // ---- where the rows of a step are.  The lanes work it out for up to 32 steps of one head at once (lane 2s + T: tile T of step s).
+    struct Run { int tile; uint32_t mask; int steps, b, hb, first, last; };       // steps of the run; the head's first step and its end
+    int next_at = at, next_b = b, next_hb = hb, next_first = first;
+    auto turn = [&]() {                              // to the next head
+        next_first += __builtin_amdgcn_readlane(round.steps, next_b - round.b0) + TURN;
+        next_at = next_first;
+        if (++next_hb == heads) {
+            next_hb = 0;
+            if (++next_b - round.b0 == 64) round.read(a, next_b, lane);
+        }
+    };
+    auto locate = [&]() {
+        Run r;
+        const Rows rows(__builtin_amdgcn_readlane(round.n, next_b - round.b0), a.window, a.sinks);
+        r.b = next_b, r.hb = next_hb, r.first = next_first;
+        r.last = next_first + rows.steps();
+        r.steps = min(32, min(r.last, end) - next_at);
+        r.tile = 0, r.mask = 0;
+        const int t = 2 * (next_at - next_first) + lane;
+        if (t < rows.count && lane < 2 * r.steps) {
+            const int tile = rows.tile(t), page = tile / a.page_tiles, id = a.table[(size_t)next_b * a.width + page];
+            if (id >= 0 && id < a.pages) {
+                r.tile = (id * a.Hkv + next_hb / a.blocks) * a.page_tiles + tile - page * a.page_tiles;
+                r.mask = rows.mask(tile);
+            }
+        }
+        next_at += r.steps;
+        if (next_at == r.last && next_at < end) turn();
+        return r;
+    };
+    if (at - first >= __builtin_amdgcn_readlane(round.steps, b - round.b0)) {       // the wave's share begins in a turn
+        turn();
+        if (next_at >= end) return;
+        b = next_b, hb = next_hb, first = next_first;
+    }
+
+    constexpr int DEEP = 2;                          // steps whose rows are under way or in use
+    struct Slot { Buf<D, FP8> buf; uint32_t seen[2]; int b, hb, first, last; bool live; };
+    Run run = locate(), then;
+    then.steps = 0;
+    if (next_at < end) then = locate();
+    int s = 0;                                       // step of the run to load next
+    auto load = [&](Slot& o) {
+        if (s >= run.steps) {
+            run = then;
+            s = 0;
+            then.steps = 0;
+            if (next_at < end) then = locate();
+        }
+        o.live = run.steps > 0;
+        o.b = run.b, o.hb = run.hb, o.first = run.first, o.last = run.last;
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+            o.seen[T] = (uint32_t)__builtin_amdgcn_readlane((int)run.mask, 2 * s + T);
+            const size_t base = (size_t)(uint32_t)__builtin_amdgcn_readlane(run.tile, 2 * s + T) * TILE_BYTES;
+            const int there = o.live && o.seen[T] ? TILE_BYTES : 0;
+            const auto k = tile_rsrc(a.k, base, there), v = tile_rsrc(a.v, base, there);
+            if constexpr (FP8) {
+#pragma unroll
+                for (int c = 0; c < D / 64; ++c) o.buf.k[T][c] = load_tile_16(k, x * D + 16 * (4 * c + g));
+#pragma unroll
+                for (int p = 0; p < 4; ++p) o.buf.v[4 * T + p] = load_tile_8(v, (4 * g + p) * D + (x & (D / 8 - 1)) * 8);
+            } else {
+#pragma unroll
+                for (int i = 0; i < KI; ++i) o.buf.k[T][i] = load_tile_16(k, (x * D + 32 * i + 8 * g) * 2);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) o.buf.v[4 * T + p] = load_tile_16(v, ((4 * g + p) * D + (x & (D / 8 - 1)) * 8) * 2);
+            }
+        }
+        ++s;
+    };
+
+    // ---- one head: Q^T operand (column x = query head q0 + x, zero beyond the block's heads) and running sums
+    __shared__ u32x4 qs[WAVES][KI][64];
+    u32x4 (&qf)[KI][64] = qs[threadIdx.x / 64];      // a lane reads what it wrote: registers are short, LDS is idle
+    f32x4 oacc[8];
+    float m2, lsum, scale_log2;
+    int nq, kvh;
+    size_t head0;
+    auto begin = [&](int b_, int hb_) {
+        kvh = hb_ / a.blocks;
+        const int q0 = (hb_ - kvh * a.blocks) * 16;
+        nq = min(16, a.G - q0);
+        head0 = (size_t)b_ * a.Hq + (size_t)kvh * a.G + q0;
         const uint16_t* qp = a.q + (head0 + min(x, nq - 1)) * D;
 #pragma unroll
         for (int i = 0; i < KI; ++i) {
-            const int d = FP8 ? 16 * (4 * (i >> 1) + g) + 8 * (i & 1) : 32 * i + 8 * g;
-            u32x4 v = ld_global_16(qp + d);
+            u32x4 v = ld_global_16(qp + (FP8 ? 16 * (4 * (i >> 1) + g) + 8 * (i & 1) : 32 * i + 8 * g));
             if (x >= nq) v = u32x4{0, 0, 0, 0};
-            qf[i] = __builtin_bit_cast(bf16x8, v);
+            qf[i][lane] = v;
         }
-    }
-    const float scale_log2 = a.scale_log2 * (a.k_scale ? a.k_scale[kvh] : 1.0f);
-
-    f32x4 oacc[8];
+        scale_log2 = a.scale_log2 * (a.k_scale ? a.k_scale[kvh] : 1.0f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) oacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m2 = -INFINITY, lsum = 0.0f;
-
-    // The waves take the piece's 32-row steps in turn.  Where a step's two tiles are and which of their rows count is worked out by
-    // the lanes for 32 steps at once (lane 2s + T: tile T of step s), and read from them as scalars.
-    const int nsteps = max(0, ((c1 - c0 + 1) / 2 - w + WAVES - 1) / WAVES);
-    const int* entries = a.table + (size_t)b * a.width;
-    struct Where { int tile; uint32_t mask; };
-    auto locate = [&](int step0) {
-        const int i = c0 + 2 * (w + WAVES * (step0 + (lane >> 1))) + (lane & 1);
-        Where r{0, 0};
-        if (i < c1) {
-            const int tile = rows.tile(i), page = tile / a.page_tiles, id = entries[page];
-            if (id >= 0 && id < a.pages) r = {(id * a.Hkv + kvh) * a.page_tiles + tile - page * a.page_tiles, rows.mask(tile)};
-        }
-        return r;
+        for (int i = 0; i < 8; ++i) oacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m2 = -INFINITY;
+        lsum = 0.0f;
     };
-    Where at[2] = {locate(0), Where{0, 0}};
-    if (nsteps > 32) at[1] = locate(32);
-
-    auto load = [&](Buf<D, FP8>& bf, int st) {
-        const int from = st & 32 ? at[1].tile : at[0].tile;
+    // The head's steps are done, or this wave's: its result where the wave had all of them, else a partial one.  A wave has at most two
+    // heads that it shares with others: one that began before it, and one that goes on behind it.  oacc[i][r] is O^T[d = 32g + 8r + i][x].
+    auto finish = [&](int first_, int last_) {
+        const float l = sum_xor32(sum_xor16(lsum)), v_scale = a.v_scale ? a.v_scale[kvh] : 1.0f;
+        if (x >= nq || 32 * g >= D) return;
+        if (first_ >= at && last_ <= end) {
+            const float f = l == 0.0f ? 0.0f : v_scale / l;
+            uint16_t* to = a.o + (head0 + x) * D + 32 * g;
 #pragma unroll
-        for (int T = 0; T < 2; ++T) {
-            const size_t base = (size_t)(uint32_t)__builtin_amdgcn_readlane(from, 2 * (st & 31) + T) * (TILE * D * ES);
-            const unsigned char *kb = static_cast<const unsigned char*>(a.k) + base, *vb = static_cast<const unsigned char*>(a.v) + base;
-            if constexpr (FP8) {
+            for (int r = 0; r < 4; ++r)
+                st_global_16(to + 8 * r, u32x4{pack_bf16(oacc[0][r] * f, oacc[1][r] * f), pack_bf16(oacc[2][r] * f, oacc[3][r] * f),
+                                               pack_bf16(oacc[4][r] * f, oacc[5][r] * f), pack_bf16(oacc[6][r] * f, oacc[7][r] * f)});
+            if (g == 0 && a.lse) a.lse[head0 + x] = l == 0.0f ? -INFINITY : logf(l) + m2 * LN2;
+        } else {
+            const size_t slot = (size_t)(2 * wave + (first_ < at ? 0 : 1)) * min(16, a.G) + x;
+            float* to = a.part_o + slot * D + 32 * g;
 #pragma unroll
-                for (int c = 0; c < D / 64; ++c) bf.k[T][c] = ld_global_16_nt(kb + x * D + 16 * (4 * c + g));
-#pragma unroll
-                for (int p = 0; p < 4; ++p)
-                    bf.v[4 * T + p] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(vb + (4 * g + p) * D + (x & (D / 8 - 1)) * 8));
-            } else {
-#pragma unroll
-                for (int i = 0; i < KI; ++i) bf.k[T][i] = ld_global_16_nt(kb + (x * D + 32 * i + 8 * g) * 2);
-#pragma unroll
-                for (int p = 0; p < 4; ++p) bf.v[4 * T + p] = ld_global_16_nt(vb + ((4 * g + p) * D + (x & (D / 8 - 1)) * 8) * 2);
+            for (int r = 0; r < 4; ++r) {
+                *reinterpret_cast<f32x4*>(to + 8 * r) = f32x4{oacc[0][r], oacc[1][r], oacc[2][r], oacc[3][r]} * v_scale;
+                *reinterpret_cast<f32x4*>(to + 8 * r + 4) = f32x4{oacc[4][r], oacc[5][r], oacc[6][r], oacc[7][r]} * v_scale;
             }
+            if (g == 0) { a.part_m[slot] = m2; a.part_l[slot] = l; }
         }
     };
 
-    auto compute = [&](const Buf<D, FP8>& bf, int st) {
-        const uint32_t masks = st & 32 ? at[1].mask : at[0].mask;
-        uint32_t seen[2];
+    int now = first, now_last = 0;                   // the head whose sums are in the registers
+    auto compute = [&](const Slot& o) {
+        if (o.first != now) {
+            finish(now, now_last);
+            begin(o.b, o.hb);
+            now = o.first;
+        }
+        now_last = o.last;
         f32x4 sacc[2];
         u32x4 v[8];
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
-            seen[T] = (uint32_t)__builtin_amdgcn_readlane((int)masks, 2 * (st & 31) + T);
             sacc[T] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < KI; ++i) {
                 u32x4 k;
-                if constexpr (FP8) k = i & 1 ? bf16_of_e4m3(bf.k[T][i / 2][2], bf.k[T][i / 2][3]) : bf16_of_e4m3(bf.k[T][i / 2][0], bf.k[T][i / 2][1]);
-                else k = bf.k[T][i];
-                sacc[T] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), qf[i], sacc[T]);
+                if constexpr (FP8) k = i & 1 ? bf16_of_e4m3(o.buf.k[T][i / 2][2], o.buf.k[T][i / 2][3]) : bf16_of_e4m3(o.buf.k[T][i / 2][0], o.buf.k[T][i / 2][1]);
+                else k = o.buf.k[T][i];
+                sacc[T] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, qf[i][lane]), sacc[T]);
             }
         }
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
-            if constexpr (FP8) v[p] = bf16_of_e4m3(bf.v[p][0], bf.v[p][1]);
-            else v[p] = bf.v[p];
+            if constexpr (FP8) v[p] = bf16_of_e4m3(o.buf.v[p][0], o.buf.v[p][1]);
+            else v[p] = o.buf.v[p];
         }
         // register r of tile T is its row 4g + r.  What is hidden may hold anything: its score goes, and its V, which 0 * NaN would keep.
-        if ((seen[0] & seen[1]) != 0xffffu) {
+        if ((o.seen[0] & o.seen[1]) != 0xffffu) {
 #pragma unroll
             for (int T = 0; T < 2; ++T)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    if (!(seen[T] >> (4 * g + r) & 1)) {
+                    if (!(o.seen[T] >> (4 * g + r) & 1)) {
                         sacc[T][r] = -INFINITY;
                         v[4 * T + r] = u32x4{0, 0, 0, 0};
                     }
@@ -251,70 +369,34 @@ __global__ __launch_bounds__(paged::THREADS) void paged_decode_kernel(const page
             hi[i] = pack_bf16(pv[2 * i], pv[2 * i + 1]);
             lo[i] = pack_bf16(pv[2 * i] - bf16_lo(hi[i]), pv[2 * i + 1] - bf16_hi(hi[i]));
         }
-        u32x4 vt[8];
-        transpose8x8_b16(v, vt);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            oacc[i] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, vt[i]), __builtin_bit_cast(bf16x8, hi), oacc[i]);
-            oacc[i] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, vt[i]), __builtin_bit_cast(bf16x8, lo), oacc[i]);
+        for (int c = 0; c < 4; ++c) {                // columns 2c and 2c + 1 of V's 8x8 piece, transposed
+            u32x4 even, odd;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                even[i] = __builtin_amdgcn_perm(v[2 * i + 1][c], v[2 * i][c], 0x05040100u);
+                odd[i] = __builtin_amdgcn_perm(v[2 * i + 1][c], v[2 * i][c], 0x07060302u);
+            }
+            oacc[2 * c] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), __builtin_bit_cast(bf16x8, hi), oacc[2 * c]);
+            oacc[2 * c] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), __builtin_bit_cast(bf16x8, lo), oacc[2 * c]);
+            oacc[2 * c + 1] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), __builtin_bit_cast(bf16x8, hi), oacc[2 * c + 1]);
+            oacc[2 * c + 1] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), __builtin_bit_cast(bf16x8, lo), oacc[2 * c + 1]);
         }
     };
 
-    Buf<D, FP8> b0, b1;
-    if (nsteps > 0) load(b0, 0);
+    begin(b, hb);
+    Slot slots[DEEP];
 #pragma unroll
-    for (int i = 0; i < KI; ++i) pin_registers(qf[i]);
-    for (int st = 0; st < nsteps; st += 2) {
-        if (st + 1 < nsteps) load(b1, st + 1);
-        compute(b0, st);
-        if (st + 1 < nsteps) {
-            if (st + 2 < nsteps) load(b0, st + 2);
-            compute(b1, st + 1);
-        }
-        // the half that steps st+2 on do not need takes the places of 32 steps further on
-        if (((st + 2) & 31) == 0 && st + 2 + 32 < nsteps) at[(st >> 5) & 1] = locate(st + 2 + 32);
-    }
-
-    // ---- merge the waves through LDS.  oacc[i][r] is O^T[d = 32g + 8r + i][q = x].
-    float* so = smem;                                // [WAVES][nq][D]
-    float* sm = smem + WAVES * nq * D;               // [WAVES][QPAD]
-    float* sl = sm + WAVES * QPAD;
-    const float ltot = sum_xor32(sum_xor16(lsum));
-    if (x < nq && 32 * g < D) {
-        float* dst = so + ((size_t)w * nq + x) * D + 32 * g;
+    for (int i = 0; i < DEEP - 1; ++i) load(slots[i]);
+    for (bool more = true; more;) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            *reinterpret_cast<f32x4*>(dst + 8 * r) = f32x4{oacc[0][r], oacc[1][r], oacc[2][r], oacc[3][r]};
-            *reinterpret_cast<f32x4*>(dst + 8 * r + 4) = f32x4{oacc[4][r], oacc[5][r], oacc[6][r], oacc[7][r]};
+        for (int i = 0; i < DEEP && more; ++i) {
+            load(slots[(i + DEEP - 1) % DEEP]);
+            compute(slots[i]);
+            more = slots[(i + 1) % DEEP].live;
         }
     }
-    if (x < nq && g == 0) { sm[w * QPAD + x] = m2; sl[w * QPAD + x] = ltot; }
-    __syncthreads();
-    const float v_scale = a.v_scale ? a.v_scale[kvh] : 1.0f;
-    const int per = min(16, a.G);                    // partial slots are laid out for this many heads
-    for (int idx = t; idx < nq * D; idx += THREADS) {
-        const int qh = idx / D, d = idx % D;
-        float m = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < WAVES; ++i) m = fmaxf(m, sm[i * QPAD + qh]);
-        const float ref = m == -INFINITY ? 0.0f : m;
-        float o = 0.0f, l = 0.0f;
-#pragma unroll
-        for (int i = 0; i < WAVES; ++i) {
-            const float wgt = fast_exp2(sm[i * QPAD + qh] - ref);       // of a wave that saw no row: 0, and so are its sums
-            o += so[((size_t)i * nq + qh) * D + d] * wgt;
-            l += sl[i * QPAD + qh] * wgt;
-        }
-        o *= v_scale;
-        if (piece.splits == 1) {
-            a.o[(head0 + qh) * D + d] = (uint16_t)(pack_bf16(l == 0.0f ? 0.0f : o / l, 0.0f) & 0xffffu);
-            if (d == 0 && a.lse) a.lse[head0 + qh] = l == 0.0f ? -INFINITY : logf(l) + m * LN2;
-        } else {
-            const size_t at_part = (size_t)blockIdx.x * per + qh;
-            a.part_o[at_part * D + d] = o;
-            if (d == 0) { a.part_m[at_part] = m; a.part_l[at_part] = l; }
-        }
-    }
+    finish(now, now_last);
 }
 
 // Joins the pieces of a sequence: one workgroup per (sequence, query head), D/4 threads of 4 elements a piece, several side by side.
@@ -326,11 +408,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged::Args a) {
     __shared__ float sm[CG], sl[CG];
     const int b = blockIdx.x / (unsigned)a.Hq, qh = blockIdx.x % (unsigned)a.Hq;
     const int2 plan = a.plan[b];
-    const int S = plan.y;
+    const int share = a.plan[a.B].x;
+    const int kvh = qh / a.G, inner = qh % a.G, hb = kvh * a.blocks + inner / 16, per = min(16, a.G);
+    // the waves that had a part of this head's steps
+    const int first = plan.x + hb * (plan.y + TURN), w0 = first / share, S = (first + plan.y - 1) / share - w0 + 1;
     if (S < 2) return;
     const int t = threadIdx.x, c = t % TPS, sg = t / TPS;
-    const int kvh = qh / a.G, inner = qh % a.G, hb = kvh * a.blocks + inner / 16, per = min(16, a.G), heads = a.Hkv * a.blocks;
-    const size_t slot0 = ((size_t)plan.x * heads + hb) * per + inner % 16, pitch = (size_t)heads * per;
+    // of the first wave: the head that goes on behind it; of the others the one that began before them
+    auto slot_of = [&](int i) { return (size_t)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * per + inner % 16; };
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.0f;
     for (int s0 = sg; s0 < S; s0 += 4 * CG) {
@@ -338,7 +423,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged::Args a) {
         float ms[4], ls[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const size_t slot = slot0 + min(s0 + i * CG, S - 1) * pitch;
+            const size_t slot = slot_of(min(s0 + i * CG, S - 1));
             ms[i] = s0 + i * CG < S ? a.part_m[slot] : -INFINITY;
             ls[i] = a.part_l[slot];
             os[i] = *reinterpret_cast<const f32x4*>(a.part_o + slot * D + 4 * c);
@@ -453,51 +538,55 @@ __global__ __launch_bounds__(256) void paged_rope_append_kernel(const paged::App
 
 // ------------------------------------------------------------------------------------------
 namespace {
-struct Grid { int heads, per, target; uint64_t pieces; };      // blocks of heads; heads of a slot; 0 = a piece a sequence; workgroups
-Grid paged_grid(int64_t B, int Hq, int Hkv, int64_t cap) {
+struct Grid { int heads, per, shares; uint64_t waves; };      // kv heads times blocks of 16 query heads; heads of a slot; waves of the launch
+Grid paged_grid(int64_t B, int Hq, int Hkv, int64_t cap, int64_t window, int64_t sinks) {
+    using namespace paged;
     const int G = Hq / Hkv, heads = Hkv * ((G + 15) / 16);
-    // sequences that cannot be longer than one piece are not cut (and not joined)
-    const int target = cap <= paged::MIN_CHUNK * paged::TILE ? 0 : paged::TARGET;
-    return {heads, G < 16 ? G : 16, target, (uint64_t)B * heads + target};
+    // a window and the sinks may each begin and end inside a tile
+    const int64_t rows = window > 0 ? std::min(cap, window + 2 * TILE + sinks + 2 * TILE) : cap;
+    const int64_t steps = std::max<int64_t>(1, (rows + STEP - 1) / STEP);
+    Grid g{heads, std::min(G, 16), 0, (uint64_t)B * heads};
+    if (steps > WHOLE) {
+        g.waves = (uint64_t)std::min<int64_t>(SHARES, (B * heads * (steps + TURN) + MIN_SHARE - 1) / MIN_SHARE);
+        g.shares = (int)g.waves;
+    }
+    return g;
 }
 }  // namespace
 
-uint64_t paged_decode_workgroups(int B, int Hq, int Hkv, int64_t cap) { return paged_grid(B, Hq, Hkv, cap).pieces; }
-
 size_t paged_decode_workspace_bytes(int B, int Hq, int Hkv, int D, int64_t cap) {
-    const Grid g = paged_grid(B, Hq, Hkv, cap);
-    if (!g.target) return 0;
-    return (size_t)g.pieces * g.per * (D + 2) * sizeof(float) + ((size_t)B * sizeof(int2) + 15) / 16 * 16;
+    const Grid g = paged_grid(B, Hq, Hkv, cap, 0, 0);       // with a window there are as many waves at most
+    if (!g.shares) return 0;
+    return (size_t)g.waves * 2 * g.per * (D + 2) * sizeof(float) + ((size_t)(B + 1) * sizeof(int2) + 15) / 16 * 16;
 }
 
 int launch_paged_decode(const void* q, const void* k_pages, const void* v_pages, const int* page_table, const int* kv_lens,
                         const float* k_scale, const float* v_scale, void* o, float* lse, int B, int Hq, int Hkv, int D, int pages,
                         int page_size, int width, int window, int sinks, int e4m3, float scale, void* workspace, hipStream_t stream) {
     using namespace paged;
-    const Grid g = paged_grid(B, Hq, Hkv, (int64_t)width * page_size);
+    const Grid g = paged_grid(B, Hq, Hkv, (int64_t)width * page_size, window, sinks);
     Args a{};
     a.q = static_cast<const uint16_t*>(q);
     a.k = k_pages, a.v = v_pages;
     a.table = page_table, a.kv_lens = kv_lens;
     a.k_scale = k_scale, a.v_scale = v_scale;
     a.o = static_cast<uint16_t*>(o), a.lse = lse;
-    if (g.target) {
+    if (g.shares) {
         a.plan = static_cast<int2*>(workspace);
-        a.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + ((size_t)B * sizeof(int2) + 15) / 16 * 16);
-        a.part_m = a.part_o + (size_t)g.pieces * g.per * D;
-        a.part_l = a.part_m + (size_t)g.pieces * g.per;
+        a.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + ((size_t)(B + 1) * sizeof(int2) + 15) / 16 * 16);
+        a.part_m = a.part_o + (size_t)g.waves * 2 * g.per * D;
+        a.part_l = a.part_m + (size_t)g.waves * 2 * g.per;
     }
     a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv, a.blocks = (a.G + 15) / 16;
     a.width = width, a.page_tiles = page_size / TILE, a.pages = pages;
-    a.cap = width * page_size, a.window = window, a.sinks = sinks, a.target = g.target;
+    a.cap = width * page_size, a.window = window, a.sinks = sinks, a.shares = g.shares;
     a.scale_log2 = scale * LOG2E;
-    const size_t lds = (size_t)(WAVES * g.per * D + 2 * WAVES * QPAD) * sizeof(float);       // at most 33 KB
-    const dim3 grid((unsigned)g.pieces);
+    const dim3 grid((unsigned)((g.waves + WAVES - 1) / WAVES));
     auto kernel = D == 128 ? (e4m3 ? &paged_decode_kernel<128, true> : &paged_decode_kernel<128, false>)
                            : (e4m3 ? &paged_decode_kernel<64, true> : &paged_decode_kernel<64, false>);
-    launch_kernel(kernel, grid, dim3(THREADS), lds, stream, a);
+    launch_kernel(kernel, grid, dim3(THREADS), 0, stream, a);
     if (hipGetLastError() != hipSuccess) return -1;
-    if (!g.target) return 0;
+    if (!g.shares) return 0;
     launch_kernel(D == 128 ? &paged_join_kernel<128> : &paged_join_kernel<64>, dim3((unsigned)((size_t)B * Hq)), dim3(256), 0, stream, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
