@@ -34,6 +34,11 @@ __device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
     return v;
 }
 
+// Stores go past the caches where the launch's bytes fit the last-level cache, whose lines the next launch then finds (CACHED; 35552 x 128
+// 4.5 us with plain stores, 3.8 so), and through them where they do not (65536 x 1024 87 us past them, 79 so).
+template <bool CACHED>
+__device__ __forceinline__ void st_stream_16(void* p, u32x4 v) { if (CACHED) st_global_16_nt(p, v); else st_global_16(p, v); }
+
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
@@ -53,6 +58,20 @@ __device__ __forceinline__ float over_lanes(float x, F op) {
 struct Add { __device__ __forceinline__ float operator()(float a, float b) const { return a + b; } };
 struct Max { __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); } };
 
+// Rows as a buffer of `bytes` bytes.  Reads beyond it give 0 and writes beyond it are dropped, without a branch: behind a branch the
+// compiler no longer knows which loads and stores are under way and waits for all of them.
+constexpr int NOWHERE = 0x40000000, NT = 2;                     // an offset beyond every buffer; cache policy: not kept
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint16_t* p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t*>(p), 0, bytes, 0x00020000);
+}
+template <bool CACHED>
+__device__ __forceinline__ u32x4 load_row_16(__amdgpu_buffer_rsrc_t rows, int at) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, at, 0, CACHED ? 0 : NT));
+}
+template <bool CACHED>
+__device__ __forceinline__ void store_row_16(__amdgpu_buffer_rsrc_t rows, int at, u32x4 v) {
+    __builtin_amdgcn_raw_buffer_store_b128(v, rows, at, 0, CACHED ? NT : 0);
+}
 // How a row lies on the lanes: LPR lanes of a wave hold it alone (64 / LPR rows a wave), or WPR waves of 64 lanes share it; a lane
 // holds P pieces of 8 elements, piece number lane + LPR * (wave + WPR * p).
 template <int LPR_, int WPR_, int P_>
@@ -98,7 +117,7 @@ __global__ __launch_bounds__(S::THREADS) void rmsnorm_residual_kernel(
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] += h[p][i];
             const u32x4 r16 = pack8(f);
-            st_global_16_nt(out_resid + at + pc * 8, r16);
+            st_stream_16<CACHED>(out_resid + at + pc * 8, r16);
             unpack8(r16, h[p]);
         }
         float wf[8];
@@ -142,123 +161,152 @@ __global__ __launch_bounds__(S::THREADS) void rmsnorm_residual_kernel(
             float o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = h[p][i] * rho;
-            st_global_16_nt(static_cast<uint16_t*>(out) + at + pc * 8, pack8(o));
+            st_stream_16<CACHED>(static_cast<uint16_t*>(out) + at + pc * 8, pack8(o));
         }
     }
 }
 
-// Gradients.  Workgroup i takes the row groups i, i + gridDim.x, ... and keeps dw of its rows in registers; rows that share a
-// workgroup are added through LDS at its end, and it writes one row of part [gridDim.x][d_model].
+// Gradients.  Workgroups of 16 waves: as many row slots as fit, slot s of workgroup i takes the rows ROWS (i + k gridDim.x) + s, the
+// next one's loads under way while it works on one, and keeps dw of its rows in registers.  The slots are added through LDS at the
+// end, half of them to the other half at a time, and the workgroup writes one row of part [gridDim.x][d_model].
+// 65536 x 1024 83 us of reading and writing 537 MB and 4 us for the parts; 2000 x 4096 12.5 and 3.  (1024 workgroups of four waves: 91 and
+// 14 and as much again for their parts; with two pieces a lane, spilling: 90 and 14; 512 workgroups: 86 and 15.)
 template <class S, bool CACHED, bool RESID>
-__global__ __launch_bounds__(S::THREADS) void rmsnorm_residual_bwd_kernel(
+__global__ __launch_bounds__(1024) void rmsnorm_residual_bwd_kernel(
     const uint16_t* __restrict__ d_out, const uint16_t* __restrict__ d_resid, const uint16_t* __restrict__ resid,
     const uint16_t* __restrict__ weight, uint16_t* __restrict__ dx, float* __restrict__ dw_part, size_t rows, int d_model, float eps) {
     using namespace rms;
-    constexpr int LPR = S::LPR, WPR = S::WPR, P = S::P;
-    __shared__ float2 part[2][S::ROWS][WPR];
-    extern __shared__ __attribute__((aligned(16))) float sums[];   // [ROWS][d_model], where a workgroup holds several rows
+    constexpr int LPR = S::LPR, WPR = S::WPR, P = S::P, ROWS = 1024 / (LPR * WPR);
+    __shared__ float2 part[2][ROWS][WPR];
+    extern __shared__ __attribute__((aligned(16))) float sums[];   // [ROWS / 2][d_model]
     const int lane = threadIdx.x % LPR, wave = threadIdx.x / 64, wr = wave % WPR;
     const int slot = WPR > 1 ? wave / WPR : threadIdx.x / LPR;
     const int all = d_model / 8;
+    int pc[P], at[P];                                            // this lane's elements of a row; their place in a group of rows
+    bool has[P];
+    constexpr bool TIGHT = P > 1;                                // registers for the rows as they came only
     float w[P][8], dw[P][8];
+    u32x4 w16[P];
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-        const int pc = lane + LPR * (wr + WPR * p);
-        u32x4 v = {0, 0, 0, 0};
-        if (pc < all) v = ld_global_16(weight + pc * 8);
-        unpack8(v, w[p]);
+        pc[p] = 8 * (lane + LPR * (wr + WPR * p));
+        has[p] = pc[p] < d_model;
+        at[p] = has[p] ? 2 * (slot * d_model + pc[p]) : NOWHERE;
+        w16[p] = has[p] ? ld_global_16(weight + pc[p]) : u32x4{0, 0, 0, 0};
+        unpack8(w16[p], w[p]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dw[p][i] = 0.0f;
     }
-    int turn = 0;
-    for (size_t first = (size_t)blockIdx.x * S::ROWS; first < rows; first += (size_t)gridDim.x * S::ROWS, turn ^= 1) {
-        const size_t row = first + slot;
-        const int pieces = row < rows ? all : 0;
-        const size_t at = row * d_model;
-        u32x4 g16[P], h16[P], r16[P];
+    // A group of ROWS rows is a buffer: what lies behind the last row is read as 0 and not written.
+    struct Row { u32x4 g[P], h[P], r[P]; };
+    auto group = [&](const uint16_t* x, size_t first) {
+        const size_t n = first < rows ? (rows - first < (size_t)ROWS ? rows - first : (size_t)ROWS) : 0;
+        return rows_rsrc(x + first * d_model, (int)n * d_model * 2);
+    };
+    auto read = [&](Row& o, size_t first) {
+        const auto g = group(d_out, first), h = group(resid, first), r = group(RESID ? d_resid : resid, first);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int pc = lane + LPR * (wr + WPR * p);
-            g16[p] = h16[p] = r16[p] = u32x4{0, 0, 0, 0};
-            if (pc < pieces) {
-                g16[p] = ld_stream_16<CACHED>(d_out + at + pc * 8);
-                h16[p] = ld_stream_16<CACHED>(resid + at + pc * 8);
-                if constexpr (RESID) r16[p] = ld_stream_16<CACHED>(d_resid + at + pc * 8);
-            }
+            o.h[p] = load_row_16<CACHED>(h, at[p]);
+            o.g[p] = load_row_16<CACHED>(g, at[p]);
+            if constexpr (RESID) o.r[p] = load_row_16<CACHED>(r, at[p]);
         }
-        float sq = 0.0f, gh = 0.0f;
+    };
+    int turn = 0;
+    // unpacks a second time what is to be kept in its 16 bits between
+    auto again = [](u32x4 v, float (&f)[8]) {
+        asm volatile("" : "+v"(v));
+        unpack8(v, f);
+    };
+    auto work = [&](const Row& o, size_t first) {
+        float sq = 0.0f, gwh = 0.0f, g[P][8], h[P][8], gh[P][8];
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            float g[8], h[8];
-            unpack8(g16[p], g);
-            unpack8(h16[p], h);
+            unpack8(o.g[p], g[p]);
+            unpack8(o.h[p], h[p]);
+            if constexpr (TIGHT) again(w16[p], w[p]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                sq += h[i] * h[i];
-                gh += g[i] * w[p][i] * h[i];
+                sq += h[p][i] * h[p][i];
+                gh[p][i] = g[p][i] * h[p][i];
+                gwh += gh[p][i] * w[p][i];
             }
         }
         sq = over_lanes<LPR>(sq, Add{});
-        gh = over_lanes<LPR>(gh, Add{});
+        gwh = over_lanes<LPR>(gwh, Add{});
         if constexpr (WPR > 1) {
             // two sets of sums in turn: a wave that is already at the next row writes the other one
-            if (lane == 0) part[turn][slot][wr] = float2{sq, gh};
+            if (lane == 0) part[turn][slot][wr] = float2{sq, gwh};
             __syncthreads();
-            sq = gh = 0.0f;
+            sq = gwh = 0.0f;
 #pragma unroll
-            for (int i = 0; i < WPR; ++i) { sq += part[turn][slot][i].x; gh += part[turn][slot][i].y; }
+            for (int i = 0; i < WPR; ++i) { sq += part[turn][slot][i].x; gwh += part[turn][slot][i].y; }
+            turn ^= 1;
         }
-        const float rho = rsqrtf(sq / (float)d_model + eps);
-        const float c = rho * rho * rho * (gh / (float)d_model);
+        const float rho = first + slot < rows ? rsqrtf(sq / (float)d_model + eps) : 0.0f;
+        const float c = rho * rho * rho * (gwh / (float)d_model);
+        const auto to = group(dx, first);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const int pc = lane + LPR * (wr + WPR * p);
-            if (pc >= pieces) continue;
-            float g[8], h[8], r[8], o[8];
-            unpack8(g16[p], g);
-            unpack8(h16[p], h);
-            if constexpr (RESID) unpack8(r16[p], r);
+            float r[8], o8[8];
+            if constexpr (RESID) unpack8(o.r[p], r);
+            if constexpr (TIGHT) {
+                again(o.g[p], g[p]);
+                again(o.h[p], h[p]);
+                again(w16[p], w[p]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) gh[p][i] = g[p][i] * h[p][i];
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                o[i] = rho * (g[i] * w[p][i]) - c * h[i];
-                if constexpr (RESID) o[i] += r[i];
-                dw[p][i] += g[i] * (h[i] * rho);
+                const float gw = g[p][i] * w[p][i];
+                o8[i] = fmaf(-c, h[p][i], RESID ? fmaf(rho, gw, r[i]) : rho * gw);
+                dw[p][i] = fmaf(gh[p][i], rho, dw[p][i]);
             }
-            st_global_16_nt(dx + at + pc * 8, pack8(o));
+            store_row_16<CACHED>(to, at[p], pack8(o8));
         }
+    };
+    const size_t stride = (size_t)gridDim.x * ROWS;
+    Row now, next;
+    read(now, (size_t)blockIdx.x * ROWS);
+    for (size_t first = (size_t)blockIdx.x * ROWS; first < rows; first += stride) {      // the same for all slots: they meet at barriers
+        read(next, first + stride);
+        work(now, first);
+        now = next;
     }
-    float* to = dw_part + (size_t)blockIdx.x * d_model;
-    if constexpr (S::ROWS > 1) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            const int pc = lane + LPR * (wr + WPR * p);
-            if (pc < all) {
-                f32x4* s = reinterpret_cast<f32x4*>(sums + (size_t)slot * d_model + pc * 8);
-                s[0] = f32x4{dw[p][0], dw[p][1], dw[p][2], dw[p][3]};
-                s[1] = f32x4{dw[p][4], dw[p][5], dw[p][6], dw[p][7]};
-            }
-        }
+    for (int half = ROWS / 2; half > 0; half /= 2) {
         __syncthreads();
-        for (int i = threadIdx.x; i < d_model / 4; i += S::THREADS) {
-            f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (slot >= half && slot < 2 * half)
 #pragma unroll
-            for (int r = 0; r < S::ROWS; ++r) v += *reinterpret_cast<const f32x4*>(sums + (size_t)r * d_model + 4 * i);
-            *reinterpret_cast<f32x4*>(to + 4 * i) = v;
-        }
-    } else {
+            for (int p = 0; p < P; ++p)
+                if (has[p]) {
+                    f32x4* s = reinterpret_cast<f32x4*>(sums + (size_t)(slot - half) * d_model + pc[p]);
+                    s[0] = f32x4{dw[p][0], dw[p][1], dw[p][2], dw[p][3]};
+                    s[1] = f32x4{dw[p][4], dw[p][5], dw[p][6], dw[p][7]};
+                }
+        __syncthreads();
+        if (slot < half)
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            const int pc = lane + LPR * (wr + WPR * p);
-            if (pc < all) {
-                f32x4* s = reinterpret_cast<f32x4*>(to + pc * 8);
+            for (int p = 0; p < P; ++p)
+                if (has[p]) {
+                    const f32x4* s = reinterpret_cast<const f32x4*>(sums + (size_t)slot * d_model + pc[p]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dw[p][i] += s[i / 4][i % 4];
+                }
+    }
+    if (slot == 0)
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+            if (has[p]) {
+                f32x4* s = reinterpret_cast<f32x4*>(dw_part + (size_t)blockIdx.x * d_model + pc[p]);
                 s[0] = f32x4{dw[p][0], dw[p][1], dw[p][2], dw[p][3]};
                 s[1] = f32x4{dw[p][4], dw[p][5], dw[p][6], dw[p][7]};
             }
-        }
-    }
 }
 
-// dw = sum of the parts: 8 threads of 4 columns, 32 parts at once, joined through LDS.
+// dw = sum of the parts: 8 threads of 4 columns, 32 parts at once, joined through LDS.  It is all latency (1024 threads for 128
+// parts at once take as long).
 __global__ __launch_bounds__(256) void rmsnorm_dweight_kernel(const float* __restrict__ part, uint16_t* __restrict__ dw, int parts, int d_model) {
     __shared__ f32x4 sums[32][8];
     const int c = threadIdx.x % 8, g = threadIdx.x / 8;
@@ -271,6 +319,7 @@ __global__ __launch_bounds__(256) void rmsnorm_dweight_kernel(const float* __res
     sums[g][c] = v;
     __syncthreads();
     if (g == 0 && col < d_model) {
+#pragma unroll
         for (int i = 1; i < 32; ++i) v += sums[i][c];
         st_global_8(dw + col, u32x2{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])});
     }
@@ -278,6 +327,20 @@ __global__ __launch_bounds__(256) void rmsnorm_dweight_kernel(const float* __res
 
 // ------------------------------------------------------------------------------------------
 namespace {
+// Of the backward: one piece a lane, whose values, weights and sums fill the registers, as long as 16 waves hold a row so.
+template <class F>
+void with_bwd_shape(int d_model, F go) {
+    using namespace rms;
+    if (d_model <= 64) go(Shape<8, 1, 1>{});
+    else if (d_model <= 128) go(Shape<16, 1, 1>{});
+    else if (d_model <= 256) go(Shape<32, 1, 1>{});
+    else if (d_model <= 512) go(Shape<64, 1, 1>{});
+    else if (d_model <= 1024) go(Shape<64, 2, 1>{});
+    else if (d_model <= 2048) go(Shape<64, 4, 1>{});
+    else if (d_model <= 4096) go(Shape<64, 8, 1>{});
+    else if (d_model <= 8192) go(Shape<64, 16, 1>{});
+    else go(Shape<64, 16, 2>{});
+}
 template <class F>
 void with_shape(int d_model, F go) {
     using namespace rms;
@@ -295,8 +358,9 @@ void with_shape(int d_model, F go) {
 // workgroups of a backward: parts of dw
 template <class S>
 size_t bwd_parts(size_t rows) {
-    const size_t groups = (rows + S::ROWS - 1) / S::ROWS;
-    return groups < 1024 ? groups : 1024;
+    constexpr int ROWS = 1024 / (S::LPR * S::WPR);
+    const size_t groups = (rows + ROWS - 1) / ROWS;
+    return groups < 256 ? groups : 256;
 }
 }  // namespace
 
@@ -321,7 +385,7 @@ int launch_rmsnorm_residual(const void* x, const void* residual, const void* wei
 
 size_t rmsnorm_residual_bwd_workspace_bytes(size_t rows, int d_model) {
     size_t parts = 0;
-    with_shape(d_model, [&](auto shape) { parts = bwd_parts<decltype(shape)>(rows); });
+    with_bwd_shape(d_model, [&](auto shape) { parts = bwd_parts<decltype(shape)>(rows); });
     return parts * d_model * sizeof(float);
 }
 
@@ -329,12 +393,12 @@ int launch_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const vo
                                 size_t rows, int d_model, float eps, void* workspace, hipStream_t stream) {
     const bool cached = rows * d_model * (d_resid ? 8 : 6) <= kStreamCached;
     size_t parts = 0;
-    with_shape(d_model, [&](auto shape) {
+    with_bwd_shape(d_model, [&](auto shape) {
         using S = decltype(shape);
         parts = bwd_parts<S>(rows);
-        const size_t lds = S::ROWS > 1 ? (size_t)S::ROWS * d_model * sizeof(float) : 0;
+        const size_t lds = (size_t)(512 / (S::LPR * S::WPR)) * d_model * sizeof(float);        // at most 32 KB
         auto go = [&](auto in_cache, auto with_resid) {
-            launch_kernel((rmsnorm_residual_bwd_kernel<S, in_cache(), with_resid()>), dim3((unsigned)parts), dim3(S::THREADS), lds, stream,
+            launch_kernel((rmsnorm_residual_bwd_kernel<S, in_cache(), with_resid()>), dim3((unsigned)parts), dim3(1024), lds, stream,
                           static_cast<const uint16_t*>(d_out), static_cast<const uint16_t*>(d_resid), static_cast<const uint16_t*>(resid),
                           static_cast<const uint16_t*>(weight), static_cast<uint16_t*>(dx), static_cast<float*>(workspace), rows, d_model, eps);
         };
