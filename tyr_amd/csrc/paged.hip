@@ -482,57 +482,67 @@ __device__ __forceinline__ void rotate8(float (&x1)[8], float (&x2)[8], const fl
 }
 }  // namespace paged
 
-// One thread takes 8 elements of each half of one head of one token; heads of a token: Hq of q, Hkv of k, Hkv of v.
+// One thread takes 8 elements of each half of one head of one token; heads of a token: Hq of q, Hkv of k, Hkv of v.  What bounds it is
+// memory, and where little is moved the chain position -> page -> store; the elements are asked for before it begins.  (Several heads a
+// thread, so that the rotary table's 64 bytes and the page are looked up once for all: 2222 tokens of 48 heads 12.3 us, 13.1 with
+// two heads, 16.5 with four.)
 template <bool FP8>
 __global__ __launch_bounds__(256) void paged_rope_append_kernel(const paged::AppendArgs a) {
     using namespace paged;
     const uint32_t id = blockIdx.x * 256u + threadIdx.x;
     if (id >= a.threads) return;
     const unsigned per_head = a.D / 16, per_token = (a.Hq + 2 * a.Hkv) * per_head;
-    const unsigned token = id / per_token, rest = id - token * per_token, head = rest / per_head;
+    const unsigned token = id / per_token, rest = id - token * per_token;
+    unsigned head = rest / per_head;
     const int e0 = (int)(rest - head * per_head) * 8, half = a.D / 2;
     const int b = (int)(token / (unsigned)a.T), step = (int)(token - (unsigned)b * a.T);
-    const int first = a.positions[b];
-    const int64_t pos = (int64_t)first + step;
-    const bool rotated = first >= 0 && pos < a.rope_rows;
-    const int hk = (int)head - a.Hq;                       // < 0: a query head; < Hkv: of k; else of v
-    const uint16_t* src = hk < 0 ? a.q + ((size_t)token * a.Hq + head) * a.D
-                          : hk < a.Hkv ? a.k_new + ((size_t)token * a.Hkv + hk) * a.D : a.v_new + ((size_t)token * a.Hkv + hk - a.Hkv) * a.D;
-    const u32x4 lo = ld_global_16(src + e0), hi = ld_global_16(src + half + e0);
+    const int kind = head < (unsigned)a.Hq ? 0 : head < (unsigned)(a.Hq + a.Hkv) ? 1 : 2;     // q, k, v
+    const unsigned heads = kind ? a.Hkv : a.Hq;
+    head -= kind ? a.Hq + (kind - 1) * a.Hkv : 0;
+    const uint16_t* src = (kind == 0 ? a.q : kind == 1 ? a.k_new : a.v_new) + ((size_t)token * heads + head) * a.D + e0;
+    const u32x4 lo = ld_global_16(src), hi = ld_global_16(src + half);
+    const int first = a.positions[b], lens = a.new_lens ? a.new_lens[b] : a.T;
+    const bool placed = first >= 0 && (int64_t)first + step < a.rope_rows;
+    const unsigned pos = (unsigned)first + step;
     float x1[8], x2[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         x1[2 * i] = bf16_lo(lo[i]), x1[2 * i + 1] = bf16_hi(lo[i]);
         x2[2 * i] = bf16_lo(hi[i]), x2[2 * i + 1] = bf16_hi(hi[i]);
     }
-    if (rotated && hk < a.Hkv) rotate8(x1, x2, a.cos + (size_t)pos * half + e0, a.sin + (size_t)pos * half + e0);
+    if (kind < 2 && placed) rotate8(x1, x2, a.cos + (size_t)pos * half + e0, a.sin + (size_t)pos * half + e0);
     auto pack = [](const float (&f)[8]) { return u32x4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])}; };
-    if (hk < 0) {
-        uint16_t* to = a.q_out + ((size_t)token * a.Hq + head) * a.D + e0;
-        st_global_16(to, rotated ? pack(x1) : u32x4{0, 0, 0, 0});
-        st_global_16(to + half, rotated ? pack(x2) : u32x4{0, 0, 0, 0});
+    if (kind == 0) {
+        uint16_t* to = a.q_out + ((size_t)token * heads + head) * a.D + e0;
+        st_global_16_nt(to, placed ? pack(x1) : u32x4{0, 0, 0, 0});
+        st_global_16_nt(to + half, placed ? pack(x2) : u32x4{0, 0, 0, 0});
         return;
     }
-    if (!rotated || (a.new_lens && step >= a.new_lens[b])) return;
-    const int64_t page = pos / a.page_size;
-    if (page >= a.width) return;
+    if (!placed || step >= lens) return;
+    const unsigned page = pos / (unsigned)a.page_size;
+    if (page >= (unsigned)a.width) return;
     const int entry = a.table[(size_t)b * a.width + page];
     if (entry < 0 || entry >= a.pages) return;
-    const bool is_v = hk >= a.Hkv;
-    const int kvh = is_v ? hk - a.Hkv : hk;
-    const size_t at = (((size_t)entry * a.Hkv + kvh) * a.page_size + (size_t)(pos - page * a.page_size)) * a.D + e0;
-    void* pool = is_v ? a.v_pages : a.k_pages;
+    const size_t at = (((size_t)entry * a.Hkv + head) * a.page_size + (pos - page * a.page_size)) * a.D + e0;
+    void* pool = kind == 2 ? a.v_pages : a.k_pages;
     if constexpr (FP8) {
-        const float* scales = is_v ? a.v_scale : a.k_scale;
-        const float s = scales ? scales[kvh] : 1.0f;
-        auto pack8 = [s](const float (&f)[8]) {
-            return u32x2{pack_e4m3(f32x4{f[0] / s, f[1] / s, f[2] / s, f[3] / s}), pack_e4m3(f32x4{f[4] / s, f[5] / s, f[6] / s, f[7] / s})};
+        const float* scales = kind == 2 ? a.v_scale : a.k_scale;
+        const float f = scales ? scales[head] : 1.0f;
+        // x / f, rounded as a division is: the product with the rounded reciprocal, and what it left, once more (infinite ones stay);
+        // 16 divisions took 1 us of 11
+        const float rf = 1.0f / f;
+        auto over = [f, rf](float x) {
+            const float y = x * rf;
+            return fabsf(y) < INFINITY ? fmaf(fmaf(-y, f, x), rf, y) : y;
+        };
+        auto pack8 = [over](const float (&x)[8]) {
+            return u32x2{pack_e4m3(f32x4{over(x[0]), over(x[1]), over(x[2]), over(x[3])}), pack_e4m3(f32x4{over(x[4]), over(x[5]), over(x[6]), over(x[7])})};
         };
         st_global_8(static_cast<uint8_t*>(pool) + at, pack8(x1));
         st_global_8(static_cast<uint8_t*>(pool) + at + half, pack8(x2));
     } else {
-        st_global_16(static_cast<uint16_t*>(pool) + at, pack(x1));
-        st_global_16(static_cast<uint16_t*>(pool) + at + half, pack(x2));
+        st_global_16_nt(static_cast<uint16_t*>(pool) + at, pack(x1));
+        st_global_16_nt(static_cast<uint16_t*>(pool) + at + half, pack(x2));
     }
 }
 
@@ -598,7 +608,8 @@ int launch_paged_rope_append(const void* q, const void* k_new, const void* v_new
     paged::AppendArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_new), static_cast<const uint16_t*>(v_new), cosp, sinp,
                         static_cast<uint16_t*>(q_out), k_pages, v_pages, page_table, positions, new_lens, k_scale, v_scale,
                         T, Hq, Hkv, D, pages, page_size, width, rope_rows, (uint32_t)((uint64_t)B * T * (Hq + 2 * Hkv) * (D / 16))};
-    launch_kernel(e4m3 ? &paged_rope_append_kernel<true> : &paged_rope_append_kernel<false>, dim3((a.threads + 255u) / 256u), dim3(256), 0, stream, a);
+    auto kernel = e4m3 ? &paged_rope_append_kernel<true> : &paged_rope_append_kernel<false>;
+    launch_kernel(kernel, dim3((a.threads + 255u) / 256u), dim3(256), 0, stream, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
