@@ -28,7 +28,9 @@
 namespace tyr {
 
 namespace paged {
-constexpr int TILE = 16, STEP = 2 * TILE, WAVES = 4, THREADS = 64 * WAVES;
+constexpr int TILE = 16, STEP = 2 * TILE;
+constexpr int WAVES = 1, THREADS = 64 * WAVES;      // of one wave, a launch with few waves has them on as many CUs (one sequence of 1500
+                                            // rows 10.2 us with four, 8.8 so)
 constexpr int SHARES = 1024;                // waves that share a launch's steps: one on every SIMD of 256 CUs
 constexpr int MIN_SHARE = 2;                // steps of a wave at least
 constexpr int WHOLE = 4;                    // sequences of so many steps at most are not cut
@@ -226,7 +228,6 @@ __global__ __launch_bounds__(paged::THREADS, 1) void paged_decode_kernel(const p
     struct Slot { Buf<D, FP8> buf; uint32_t seen[2]; int b, hb, first, last; bool live; };
     Run run = locate(), then;
     then.steps = 0;
-    if (next_at < end) then = locate();
     int s = 0;                                       // step of the run to load next
     auto load = [&](Slot& o) {
         if (s >= run.steps) {
@@ -384,10 +385,12 @@ __global__ __launch_bounds__(paged::THREADS, 1) void paged_decode_kernel(const p
         }
     };
 
-    begin(b, hb);
     Slot slots[DEEP];
+    load(slots[0]);
+    begin(b, hb);
+    if (next_at < end) then = locate();
 #pragma unroll
-    for (int i = 0; i < DEEP - 1; ++i) load(slots[i]);
+    for (int i = 1; i < DEEP - 1; ++i) load(slots[i]);
     for (bool more = true; more;) {
 #pragma unroll
         for (int i = 0; i < DEEP && more; ++i) {
@@ -399,7 +402,8 @@ __global__ __launch_bounds__(paged::THREADS, 1) void paged_decode_kernel(const p
     finish(now, now_last);
 }
 
-// Joins the pieces of a sequence: one workgroup per (sequence, query head), D/4 threads of 4 elements a piece, several side by side.
+// Joins the parts of a head: one workgroup per (sequence, query head), D/4 threads of 4 elements a part, several side by side.  It is all
+// latency, 3-4 us (m, l and the weights of 64 parts by the lanes of a wave instead, no serial step: as long).
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(const paged::Args a) {
     using namespace paged;
