@@ -12,7 +12,7 @@
 // backward is given.
 //
 // HBM-bound: 8 bytes an element (bf16 with a residual, and the backward), 7 with e4m3 out.  A row is read once and stays in
-// registers between its statistics and its output.
+// registers between its statistics and its output.  Stores go past the caches (plain ones: 65536 x 1024 91.5 us, 87 so; 35552 x 128 4.5, 3.8).
 #include "common.hpp"
 #include "launch.hpp"
 #include <type_traits>
@@ -33,11 +33,6 @@ __device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
     for (int i = 0; i < 4; ++i) v[i] = pack_bf16(f[2 * i], f[2 * i + 1]);
     return v;
 }
-
-// Stores go past the caches where the launch's bytes fit the last-level cache, whose lines the next launch then finds (CACHED; 35552 x 128
-// 4.5 us with plain stores, 3.8 so), and through them where they do not (65536 x 1024 87 us past them, 79 so).
-template <bool CACHED>
-__device__ __forceinline__ void st_stream_16(void* p, u32x4 v) { if (CACHED) st_global_16_nt(p, v); else st_global_16(p, v); }
 
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
@@ -68,9 +63,8 @@ template <bool CACHED>
 __device__ __forceinline__ u32x4 load_row_16(__amdgpu_buffer_rsrc_t rows, int at) {
     return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rows, at, 0, CACHED ? 0 : NT));
 }
-template <bool CACHED>
 __device__ __forceinline__ void store_row_16(__amdgpu_buffer_rsrc_t rows, int at, u32x4 v) {
-    __builtin_amdgcn_raw_buffer_store_b128(v, rows, at, 0, CACHED ? NT : 0);
+    __builtin_amdgcn_raw_buffer_store_b128(v, rows, at, 0, NT);
 }
 // How a row lies on the lanes: LPR lanes of a wave hold it alone (64 / LPR rows a wave), or WPR waves of 64 lanes share it; a lane
 // holds P pieces of 8 elements, piece number lane + LPR * (wave + WPR * p).
@@ -117,7 +111,7 @@ __global__ __launch_bounds__(S::THREADS) void rmsnorm_residual_kernel(
 #pragma unroll
             for (int i = 0; i < 8; ++i) f[i] += h[p][i];
             const u32x4 r16 = pack8(f);
-            st_stream_16<CACHED>(out_resid + at + pc * 8, r16);
+            st_global_16_nt(out_resid + at + pc * 8, r16);
             unpack8(r16, h[p]);
         }
         float wf[8];
@@ -161,7 +155,7 @@ __global__ __launch_bounds__(S::THREADS) void rmsnorm_residual_kernel(
             float o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = h[p][i] * rho;
-            st_stream_16<CACHED>(static_cast<uint16_t*>(out) + at + pc * 8, pack8(o));
+            st_global_16_nt(static_cast<uint16_t*>(out) + at + pc * 8, pack8(o));
         }
     }
 }
@@ -263,7 +257,7 @@ __global__ __launch_bounds__(1024) void rmsnorm_residual_bwd_kernel(
                 o8[i] = fmaf(-c, h[p][i], RESID ? fmaf(rho, gw, r[i]) : rho * gw);
                 dw[p][i] = fmaf(gh[p][i], rho, dw[p][i]);
             }
-            store_row_16<CACHED>(to, at[p], pack8(o8));
+            store_row_16(to, at[p], pack8(o8));
         }
     };
     const size_t stride = (size_t)gridDim.x * ROWS;
