@@ -35,6 +35,8 @@ constexpr int SHARES = 1024;                // waves that share a launch's steps
 constexpr int MIN_SHARE = 2;                // steps of a wave at least
 constexpr int WHOLE = 4;                    // sequences of so many steps at most are not cut
 constexpr int TURN = 3;                     // steps that going from one head to the next is counted as
+constexpr int MANY_HEADS = 64;              // heads of a launch from which one wave joins each, not four (1024 heads of 3-22 steps 40.7 us, 37.4 so;
+                                            // with 8 heads of 128 parts four waves have more of them under way)
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -99,6 +101,12 @@ struct Round {
     __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(upto, 63); }
 };
 
+// A factor that is the same for all lanes, by a scalar load: one more vector load that may be under way at the end of a branch would have the
+// compiler wait there, in every step, for all the rows asked for since.
+__device__ __forceinline__ float factor(const float* scales, int i) {
+    return scales ? *reinterpret_cast<const __attribute__((address_space(4))) float*>(reinterpret_cast<uintptr_t>(scales + i)) : 1.0f;
+}
+
 // What a lane holds of 32 rows.
 template <int D, bool FP8> struct Buf {
     u32x4 k[2][D / 32];                     // [T][i]: row x of tile T, d = 32i + 8g + [0,8)
@@ -132,7 +140,7 @@ __device__ __forceinline__ u32x4 bf16_of_e4m3(uint32_t lo, uint32_t hi) {
 }  // namespace paged
 
 template <int D, bool FP8>
-__global__ __launch_bounds__(paged::THREADS, 1) void paged_decode_kernel(const paged::Args a) {
+__global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const paged::Args a) {
     using namespace paged;
     const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * WAVES + threadIdx.x / 64));
@@ -224,8 +232,7 @@ __global__ __launch_bounds__(paged::THREADS, 1) void paged_decode_kernel(const p
         b = next_b, hb = next_hb, first = next_first;
     }
 
-    constexpr int DEEP = 2;                          // steps whose rows are under way or in use
-    struct Slot { Buf<D, FP8> buf; uint32_t seen[2]; int b, hb, first, last; bool live; };
+    struct Slot { Buf<D, FP8> buf; uint32_t seen[2]; int b, hb, first, last, live; };
     Run run = locate(), then;
     then.steps = 0;
     int s = 0;                                       // step of the run to load next
@@ -236,13 +243,13 @@ __global__ __launch_bounds__(paged::THREADS, 1) void paged_decode_kernel(const p
             then.steps = 0;
             if (next_at < end) then = locate();
         }
-        o.live = run.steps > 0;
+        o.live = __builtin_amdgcn_readfirstlane(run.steps);      // 0: there was no step left
         o.b = run.b, o.hb = run.hb, o.first = run.first, o.last = run.last;
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
             o.seen[T] = (uint32_t)__builtin_amdgcn_readlane((int)run.mask, 2 * s + T);
             const size_t base = (size_t)(uint32_t)__builtin_amdgcn_readlane(run.tile, 2 * s + T) * TILE_BYTES;
-            const int there = o.live && o.seen[T] ? TILE_BYTES : 0;
+            const int there = o.live > 0 && o.seen[T] ? TILE_BYTES : 0;
             const auto k = tile_rsrc(a.k, base, there), v = tile_rsrc(a.v, base, there);
             if constexpr (FP8) {
 #pragma unroll
@@ -278,7 +285,7 @@ __global__ __launch_bounds__(paged::THREADS, 1) void paged_decode_kernel(const p
             if (x >= nq) v = u32x4{0, 0, 0, 0};
             qf[i][lane] = v;
         }
-        scale_log2 = a.scale_log2 * (a.k_scale ? a.k_scale[kvh] : 1.0f);
+        scale_log2 = a.scale_log2 * factor(a.k_scale, kvh);
 #pragma unroll
         for (int i = 0; i < 8; ++i) oacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
         m2 = -INFINITY;
@@ -287,7 +294,7 @@ __global__ __launch_bounds__(paged::THREADS, 1) void paged_decode_kernel(const p
     // The head's steps are done, or this wave's: its result where the wave had all of them, else a partial one.  A wave has at most two
     // heads that it shares with others: one that began before it, and one that goes on behind it.  oacc[i][r] is O^T[d = 32g + 8r + i][x].
     auto finish = [&](int first_, int last_) {
-        const float l = sum_xor32(sum_xor16(lsum)), v_scale = a.v_scale ? a.v_scale[kvh] : 1.0f;
+        const float l = sum_xor32(sum_xor16(lsum)), v_scale = factor(a.v_scale, kvh);
         if (x >= nq || 32 * g >= D) return;
         if (first_ >= at && last_ <= end) {
             const float f = l == 0.0f ? 0.0f : v_scale / l;
@@ -385,20 +392,18 @@ __global__ __launch_bounds__(paged::THREADS, 1) void paged_decode_kernel(const p
         }
     };
 
-    Slot slots[DEEP];
-    load(slots[0]);
+    Slot s0, s1;                                     // the rows of one step are under way while those of the other are in use
+    load(s0);
     begin(b, hb);
     if (next_at < end) then = locate();
-#pragma unroll
-    for (int i = 1; i < DEEP - 1; ++i) load(slots[i]);
-    for (bool more = true; more;) {
-#pragma unroll
-        for (int i = 0; i < DEEP && more; ++i) {
-            load(slots[(i + DEEP - 1) % DEEP]);
-            compute(slots[i]);
-            more = slots[(i + 1) % DEEP].live;
-        }
-    }
+    // One way out, behind both halves' loads: with one between them the compiler would take s1's for the last ones made, and wait for
+    // s0's with them.
+    do {
+        load(s1);
+        compute(s0);
+        load(s0);
+        if (s1.live) compute(s1);
+    } while (s0.live);
     finish(now, now_last);
 }
 
@@ -460,6 +465,65 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged::Args a) {
     const size_t head = (size_t)b * a.Hq + qh;
     reinterpret_cast<u32x2*>(a.o + head * D)[c] = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
     if (a.lse && c == 0) a.lse[head] = l == 0.0f ? -INFINITY : logf(l) + m * LN2;
+}
+
+// The same with a wave a head, for launches of many heads, whose heads have few parts.
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_few_kernel(const paged::Args a) {
+    using namespace paged;
+    constexpr int TPS = D / 4, CG = 64 / TPS;
+    const int id = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + threadIdx.x / 64));
+    const int b = id / a.Hq, qh = id - b * a.Hq;
+    if (b >= a.B) return;
+    const int2 plan = a.plan[b];
+    const int share = a.plan[a.B].x;
+    const int kvh = qh / a.G, inner = qh % a.G, hb = kvh * a.blocks + inner / 16, per = min(16, a.G);
+    const int first = plan.x + hb * (plan.y + TURN), w0 = first / share, S = (first + plan.y - 1) / share - w0 + 1;
+    if (S < 2) return;
+    const int lane = threadIdx.x & 63, c = lane % TPS, sg = lane / TPS;
+    auto slot_of = [&](int i) { return (size_t)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * per + inner % 16; };
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.0f;
+    for (int s0 = 0; s0 < S; s0 += 4 * CG) {
+        f32x4 os[4];
+        float ms[4], ls[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const size_t slot = slot_of(min(s0 + i * CG + sg, S - 1));
+            ms[i] = s0 + i * CG + sg < S ? a.part_m[slot] : -INFINITY;
+            ls[i] = a.part_l[slot];
+            os[i] = *reinterpret_cast<const f32x4*>(a.part_o + slot * D + 4 * c);
+        }
+        const float mn = fmaxf(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), m), ref = mn == -INFINITY ? 0.0f : mn;
+        const float alpha = fast_exp2(m - ref);
+        o *= alpha;
+        l *= alpha;
+        m = mn;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s0 + i * CG + sg < S) {
+                const float wgt = fast_exp2(ms[i] - ref);
+                o += os[i] * wgt;
+                l += ls[i] * wgt;
+            }
+    }
+    // the groups of lanes together
+    float all = max_xor32(m);
+    if constexpr (CG == 4) all = max_xor16(all);
+    const float f = fast_exp2(m - (all == -INFINITY ? 0.0f : all));
+    auto sum = [&](float x) {
+        x = sum_xor32(x * f);
+        if constexpr (CG == 4) x = sum_xor16(x);
+        return x;
+    };
+    l = sum(l);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = sum(o[i]);
+    if (sg != 0) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t head = (size_t)b * a.Hq + qh;
+    reinterpret_cast<u32x2*>(a.o + head * D)[c] = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
+    if (a.lse && c == 0) a.lse[head] = l == 0.0f ? -INFINITY : logf(l) + all * LN2;
 }
 
 // ---- new tokens into the pages ---------------------------------------------------------------
@@ -601,7 +665,11 @@ int launch_paged_decode(const void* q, const void* k_pages, const void* v_pages,
     launch_kernel(kernel, grid, dim3(THREADS), 0, stream, a);
     if (hipGetLastError() != hipSuccess) return -1;
     if (!g.shares) return 0;
-    launch_kernel(D == 128 ? &paged_join_kernel<128> : &paged_join_kernel<64>, dim3((unsigned)((size_t)B * Hq)), dim3(256), 0, stream, a);
+    const size_t heads = (size_t)B * Hq;
+    if ((int64_t)B * g.heads < MANY_HEADS)
+        launch_kernel(D == 128 ? &paged_join_kernel<128> : &paged_join_kernel<64>, dim3((unsigned)heads), dim3(256), 0, stream, a);
+    else
+        launch_kernel(D == 128 ? &paged_join_few_kernel<128> : &paged_join_few_kernel<64>, dim3((unsigned)((heads + 3) / 4)), dim3(256), 0, stream, a);
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 
