@@ -104,6 +104,20 @@ def test_decode_windows_and_sinks(window, sinks, page, e4m3, D):
         assert torch.equal(o, whole[0]) and torch.equal(lse, whole[1])
 
 
+def test_window_beyond_64_bits_is_all_rows():
+    import tyr_amd
+    g = _gen(78)
+    (k, v), table, _, _ = _cache(g, [700], 16, 2, 64, False)
+    lens = torch.tensor([700], dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 4, 1, 64, generator=g, device="cuda").bfloat16()
+    want = tyr_amd.paged_decode(q, k, v, table, lens)
+    for n in (2 ** 31 - 1, 2 ** 63, 2 ** 64 + 5):
+        got = tyr_amd.paged_decode(q, k, v, table, lens, window=n, sinks=n)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(tyr_amd.TyrGpuError, match="negative"):
+        tyr_amd.paged_decode(q, k, v, table, lens, window=-2 ** 70)
+
+
 @pytest.mark.parametrize("e4m3", [False, True])
 def test_what_hidden_rows_hold_does_not_matter(e4m3):
     import tyr_amd
@@ -429,6 +443,45 @@ def test_on_a_side_stream():
         side.synchronize()
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         del junk
+
+
+def test_shared_pages_and_large_ones():
+    """Sequences that share the pages of a common beginning; a page longer than any sequence; one row."""
+    import tyr_amd
+    g = _gen(24)
+    (k, v), table, _, _ = _cache(g, [333, 333], 16, 2, 128, False)
+    table[1, :15] = table[0, :15]
+    lens = torch.tensor([333, 300], dtype=torch.int32, device="cuda")
+    q = torch.randn(2, 8, 1, 128, generator=g, device="cuda").bfloat16()
+    o, lse = tyr_amd.paged_decode(q, k, v, table, lens)
+    _check(o, lse, q, k, v, table, [333, 300], 1 / math.sqrt(128))
+    for e4m3 in (False, True):
+        (k, v), table, ks, vs = _cache(g, [900, 1, 4000], 4096, 2, 64, e4m3, spare=1)
+        lens = torch.tensor([900, 1, 4000], dtype=torch.int32, device="cuda")
+        q = torch.randn(3, 4, 1, 64, generator=g, device="cuda").bfloat16()
+        for window, sinks in ((0, 0), (50, 20)):
+            o, lse = tyr_amd.paged_decode(q, k, v, table, lens, window=window, sinks=sinks, k_scale=ks, v_scale=vs)
+            _check(o, lse, q, k, v, table, [900, 1, 4000], 0.125, window, sinks, ks, vs)
+
+
+def test_calls_at_the_same_time():
+    """Calls of unlike batches on two streams, queued without a wait: each has its own scratch."""
+    import tyr_amd
+    g = _gen(25)
+    work = []
+    for lens_, Hq, Hkv, D, e4m3 in (([9000, 100, 3000], 8, 2, 128, False), ([50, 20000], 16, 1, 64, True)):
+        (k, v), table, ks, vs = _cache(g, lens_, 16, Hkv, D, e4m3)
+        lens = torch.tensor(lens_, dtype=torch.int32, device="cuda")
+        q = torch.randn(len(lens_), Hq, 1, D, generator=g, device="cuda").bfloat16()
+        work.append(lambda s=None, a=(q, k, v, table, lens), f=(ks, vs): tyr_amd.paged_decode(*a, k_scale=f[0], v_scale=f[1], stream=s))
+    want = [f() for f in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    got = [[f(s) for f, s in zip(work, streams)] for _ in range(20)]
+    torch.cuda.synchronize()
+    for round_ in got:
+        for a, b in zip(round_, want):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
 def test_refusals():

@@ -44,7 +44,8 @@ def test_paged_decode():
     assert call(B=1 << 20, Hq=1 << 14) == SHAPE                       # B * Hq
     assert call(width=1 << 27, page=16) == SHAPE                      # rows of a sequence
     assert call(pages=1 << 30) == SHAPE                               # tiles of the pool
-    assert call(B=2 ** 31 - 1, Hq=1, Hkv=1) == SHAPE                  # workgroups
+    assert call(B=2 ** 31 - 1, Hq=1, Hkv=1) == call(B=1 << 26, Hq=1, Hkv=1, width=1) == SHAPE       # waves
+    assert call(B=1 << 16, Hq=1, Hkv=1, width=1 << 15) == SHAPE       # steps of all heads
     assert call(D=96) == call(page=24) == call(page=8) == call(dtype=2) == call(scale=0.0) == call(scale=float("nan")) == call(scale=float("inf")) == UNSUP
     assert call(ks=P) == call(vs=P) == UNSUP                          # factors of bf16 pages
     assert call(q=P + 8) == call(k=P + 8) == call(v=P + 8) == call(o=P + 8) == call(table=P + 2) == call(lens=P + 2) == call(lse=P + 2) == MISAL

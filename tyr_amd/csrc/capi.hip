@@ -510,7 +510,8 @@ int tyr_hip_paged_decode(const void* q, const void* k_pages, const void* v_pages
     if (rc != TYR_HIP_OK) return rc;
     if (!(scale > 0.0f) || scale > 3.0e38f) return TYR_HIP_ERR_UNSUPPORTED;
     const uint64_t cap = table_width * page_size;
-    if (B * Hkv * ((Hq / Hkv + 15) / 16) > (uint64_t)INT_MAX / (cap / 32 + 8)) return TYR_HIP_ERR_BAD_SHAPE;      // steps of all heads
+    if (B * Hq >= (uint64_t)1 << 26) return TYR_HIP_ERR_BAD_SHAPE;            // waves of a launch
+    if (B * Hkv * ((Hq / Hkv + 15) / 16) > ((uint64_t)1 << 30) / (cap / 32 + 8)) return TYR_HIP_ERR_BAD_SHAPE;      // steps of all heads
     if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o) || !aligned4(page_table) || !aligned4(kv_lens) || !aligned4(lse))
         return TYR_HIP_ERR_MISALIGNED;
     const size_t need = tyr_hip_paged_decode_workspace_bytes(B, Hq, Hkv, D, page_size, table_width);

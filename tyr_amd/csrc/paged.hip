@@ -160,33 +160,31 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
     } else {
         round.read(a, 0, lane);
         int all = round.total();
-        for (int b0 = 64; b0 < a.B; b0 += 64) {
-            Round r;
-            r.read(a, b0, lane);
-            all += r.total();
+        if (a.B > 64) {
+            int more = 0;
+#pragma unroll 4
+            for (int i = 64 + lane; i < a.B; i += 64) more += Rows(max(0, min(a.kv_lens[i], a.cap)), a.window, a.sinks).steps() + TURN;
+            all += __builtin_amdgcn_readlane(sum_upto(more), 63);
         }
         all *= heads;
         const int share = max(MIN_SHARE, (all + a.shares - 1) / a.shares);
-        if (wave == 0 && lane == 0) a.plan[a.B] = int2{share, 0};
+        // one wave more than there are shares writes down the plan, for the launch that joins
+        const bool scribe = wave == a.shares;
+        if (scribe && lane == 0) a.plan[a.B] = int2{share, 0};
         at = min((int64_t)wave * share, (int64_t)all);
         end = min(at + share, all);
-        // the round in which step `at` lies; the first wave goes through all of them and writes down the plan
-        int before = 0, base = 0;
-        Round r = round;
-        for (int b0 = 0;;) {
-            const int upto = before + r.total() * heads;
-            if (wave == 0 && b0 + lane < a.B) a.plan[b0 + lane] = int2{before + (r.upto - r.steps - TURN) * heads, r.steps};
-            if (before <= at && at < upto) {
-                round = r;
-                base = before;
-            }
-            if (wave != 0 && at < upto) break;
-            before = upto;
-            b0 += 64;
-            if (b0 >= a.B) break;
-            r.read(a, b0, lane);
+        if (!scribe && at >= end) return;
+        // the round in which step `at` lies
+        int base = 0;
+        for (;;) {
+            const int upto = base + round.total() * heads, b0 = round.b0 + lane;
+            if (scribe) { if (b0 < a.B) a.plan[b0] = int2{base + (round.upto - round.steps - TURN) * heads, round.steps}; }
+            else if (at < upto) break;
+            base = upto;
+            if (round.b0 + 64 >= a.B) break;
+            round.read(a, round.b0 + 64, lane);
         }
-        if (at >= end) return;
+        if (scribe) return;
         // the first lane whose sequence ends behind `at`
         const int i = __builtin_ctzll(__builtin_amdgcn_ballot_w64(at < base + round.upto * heads));
         const int each = __builtin_amdgcn_readlane(round.steps, i) + TURN;
@@ -625,8 +623,8 @@ Grid paged_grid(int64_t B, int Hq, int Hkv, int64_t cap, int64_t window, int64_t
     const int64_t steps = std::max<int64_t>(1, (rows + STEP - 1) / STEP);
     Grid g{heads, std::min(G, 16), 0, (uint64_t)B * heads};
     if (steps > WHOLE) {
-        g.waves = (uint64_t)std::min<int64_t>(SHARES, (B * heads * (steps + TURN) + MIN_SHARE - 1) / MIN_SHARE);
-        g.shares = (int)g.waves;
+        g.shares = (int)std::min<int64_t>(SHARES, (B * heads * (steps + TURN) + MIN_SHARE - 1) / MIN_SHARE);
+        g.waves = g.shares + 1;
     }
     return g;
 }
@@ -635,7 +633,7 @@ Grid paged_grid(int64_t B, int Hq, int Hkv, int64_t cap, int64_t window, int64_t
 size_t paged_decode_workspace_bytes(int B, int Hq, int Hkv, int D, int64_t cap) {
     const Grid g = paged_grid(B, Hq, Hkv, cap, 0, 0);       // with a window there are as many waves at most
     if (!g.shares) return 0;
-    return (size_t)g.waves * 2 * g.per * (D + 2) * sizeof(float) + ((size_t)(B + 1) * sizeof(int2) + 15) / 16 * 16;
+    return (size_t)g.shares * 2 * g.per * (D + 2) * sizeof(float) + ((size_t)(B + 1) * sizeof(int2) + 15) / 16 * 16;
 }
 
 int launch_paged_decode(const void* q, const void* k_pages, const void* v_pages, const int* page_table, const int* kv_lens,
@@ -652,8 +650,8 @@ int launch_paged_decode(const void* q, const void* k_pages, const void* v_pages,
     if (g.shares) {
         a.plan = static_cast<int2*>(workspace);
         a.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + ((size_t)(B + 1) * sizeof(int2) + 15) / 16 * 16);
-        a.part_m = a.part_o + (size_t)g.waves * 2 * g.per * D;
-        a.part_l = a.part_m + (size_t)g.waves * 2 * g.per;
+        a.part_m = a.part_o + (size_t)g.shares * 2 * g.per * D;
+        a.part_l = a.part_m + (size_t)g.shares * 2 * g.per;
     }
     a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv, a.blocks = (a.G + 15) / 16;
     a.width = width, a.page_tiles = page_size / TILE, a.pages = pages;

@@ -447,6 +447,17 @@ struct Pages {
         if ((k_scale && k_scale->numel() != Hkv) || (v_scale && v_scale->numel() != Hkv)) fail("kScale and vScale must hold one factor per kv head");
     }
 };
+// a number of rows; more than fit 64 bits are as many as there are
+int64_t count(PyObject* o, const char* name) {
+    PyObject* i = PyNumber_Index(o);
+    if (!i) throw python_error();
+    int beyond = 0;
+    const long long v = PyLong_AsLongLongAndOverflow(i, &beyond);
+    Py_DECREF(i);
+    if (PyErr_Occurred()) throw python_error();
+    if (beyond < 0 || (beyond == 0 && v < 0)) fail(std::string(name) + " must not be negative");
+    return beyond > 0 ? INT64_MAX : v;
+}
 const at::Tensor& one_each(PyObject* o, const char* name, int64_t B) {
     const at::Tensor& t = checked(o, name, at::kInt, 1);
     if (t.numel() != B) fail(std::string(name) + " must hold one value per sequence");
@@ -490,8 +501,7 @@ PyObject* paged_decode(PyObject* const* a) {
     const Pages c(a[1], a[2], a[3], a[8], a[9], B, D);
     const at::Tensor& lens = one_each(a[4], "kvLens", B);
     const float scale = attn_scale(a[5], D);
-    const int64_t window = integer(a[6]), sinks = integer(a[7]);
-    if (window < 0 || sinks < 0) fail("window and sinks must not be negative");
+    const int64_t window = count(a[6], "window"), sinks = count(a[7], "sinks");
     not_empty({&q, &c.k, &c.table}, "pagedDecode");
     const OnDevice on(q, {&c.k, &c.v, &c.table, &lens, c.k_scale, c.v_scale}, truth(a[10]));
     at::Tensor o, lse;
