@@ -10,8 +10,8 @@
 //   sequence, and are dealt out evenly to as many waves as the device holds, one a SIMD: each works out its share from the lengths
 //   that are there, so neither unequal lengths nor a table much wider than they are leave CUs idle, and a captured launch follows
 //   lengths that change between replays.  A wave goes through its share without a pause between heads.  (Workgroups of four waves on
-//   one piece of a sequence, joined through LDS, 512 and more of them: 64 sequences of 37 to 32768 e4m3 rows took 160-190 us, so 117;
-//   32 sequences of 8192 bf16 rows 182, so 173.)
+//   one piece of a sequence, joined through LDS, 512 and more of them: 64 sequences of 37 to 32768 e4m3 rows took 160-190 us, 116 so;
+//   32 sequences of 8192 bf16 rows 182, 172 so.)
 //   Heads that several waves have a part of are joined by a second launch from partial results (O, m, l), as
 //     m = max m_s ; l = sum l_s 2^(m_s-m) ; O = sum O_s 2^(m_s-m) / l ; LSE = ln l + m ln 2.
 // HBM-bound: each visible row of K and V is read once a block of query heads, straight into MFMA operand registers (16x16x32 bf16):
@@ -185,8 +185,10 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
             round.read(a, round.b0 + 64, lane);
         }
         if (scribe) return;
-        // the first lane whose sequence ends behind `at`
-        const int i = __builtin_ctzll(__builtin_amdgcn_ballot_w64(at < base + round.upto * heads));
+        // the first lane whose sequence ends behind `at`; none if the lengths changed under the two readings of them
+        const uint64_t behind = __builtin_amdgcn_ballot_w64(at < base + round.upto * heads);
+        if (behind == 0) return;
+        const int i = __builtin_ctzll(behind);
         const int each = __builtin_amdgcn_readlane(round.steps, i) + TURN;
         const int start = base + (__builtin_amdgcn_readlane(round.upto, i) - each) * heads;
         b = round.b0 + i;
@@ -231,7 +233,7 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
     }
 
     struct Slot { Buf<D, FP8> buf; uint32_t seen[2]; int b, hb, first, last, live; };
-    Run run = locate(), then;
+    Run run = locate(), then = run;
     then.steps = 0;
     int s = 0;                                       // step of the run to load next
     auto load = [&](Slot& o) {
@@ -418,7 +420,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged::Args a) {
     const int share = a.plan[a.B].x;
     const int kvh = qh / a.G, inner = qh % a.G, hb = kvh * a.blocks + inner / 16, per = min(16, a.G);
     // the waves that had a part of this head's steps
-    const int first = plan.x + hb * (plan.y + TURN), w0 = first / share, S = (first + plan.y - 1) / share - w0 + 1;
+    const int first = plan.x + hb * (plan.y + TURN), w0 = first / share, S = min((first + plan.y - 1) / share, a.shares - 1) - w0 + 1;
     if (S < 2) return;
     const int t = threadIdx.x, c = t % TPS, sg = t / TPS;
     // of the first wave: the head that goes on behind it; of the others the one that began before them
@@ -476,7 +478,7 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(const paged::Args a
     const int2 plan = a.plan[b];
     const int share = a.plan[a.B].x;
     const int kvh = qh / a.G, inner = qh % a.G, hb = kvh * a.blocks + inner / 16, per = min(16, a.G);
-    const int first = plan.x + hb * (plan.y + TURN), w0 = first / share, S = (first + plan.y - 1) / share - w0 + 1;
+    const int first = plan.x + hb * (plan.y + TURN), w0 = first / share, S = min((first + plan.y - 1) / share, a.shares - 1) - w0 + 1;
     if (S < 2) return;
     const int lane = threadIdx.x & 63, c = lane % TPS, sg = lane / TPS;
     auto slot_of = [&](int i) { return (size_t)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * per + inner % 16; };

@@ -163,8 +163,8 @@ __global__ __launch_bounds__(S::THREADS) void rmsnorm_residual_kernel(
 // Gradients.  Workgroups of 16 waves: as many row slots as fit, slot s of workgroup i takes the rows ROWS (i + k gridDim.x) + s, the
 // next one's loads under way while it works on one, and keeps dw of its rows in registers.  The slots are added through LDS at the
 // end, half of them to the other half at a time, and the workgroup writes one row of part [gridDim.x][d_model].
-// 65536 x 1024 83 us of reading and writing 537 MB and 4 us for the parts; 2000 x 4096 12.5 and 3.  (1024 workgroups of four waves: 91 and
-// 14 and as much again for their parts; with two pieces a lane, spilling: 90 and 14; 512 workgroups: 86 and 15.)
+// 65536 x 1024 85 us of reading and writing 537 MB and 5 us for the parts; 2000 x 4096 12.5 and 3.  (1024 workgroups of four waves: 91 and
+// 14, and 17 MB of parts; two pieces a lane, spilling: 93 and 15; 512 workgroups: 86 and 15.)
 template <class S, bool CACHED, bool RESID>
 __global__ __launch_bounds__(1024) void rmsnorm_residual_bwd_kernel(
     const uint16_t* __restrict__ d_out, const uint16_t* __restrict__ d_resid, const uint16_t* __restrict__ resid,
