@@ -84,6 +84,22 @@ def test_decode_lengths_heads_and_pages(Hq, Hkv, D, page, e4m3):
     _check(o, lse, q, k, v, table, LENS, 1 / math.sqrt(D), ks=ks, vs=vs)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(4, 4, 128), (8, 2, 64), (34, 2, 128), (16, 1, 64)])
+@pytest.mark.parametrize("page,rows", [(16, 256), (48, 240), (256, 256), (16, 272)])
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_decode_short_tables(Hq, Hkv, D, page, rows, e4m3):
+    """Tables up to and just beyond the rows from which sequences are cut, also more of them than lanes."""
+    import tyr_amd
+    lens_ = [0, 1, 15, 16, 17, 100, 129, rows - 1, rows] * 8
+    g = _gen(Hq * 7 + D + page + rows)
+    (k, v), table, ks, vs = _cache(g, lens_, page, Hkv, D, e4m3, width=-(-rows // page))
+    lens = torch.tensor(lens_, dtype=torch.int32, device="cuda")
+    q = torch.randn(len(lens_), Hq, 1, D, generator=g, device="cuda").bfloat16()
+    for window, sinks in ((0, 0), (60, 5)):
+        o, lse = tyr_amd.paged_decode(q, k, v, table, lens, window=window, sinks=sinks, k_scale=ks, v_scale=vs)
+        _check(o, lse, q, k, v, table, lens_, 1 / math.sqrt(D), window, sinks, ks, vs)
+
+
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (16, 4), (17, 16), (100, 0), (100, 17), (1000, 64), (33, 300), (5000, 4), (2 ** 40, 2 ** 40)])
 @pytest.mark.parametrize("page,e4m3,D", [(16, False, 128), (48, True, 128), (64, False, 64)])
 def test_decode_windows_and_sinks(window, sinks, page, e4m3, D):

@@ -33,7 +33,8 @@ constexpr int WAVES = 1, THREADS = 64 * WAVES;      // of one wave, a launch wit
                                             // rows 10.2 us with four, 8.8 so)
 constexpr int SHARES = 1024;                // waves that share a launch's steps: one on every SIMD of 256 CUs
 constexpr int MIN_SHARE = 2;                // steps of a wave at least
-constexpr int WHOLE = 4;                    // sequences of so many steps at most are not cut
+constexpr int WHOLE = 8;                    // sequences of so many steps at most are not cut, and so need no join: 88 heads of 6 steps 7.5 us whole, 8.8
+                                            // cut; of 8 8.7, 9.0; 1024 heads of 8 23.2, 25.4; 32 heads of 10 9.6, 8.0
 constexpr int TURN = 3;                     // steps that going from one head to the next is counted as
 constexpr int MANY_HEADS = 64;              // heads of a launch from which one wave joins each, not four (1024 heads of 3-22 steps 40.7 us, 37.4 so;
                                             // with 8 heads of 128 parts four waves have more of them under way)
