@@ -442,8 +442,8 @@ int tyr_hip_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const v
  *   page_table       : device int32 [B, table_width]; row j of sequence b is row j % page_size of page
  *                      page_table[b * table_width + j / page_size].  An entry outside [0, num_pages) is a page that is not there:
  *                      nothing is written to it, and its rows are not seen.
- *   k_scale, v_scale : device f32 [Hkv], positive and not denormal: a cached K is k_scale[kv head] * the stored value, V alike; NULL = all ones.
- *                      Only with e4m3 pages.
+ *   k_scale, v_scale : device f32 [Hkv]: a cached K is k_scale[kv head] * the stored value, V alike; NULL = all ones.  Only with e4m3
+ *                      pages.  The append divides by them: positive there, and not denormal.
  * Supported: D in {64, 128}; page_size a multiple of 16; num_pages * Hkv * page_size / 16 < 2^31; table_width * page_size < 2^31.
  *
  * tyr_hip_paged_rope_append: rotary embedding of T new tokens a sequence and their way into the pages.

@@ -242,6 +242,22 @@ def test_e4m3_pages_without_factors():
         _check(o, lse, q, k, v, table, [300, 20], 1 / math.sqrt(128), ks=one, vs=one)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 5)])
+def test_factors_of_zero_and_below(window, sinks):
+    """A kv head of factor 0 has scores of 0 (its rows count alike) or values of 0; a negative factor turns them round.  What is hidden
+    stays hidden."""
+    import tyr_amd
+    lens_ = [1, 17, 100, 777]
+    g = _gen(12)
+    (k, v), table, ks, vs = _cache(g, lens_, 16, 3, 128, True)
+    ks[0], vs[1] = 0.0, 0.0
+    ks[2], vs[2] = -ks[2], -vs[2]
+    lens = torch.tensor(lens_, dtype=torch.int32, device="cuda")
+    q = torch.randn(4, 12, 1, 128, generator=g, device="cuda").bfloat16()
+    o, lse = tyr_amd.paged_decode(q, k, v, table, lens, window=window, sinks=sinks, k_scale=ks, v_scale=vs)
+    _check(o, lse, q, k, v, table, lens_, 1 / math.sqrt(128), window, sinks, ks, vs)
+
+
 def test_equals_the_contiguous_decode():
     """The same rows in a contiguous cache: both are within their rounding of the same result."""
     import tyr_amd

@@ -188,7 +188,7 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
         if (scribe) return;
         // the first lane whose sequence ends behind `at`; none if the lengths changed under the two readings of them
         const uint64_t behind = __builtin_amdgcn_ballot_w64(at < base + round.upto * heads);
-        if (behind == 0) return;
+        if (behind == 0 || at < base) return;
         const int i = __builtin_ctzll(behind);
         const int each = __builtin_amdgcn_readlane(round.steps, i) + TURN;
         const int start = base + (__builtin_amdgcn_readlane(round.upto, i) - each) * heads;
@@ -206,6 +206,7 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
         if (++next_hb == heads) {
             next_hb = 0;
             if (++next_b - round.b0 == 64) round.read(a, next_b, lane);
+            if (next_b >= a.B) next_at = end;        // the lengths changed: no sequence is left
         }
     };
     auto locate = [&]() {
@@ -343,6 +344,8 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
             if constexpr (FP8) v[p] = bf16_of_e4m3(o.buf.v[p][0], o.buf.v[p][1]);
             else v[p] = o.buf.v[p];
         }
+        sacc[0] *= scale_log2;                       // before anything is hidden: the pages' factor may be 0 or negative
+        sacc[1] *= scale_log2;
         // register r of tile T is its row 4g + r.  What is hidden may hold anything: its score goes, and its V, which 0 * NaN would keep.
         if ((o.seen[0] & o.seen[1]) != 0xffffu) {
 #pragma unroll
@@ -357,7 +360,7 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
         float mx = fmaxf(fmaxf(fmaxf(sacc[0][0], sacc[0][1]), fmaxf(sacc[0][2], sacc[0][3])),
                          fmaxf(fmaxf(sacc[1][0], sacc[1][1]), fmaxf(sacc[1][2], sacc[1][3])));
         mx = max_xor32(max_xor16(mx));
-        const float m2new = fmaxf(m2, mx * scale_log2);
+        const float m2new = fmaxf(m2, mx);
         const float ref = m2new == -INFINITY ? 0.0f : m2new;       // nothing seen yet: every power below is of -inf
         const float alpha = fast_exp2(m2 - ref);
         if (__builtin_amdgcn_ballot_w64(m2new > m2) != 0) {
@@ -368,7 +371,7 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
         float pv[8], psum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            pv[i] = fast_exp2(fmaf(sacc[i >> 2][i & 3], scale_log2, -ref));
+            pv[i] = fast_exp2(sacc[i >> 2][i & 3] - ref);
             psum += pv[i];
         }
         lsum = lsum * alpha + psum;
