@@ -413,7 +413,7 @@ int tyr_hip_gemm_fp8_ws(const void* aq, const void* bq, void* c,
  *
  *   x, residual, out_resid : bf16 [rows, d_model]; residual and out_resid both given or both NULL; outputs overlap no input
  *   weight : bf16 [d_model]     out : bf16 or e4m3 [rows, d_model]     row_scale : f32 [rows] (e4m3), not looked at for bf16
- * Supported: d_model % 8 == 0 up to 16384.
+ * Supported: d_model % 8 == 0 up to 16384; rows * (elements of a row, rounded up to 64 * 2^n) < 2^35, twice that above 512.
  */
 int tyr_hip_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* out, void* out_resid,
                              float* row_scale, uint64_t rows, uint64_t d_model, float eps, int out_dtype, void* stream);

@@ -142,6 +142,16 @@ def test_backward(rows, d):
         assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("d", [64, 1000, 16384])
+@pytest.mark.parametrize("size", [1e-15, 1e15])
+def test_backward_of_large_and_small_rows(d, size):
+    """rho^3 is beyond f32; the gradients are not."""
+    import tyr_amd
+    (h, g), w = _data(20, d, 13, 2)
+    h = (h.float() * size).bfloat16()
+    _check_grads(tyr_amd.rmsnorm_residual_bwd(g, h, w, 0.0), g, h, w, 0.0, None)
+
+
 @pytest.mark.parametrize("rows,d", [(60000, 72), (9000, 1024), (3001, 4096), (1030, 16384)])
 def test_backward_of_many_rows(rows, d):
     """More row groups than workgroups."""

@@ -19,6 +19,10 @@ def test_rmsnorm():
     assert fwd(d=60) == fwd(d=16392) == fwd(dtype=1) == fwd(dtype=7) == fwd(eps=-1.0) == fwd(eps=float("nan")) == UNSUP
     assert fwd(x=P + 2) == fwd(res=P + 8) == fwd(w=P + 8) == fwd(out=P + 4) == fwd(out_res=P + 8) == fwd(scale=P + 2, dtype=2) == MISAL
 
+    # threads of a launch: eight elements each up to a row of 512, then sixteen
+    for rows, d in ((1 << 29, 64), (1 << 29, 8), (1 << 28, 72), (1 << 26, 512), (1 << 26, 520), (1 << 22, 8200), (1 << 22, 16384)):
+        assert fwd(rows=rows, d=d) == SHAPE and fwd(rows=rows, d=d, x=P + 2) == SHAPE and fwd(rows=rows - 32, d=d, x=P + 2) == MISAL, (rows, d)
+
     def bwd(g=P, dr=P, h=P, w=P, dx=P, dw=P, rows=4, d=64, eps=1e-6, ws=P, n=BIG):
         return L.tyr_hip_rmsnorm_residual_bwd(g, dr, h, w, dx, dw, rows, d, eps, ws, n, None)
     assert bwd(g=None) == bwd(h=None) == bwd(w=None) == bwd(dx=None) == bwd(dw=None) == NULL

@@ -426,6 +426,7 @@ int tyr_hip_rmsnorm_residual(const void* x, const void* residual, const void* we
     int rc;
     if (!norm_extents(rows, d_model, &rc)) return rc;
     if ((out_dtype != TYR_HIP_OUT_BF16 && out_dtype != TYR_HIP_OUT_E4M3) || !(eps >= 0.0f)) return TYR_HIP_ERR_UNSUPPORTED;
+    if (!tyr::rmsnorm_residual_fits((size_t)rows, (int)d_model)) return TYR_HIP_ERR_BAD_SHAPE;
     if (out_dtype == TYR_HIP_OUT_E4M3 && !row_scale) return TYR_HIP_ERR_NULL_POINTER;
     if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(out) || !aligned16(out_resid) || !aligned4(row_scale))
         return TYR_HIP_ERR_MISALIGNED;

@@ -51,6 +51,7 @@ int launch_decode_rope_append(const void* q, const void* k_new, const void* v_ne
 int launch_layernorm_residual(const void* x, const void* residual, const void* weight, const void* bias, void* out,
                               void* out_resid, size_t rows, int d_model, float eps, hipStream_t stream);
 // residual and out_resid: both or neither; row_scale [rows] with e4m3
+bool rmsnorm_residual_fits(size_t rows, int d_model);      // a launch has fewer than 2^32 threads
 int launch_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* out, void* out_resid, float* row_scale,
                             size_t rows, int d_model, float eps, int e4m3, hipStream_t stream);
 size_t rmsnorm_residual_bwd_workspace_bytes(size_t rows, int d_model);

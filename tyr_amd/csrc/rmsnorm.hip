@@ -175,7 +175,6 @@ __global__ __launch_bounds__(1024) void rmsnorm_residual_bwd_kernel(
     extern __shared__ __attribute__((aligned(16))) float sums[];   // [ROWS / 2][d_model]
     const int lane = threadIdx.x % LPR, wave = threadIdx.x / 64, wr = wave % WPR;
     const int slot = WPR > 1 ? wave / WPR : threadIdx.x / LPR;
-    const int all = d_model / 8;
     int pc[P], at[P];                                            // this lane's elements of a row; their place in a group of rows
     bool has[P];
     constexpr bool TIGHT = P > 1;                                // registers for the rows as they came only
@@ -238,7 +237,7 @@ __global__ __launch_bounds__(1024) void rmsnorm_residual_bwd_kernel(
             turn ^= 1;
         }
         const float rho = first + slot < rows ? rsqrtf(sq / (float)d_model + eps) : 0.0f;
-        const float c = rho * rho * rho * (gwh / (float)d_model);
+        const float c = gwh / (float)d_model * rho * rho * rho;      // in this order: rho^3 alone leaves f32 for rows of 1e13 or 1e-13
         const auto to = group(dx, first);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
@@ -357,6 +356,15 @@ size_t bwd_parts(size_t rows) {
     return groups < 256 ? groups : 256;
 }
 }  // namespace
+
+bool rmsnorm_residual_fits(size_t rows, int d_model) {
+    bool fits = false;
+    with_shape(d_model, [&](auto shape) {
+        using S = decltype(shape);
+        fits = (rows + S::ROWS - 1) / S::ROWS * S::THREADS < ((size_t)1 << 32);
+    });
+    return fits;
+}
 
 int launch_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* out, void* out_resid, float* row_scale,
                             size_t rows, int d_model, float eps, int e4m3, hipStream_t stream) {
