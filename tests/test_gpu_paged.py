@@ -84,6 +84,40 @@ def test_decode_lengths_heads_and_pages(Hq, Hkv, D, page, e4m3):
     _check(o, lse, q, k, v, table, LENS, 1 / math.sqrt(D), ks=ks, vs=vs)
 
 
+@pytest.mark.parametrize("Hq,Hkv", [(17, 1), (32, 1), (66, 2), (33, 1), (130, 1)])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("rows", [256, 3100, 70000])
+def test_decode_many_query_heads_of_a_kv_head(Hq, Hkv, D, e4m3, rows):
+    """Blocks of query heads, apart and together, and waves side by side: which of them depends on the tables' width."""
+    import tyr_amd
+    lens_ = [0, 1, 17, 31, 33, 100, rows // 2 - 5, 255, rows]
+    g = _gen(Hq * 31 + D + rows)
+    (k, v), table, ks, vs = _cache(g, lens_, 16, Hkv, D, e4m3, width=-(-rows // 16))
+    copies = 8 if rows == 70000 else 1               # the same sequences again
+    lens_ = lens_ * copies
+    table = table.repeat(copies, 1)
+    lens = torch.tensor(lens_, dtype=torch.int32, device="cuda")
+    q = torch.randn(len(lens_), Hq, 1, D, generator=g, device="cuda").bfloat16()
+    for window, sinks in ((0, 0), (300, 7), (60, 0)):
+        o, lse = tyr_amd.paged_decode(q, k, v, table, lens, window=window, sinks=sinks, k_scale=ks, v_scale=vs)
+        _check(o, lse, q, k, v, table, lens_, 1 / math.sqrt(D), window, sinks, ks, vs, only=range(9 * copies - 9, 9 * copies) if copies > 1 else None)
+        again, lse2 = tyr_amd.paged_decode(q, k, v, table, lens, window=window, sinks=sinks, k_scale=ks, v_scale=vs)
+        assert torch.equal(o, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("D,e4m3", [(64, False), (64, True), (128, False), (128, True)])
+def test_decode_many_short_sequences_of_many_query_heads(D, e4m3):
+    import tyr_amd
+    lens_ = [(37 * i) % 257 for i in range(2050)]
+    g = _gen(21 + D)
+    (k, v), table, ks, vs = _cache(g, lens_, 16, 1, D, e4m3, width=16)
+    lens = torch.tensor(lens_, dtype=torch.int32, device="cuda")
+    q = torch.randn(2050, 20, 1, D, generator=g, device="cuda").bfloat16()
+    o, lse = tyr_amd.paged_decode(q, k, v, table, lens, k_scale=ks, v_scale=vs)
+    _check(o, lse, q, k, v, table, lens_, 1 / math.sqrt(D), ks=ks, vs=vs, only=[*range(0, 2050, 41), 2049])
+
+
 @pytest.mark.parametrize("Hq,Hkv,D", [(4, 4, 128), (8, 2, 64), (34, 2, 128), (16, 1, 64)])
 @pytest.mark.parametrize("page,rows", [(16, 256), (48, 240), (256, 256), (16, 272)])
 @pytest.mark.parametrize("e4m3", [False, True])

@@ -6,7 +6,7 @@
 //
 // Attention.  Row j of a sequence of n rows is visible iff j < n and (no window, or j >= n - window, or j < sinks).  The visible
 // rows are walked as a list of 16-row tiles, the sinks' first, two tiles a step; pages without a visible row are never looked at.
-//   All steps of all heads (a head: one kv head of one sequence, and at most 16 of its query heads) stand in one row, sequence by
+//   All steps of all heads (a head: one kv head of one sequence, and a block of its query heads) stand in one row, sequence by
 //   sequence, and are dealt out evenly to as many waves as the device holds, one a SIMD: each works out its share from the lengths
 //   that are there, so neither unequal lengths nor a table much wider than they are leave CUs idle, and a captured launch follows
 //   lengths that change between replays.  A wave goes through its share without a pause between heads.  (Workgroups of four waves on
@@ -24,17 +24,25 @@
 #include "launch.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tyr {
 
 namespace paged {
 constexpr int TILE = 16, STEP = 2 * TILE;
-constexpr int WAVES = 1, THREADS = 64 * WAVES;      // of one wave, a launch with few waves has them on as many CUs (one sequence of 1500
-                                            // rows 10.2 us with four, 8.8 so)
 constexpr int SHARES = 1024;                // waves that share a launch's steps: one on every SIMD of 256 CUs
 constexpr int MIN_SHARE = 2;                // steps of a wave at least
 constexpr int WHOLE = 8;                    // sequences of so many steps at most are not cut, and so need no join: 88 heads of 6 steps 7.5 us whole, 8.8
                                             // cut; of 8 8.7, 9.0; 1024 heads of 8 23.2, 25.4; 32 heads of 10 9.6, 8.0
+// More than 16 query heads of a kv head are several blocks.  Where each block is a head of its own, its rows come from memory once a block.
+// Two other ways have them come once for two blocks, or for all:
+//   - a wave takes two blocks (bf16 rows of 128 leave no registers for that).  Its steps take longer, so only launches that have many of
+//     them, by their tables' width: 128 sequences of 8192 e4m3 rows, 32 query heads of one kv head 98.7 us, 63.8 so; 64 of 4000 29.1, 30.4.
+constexpr int WIDE = 32768;                 // steps of all blocks from which
+//   - waves side by side in a workgroup take a block each of the same steps and keep together by a barrier, so that all but the first find
+//     the rows in the caches: bf16 rows of 128 where sequences are cut.  128 sequences of 8192 rows, 32 heads 182 us, 118 so (1024 shares
+//     124, and without the barrier 162); 28 of 2517 24.6, 19.0; 96 of 5 steps, not cut, 6.7, 7.4; 128 of 8192 e4m3 rows 98.7, 94.2.
+constexpr int SIDE_BY_SIDE = 8;             // of them at most: as many as have their registers on a CU at once
 constexpr int TURN = 3;                     // steps that going from one head to the next is counted as
 constexpr int MANY_HEADS = 64;              // heads of a launch from which one wave joins each, not four (1024 heads of 3-22 steps 40.7 us, 37.4 so;
                                             // with 8 heads of 128 parts four waves have more of them under way)
@@ -83,7 +91,8 @@ struct Args {
     uint16_t* o;
     float *lse, *part_o, *part_m, *part_l;
     int2* plan;                             // [B] first step of each sequence's first head, steps of a head; [B]: steps of a wave
-    int B, Hq, Hkv, G, blocks;              // G = query heads of a kv head; blocks of 16 of them
+    int B, Hq, Hkv, G;                      // G = query heads of a kv head
+    int per, apart, beside;                 // query heads of a block; blocks that are heads of their own; blocks of waves side by side
     int width, page_tiles, pages;           // pages of a table row; tiles of a page; pages of the pool
     int cap, window, sinks, shares;         // shares = 0: every wave takes one head of one sequence, nothing is cut
     float scale_log2;
@@ -123,12 +132,12 @@ template <int D> struct Buf<D, true> {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const void* pool, size_t at, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(pool) + at), 0, bytes, 0x00020000);
 }
-constexpr int NT = 2;                       // cache policy: not kept
-__device__ __forceinline__ u32x4 load_tile_16(__amdgpu_buffer_rsrc_t t, int at) {
-    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(t, at, 0, NT));
+// AGAIN: waves beside this one read the same.  Else the caches are not to keep it (32 sequences of 8192 rows 172 us, 195 if they do).
+template <bool AGAIN> __device__ __forceinline__ u32x4 load_tile_16(__amdgpu_buffer_rsrc_t t, int at) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(t, at, 0, AGAIN ? 0 : 2));
 }
-__device__ __forceinline__ u32x2 load_tile_8(__amdgpu_buffer_rsrc_t t, int at) {
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(t, at, 0, NT));
+template <bool AGAIN> __device__ __forceinline__ u32x2 load_tile_8(__amdgpu_buffer_rsrc_t t, int at) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(t, at, 0, AGAIN ? 0 : 2));
 }
 
 __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t four, bool upper) {
@@ -140,21 +149,24 @@ __device__ __forceinline__ u32x4 bf16_of_e4m3(uint32_t lo, uint32_t hi) {
 }
 }  // namespace paged
 
-template <int D, bool FP8>
-__global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const paged::Args a) {
+// QB: 16 query heads or 32 of a wave.  AGAIN: a workgroup is a.beside waves side by side, else one (of four, a launch with few waves would
+// have them on fewer CUs: one sequence of 1500 rows 8.8 us, 10.2 so).
+template <int D, bool FP8, int QB, bool AGAIN>
+__global__ __launch_bounds__(64 * (AGAIN ? paged::SIDE_BY_SIDE : 1), 2) void paged_decode_kernel(const paged::Args a) {
     using namespace paged;
     const int lane = threadIdx.x & 63, x = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * WAVES + threadIdx.x / 64));
-    const int heads = a.Hkv * a.blocks;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(AGAIN ? blockIdx.x * a.beside + threadIdx.x / 64 : blockIdx.x));
+    const int place = AGAIN ? blockIdx.x : wave;     // which share of the steps
+    const int side = AGAIN ? __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64)) : 0;
+    const int heads = a.Hkv * a.apart;
     constexpr int KI = D / 32, TILE_BYTES = TILE * D * (FP8 ? 1 : 2);
 
     // ---- this wave's steps [at, end) of all, and the head of the sequence in which they begin
     Round round;
     int at, end, b, hb, first;                       // first = the sequence's (head's) first step
     if (a.shares == 0) {
-        if (wave >= a.B * heads) return;
-        b = wave / heads;
-        hb = wave - b * heads;
+        b = place / heads;
+        hb = place - b * heads;
         round.read(a, b & ~63, lane);
         at = first = 0;
         end = __builtin_amdgcn_readlane(round.steps, b & 63);
@@ -170,9 +182,10 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
         all *= heads;
         const int share = max(MIN_SHARE, (all + a.shares - 1) / a.shares);
         // one wave more than there are shares writes down the plan, for the launch that joins
-        const bool scribe = wave == a.shares;
+        const bool scribe = place == a.shares;
+        if (scribe && side > 0) return;
         if (scribe && lane == 0) a.plan[a.B] = int2{share, 0};
-        at = min((int64_t)wave * share, (int64_t)all);
+        at = min((int64_t)place * share, (int64_t)all);
         end = min(at + share, all);
         if (!scribe && at >= end) return;
         // the round in which step `at` lies
@@ -220,7 +233,7 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
         if (t < rows.count && lane < 2 * r.steps) {
             const int tile = rows.tile(t), page = tile / a.page_tiles, id = a.table[(size_t)next_b * a.width + page];
             if (id >= 0 && id < a.pages) {
-                r.tile = (id * a.Hkv + next_hb / a.blocks) * a.page_tiles + tile - page * a.page_tiles;
+                r.tile = (id * a.Hkv + next_hb / a.apart) * a.page_tiles + tile - page * a.page_tiles;
                 r.mask = rows.mask(tile);
             }
         }
@@ -255,66 +268,75 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
             const auto k = tile_rsrc(a.k, base, there), v = tile_rsrc(a.v, base, there);
             if constexpr (FP8) {
 #pragma unroll
-                for (int c = 0; c < D / 64; ++c) o.buf.k[T][c] = load_tile_16(k, x * D + 16 * (4 * c + g));
+                for (int c = 0; c < D / 64; ++c) o.buf.k[T][c] = load_tile_16<AGAIN>(k, x * D + 16 * (4 * c + g));
 #pragma unroll
-                for (int p = 0; p < 4; ++p) o.buf.v[4 * T + p] = load_tile_8(v, (4 * g + p) * D + (x & (D / 8 - 1)) * 8);
+                for (int p = 0; p < 4; ++p) o.buf.v[4 * T + p] = load_tile_8<AGAIN>(v, (4 * g + p) * D + (x & (D / 8 - 1)) * 8);
             } else {
 #pragma unroll
-                for (int i = 0; i < KI; ++i) o.buf.k[T][i] = load_tile_16(k, (x * D + 32 * i + 8 * g) * 2);
+                for (int i = 0; i < KI; ++i) o.buf.k[T][i] = load_tile_16<AGAIN>(k, (x * D + 32 * i + 8 * g) * 2);
 #pragma unroll
-                for (int p = 0; p < 4; ++p) o.buf.v[4 * T + p] = load_tile_16(v, ((4 * g + p) * D + (x & (D / 8 - 1)) * 8) * 2);
+                for (int p = 0; p < 4; ++p) o.buf.v[4 * T + p] = load_tile_16<AGAIN>(v, ((4 * g + p) * D + (x & (D / 8 - 1)) * 8) * 2);
             }
         }
         ++s;
     };
 
     // ---- one head: Q^T operand (column x = query head q0 + x, zero beyond the block's heads) and running sums
-    __shared__ u32x4 qs[WAVES][KI][64];
-    u32x4 (&qf)[KI][64] = qs[threadIdx.x / 64];      // a lane reads what it wrote: registers are short, LDS is idle
-    f32x4 oacc[8];
-    float m2, lsum, scale_log2;
+    __shared__ u32x4 qs[AGAIN ? SIDE_BY_SIDE : 1][QB * KI][64];
+    u32x4 (&qf)[QB * KI][64] = qs[side];      // a lane reads what it wrote: registers are short, LDS is idle
+    f32x4 oacc[QB][8];
+    float m2[QB], lsum[QB], scale_log2;
     int nq, kvh;
     size_t head0;
     auto begin = [&](int b_, int hb_) {
-        kvh = hb_ / a.blocks;
-        const int q0 = (hb_ - kvh * a.blocks) * 16;
-        nq = min(16, a.G - q0);
+        kvh = hb_ / a.apart;
+        const int q0 = (AGAIN ? side : hb_ - kvh * a.apart) * (16 * QB);
+        nq = min(16 * QB, a.G - q0);
         head0 = (size_t)b_ * a.Hq + (size_t)kvh * a.G + q0;
-        const uint16_t* qp = a.q + (head0 + min(x, nq - 1)) * D;
 #pragma unroll
-        for (int i = 0; i < KI; ++i) {
-            u32x4 v = ld_global_16(qp + (FP8 ? 16 * (4 * (i >> 1) + g) + 8 * (i & 1) : 32 * i + 8 * g));
-            if (x >= nq) v = u32x4{0, 0, 0, 0};
-            qf[i][lane] = v;
+        for (int c = 0; c < QB; ++c) {
+            const uint16_t* qp = a.q + (head0 + min(16 * c + x, nq - 1)) * D;
+#pragma unroll
+            for (int i = 0; i < KI; ++i) {
+                u32x4 v = ld_global_16(qp + (FP8 ? 16 * (4 * (i >> 1) + g) + 8 * (i & 1) : 32 * i + 8 * g));
+                if (16 * c + x >= nq) v = u32x4{0, 0, 0, 0};
+                qf[c * KI + i][lane] = v;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) oacc[c][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+            m2[c] = -INFINITY;
+            lsum[c] = 0.0f;
         }
         scale_log2 = a.scale_log2 * factor(a.k_scale, kvh);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) oacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        m2 = -INFINITY;
-        lsum = 0.0f;
     };
     // The head's steps are done, or this wave's: its result where the wave had all of them, else a partial one.  A wave has at most two
     // heads that it shares with others: one that began before it, and one that goes on behind it.  oacc[i][r] is O^T[d = 32g + 8r + i][x].
     auto finish = [&](int first_, int last_) {
-        const float l = sum_xor32(sum_xor16(lsum)), v_scale = factor(a.v_scale, kvh);
-        if (x >= nq || 32 * g >= D) return;
-        if (first_ >= at && last_ <= end) {
-            const float f = l == 0.0f ? 0.0f : v_scale / l;
-            uint16_t* to = a.o + (head0 + x) * D + 32 * g;
+        const float v_scale = factor(a.v_scale, kvh);
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                st_global_16(to + 8 * r, u32x4{pack_bf16(oacc[0][r] * f, oacc[1][r] * f), pack_bf16(oacc[2][r] * f, oacc[3][r] * f),
-                                               pack_bf16(oacc[4][r] * f, oacc[5][r] * f), pack_bf16(oacc[6][r] * f, oacc[7][r] * f)});
-            if (g == 0 && a.lse) a.lse[head0 + x] = l == 0.0f ? -INFINITY : logf(l) + m2 * LN2;
-        } else {
-            const size_t slot = (size_t)(2 * wave + (first_ < at ? 0 : 1)) * min(16, a.G) + x;
-            float* to = a.part_o + slot * D + 32 * g;
+        for (int c = 0; c < QB; ++c) {
+            const float l = sum_xor32(sum_xor16(lsum[c]));
+            const int h = 16 * c + x;
+            if (h >= nq || 32 * g >= D) continue;
+            const f32x4 (&o)[8] = oacc[c];
+            if (first_ >= at && last_ <= end) {
+                const float f = l == 0.0f ? 0.0f : v_scale / l;
+                uint16_t* to = a.o + (head0 + h) * D + 32 * g;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                *reinterpret_cast<f32x4*>(to + 8 * r) = f32x4{oacc[0][r], oacc[1][r], oacc[2][r], oacc[3][r]} * v_scale;
-                *reinterpret_cast<f32x4*>(to + 8 * r + 4) = f32x4{oacc[4][r], oacc[5][r], oacc[6][r], oacc[7][r]} * v_scale;
+                for (int r = 0; r < 4; ++r)
+                    st_global_16(to + 8 * r, u32x4{pack_bf16(o[0][r] * f, o[1][r] * f), pack_bf16(o[2][r] * f, o[3][r] * f),
+                                                   pack_bf16(o[4][r] * f, o[5][r] * f), pack_bf16(o[6][r] * f, o[7][r] * f)});
+                if (g == 0 && a.lse) a.lse[head0 + h] = l == 0.0f ? -INFINITY : logf(l) + m2[c] * LN2;
+            } else {
+                const size_t slot = (size_t)(2 * wave + (first_ < at ? 0 : 1)) * min(16 * QB, a.G) + h;
+                float* to = a.part_o + slot * D + 32 * g;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    *reinterpret_cast<f32x4*>(to + 8 * r) = f32x4{o[0][r], o[1][r], o[2][r], o[3][r]} * v_scale;
+                    *reinterpret_cast<f32x4*>(to + 8 * r + 4) = f32x4{o[4][r], o[5][r], o[6][r], o[7][r]} * v_scale;
+                }
+                if (g == 0) { a.part_m[slot] = m2[c]; a.part_l[slot] = l; }
             }
-            if (g == 0) { a.part_m[slot] = m2; a.part_l[slot] = l; }
         }
     };
 
@@ -326,17 +348,20 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
             now = o.first;
         }
         now_last = o.last;
-        f32x4 sacc[2];
+        f32x4 sacc[QB][2];
         u32x4 v[8];
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
-            sacc[T] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < QB; ++c) sacc[c][T] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < KI; ++i) {
                 u32x4 k;
                 if constexpr (FP8) k = i & 1 ? bf16_of_e4m3(o.buf.k[T][i / 2][2], o.buf.k[T][i / 2][3]) : bf16_of_e4m3(o.buf.k[T][i / 2][0], o.buf.k[T][i / 2][1]);
                 else k = o.buf.k[T][i];
-                sacc[T] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, qf[i][lane]), sacc[T]);
+#pragma unroll
+                for (int c = 0; c < QB; ++c)
+                    sacc[c][T] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, k), __builtin_bit_cast(bf16x8, qf[c * KI + i][lane]), sacc[c][T]);
             }
         }
 #pragma unroll
@@ -344,8 +369,10 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
             if constexpr (FP8) v[p] = bf16_of_e4m3(o.buf.v[p][0], o.buf.v[p][1]);
             else v[p] = o.buf.v[p];
         }
-        sacc[0] *= scale_log2;                       // before anything is hidden: the pages' factor may be 0 or negative
-        sacc[1] *= scale_log2;
+#pragma unroll
+        for (int c = 0; c < QB; ++c)                 // before anything is hidden: the pages' factor may be 0 or negative
+#pragma unroll
+            for (int T = 0; T < 2; ++T) sacc[c][T] *= scale_log2;
         // register r of tile T is its row 4g + r.  What is hidden may hold anything: its score goes, and its V, which 0 * NaN would keep.
         if ((o.seen[0] & o.seen[1]) != 0xffffu) {
 #pragma unroll
@@ -353,46 +380,53 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (!(o.seen[T] >> (4 * g + r) & 1)) {
-                        sacc[T][r] = -INFINITY;
+#pragma unroll
+                        for (int c = 0; c < QB; ++c) sacc[c][T][r] = -INFINITY;
                         v[4 * T + r] = u32x4{0, 0, 0, 0};
                     }
         }
-        float mx = fmaxf(fmaxf(fmaxf(sacc[0][0], sacc[0][1]), fmaxf(sacc[0][2], sacc[0][3])),
-                         fmaxf(fmaxf(sacc[1][0], sacc[1][1]), fmaxf(sacc[1][2], sacc[1][3])));
-        mx = max_xor32(max_xor16(mx));
-        const float m2new = fmaxf(m2, mx);
-        const float ref = m2new == -INFINITY ? 0.0f : m2new;       // nothing seen yet: every power below is of -inf
-        const float alpha = fast_exp2(m2 - ref);
-        if (__builtin_amdgcn_ballot_w64(m2new > m2) != 0) {
+        u32x4 hi[QB], lo[QB];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) oacc[i] *= alpha;
+        for (int c = 0; c < QB; ++c) {
+            const f32x4 (&sc)[2] = sacc[c];
+            float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+            mx = max_xor32(max_xor16(mx));
+            const float m2new = fmaxf(m2[c], mx);
+            const float ref = m2new == -INFINITY ? 0.0f : m2new;       // nothing seen yet: every power below is of -inf
+            const float alpha = fast_exp2(m2[c] - ref);
+            if (__builtin_amdgcn_ballot_w64(m2new > m2[c]) != 0) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) oacc[c][i] *= alpha;
+            }
+            m2[c] = m2new;
+            float pv[8], psum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                pv[i] = fast_exp2(sc[i >> 2][i & 3] - ref);
+                psum += pv[i];
+            }
+            lsum[c] = lsum[c] * alpha + psum;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                hi[c][i] = pack_bf16(pv[2 * i], pv[2 * i + 1]);
+                lo[c][i] = pack_bf16(pv[2 * i] - bf16_lo(hi[c][i]), pv[2 * i + 1] - bf16_hi(hi[c][i]));
+            }
         }
-        m2 = m2new;
-        float pv[8], psum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            pv[i] = fast_exp2(sacc[i >> 2][i & 3] - ref);
-            psum += pv[i];
-        }
-        lsum = lsum * alpha + psum;
-        u32x4 hi, lo;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            hi[i] = pack_bf16(pv[2 * i], pv[2 * i + 1]);
-            lo[i] = pack_bf16(pv[2 * i] - bf16_lo(hi[i]), pv[2 * i + 1] - bf16_hi(hi[i]));
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {                // columns 2c and 2c + 1 of V's 8x8 piece, transposed
+        for (int n = 0; n < 4; ++n) {                // columns 2n and 2n + 1 of V's 8x8 piece, transposed
             u32x4 even, odd;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                even[i] = __builtin_amdgcn_perm(v[2 * i + 1][c], v[2 * i][c], 0x05040100u);
-                odd[i] = __builtin_amdgcn_perm(v[2 * i + 1][c], v[2 * i][c], 0x07060302u);
+                even[i] = __builtin_amdgcn_perm(v[2 * i + 1][n], v[2 * i][n], 0x05040100u);
+                odd[i] = __builtin_amdgcn_perm(v[2 * i + 1][n], v[2 * i][n], 0x07060302u);
             }
-            oacc[2 * c] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), __builtin_bit_cast(bf16x8, hi), oacc[2 * c]);
-            oacc[2 * c] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), __builtin_bit_cast(bf16x8, lo), oacc[2 * c]);
-            oacc[2 * c + 1] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), __builtin_bit_cast(bf16x8, hi), oacc[2 * c + 1]);
-            oacc[2 * c + 1] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), __builtin_bit_cast(bf16x8, lo), oacc[2 * c + 1]);
+#pragma unroll
+            for (int c = 0; c < QB; ++c) {
+                oacc[c][2 * n] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), __builtin_bit_cast(bf16x8, hi[c]), oacc[c][2 * n]);
+                oacc[c][2 * n] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, even), __builtin_bit_cast(bf16x8, lo[c]), oacc[c][2 * n]);
+                oacc[c][2 * n + 1] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), __builtin_bit_cast(bf16x8, hi[c]), oacc[c][2 * n + 1]);
+                oacc[c][2 * n + 1] = mfma_16x16x32_bf16(__builtin_bit_cast(bf16x8, odd), __builtin_bit_cast(bf16x8, lo[c]), oacc[c][2 * n + 1]);
+            }
         }
     };
 
@@ -403,8 +437,10 @@ __global__ __launch_bounds__(paged::THREADS, 2) void paged_decode_kernel(const p
     // One way out, behind both halves' loads: with one between them the compiler would take s1's for the last ones made, and wait for
     // s0's with them.
     do {
+        if constexpr (AGAIN) __builtin_amdgcn_s_barrier();
         load(s1);
         compute(s0);
+        if constexpr (AGAIN) __builtin_amdgcn_s_barrier();
         load(s0);
         if (s1.live) compute(s1);
     } while (s0.live);
@@ -422,13 +458,14 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged::Args a) {
     const int b = blockIdx.x / (unsigned)a.Hq, qh = blockIdx.x % (unsigned)a.Hq;
     const int2 plan = a.plan[b];
     const int share = a.plan[a.B].x;
-    const int kvh = qh / a.G, inner = qh % a.G, hb = kvh * a.blocks + inner / 16, per = min(16, a.G);
+    const int kvh = qh / a.G, inner = qh % a.G, block = a.per < a.G ? inner / a.per : 0;
+    const int hb = a.apart > 1 ? kvh * a.apart + block : kvh, beside = a.beside > 1 ? block : 0;
     // the waves that had a part of this head's steps
     const int first = plan.x + hb * (plan.y + TURN), w0 = first / share, S = min((first + plan.y - 1) / share, a.shares - 1) - w0 + 1;
     if (S < 2) return;
     const int t = threadIdx.x, c = t % TPS, sg = t / TPS;
     // of the first wave: the head that goes on behind it; of the others the one that began before them
-    auto slot_of = [&](int i) { return (size_t)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * per + inner % 16; };
+    auto slot_of = [&](int i) { return (size_t)(2 * ((w0 + i) * a.beside + beside) + (i == 0 ? 1 : 0)) * a.per + inner - block * a.per; };
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.0f;
     for (int s0 = sg; s0 < S; s0 += 4 * CG) {
@@ -481,11 +518,12 @@ __global__ __launch_bounds__(256) void paged_join_few_kernel(const paged::Args a
     if (b >= a.B) return;
     const int2 plan = a.plan[b];
     const int share = a.plan[a.B].x;
-    const int kvh = qh / a.G, inner = qh % a.G, hb = kvh * a.blocks + inner / 16, per = min(16, a.G);
+    const int kvh = qh / a.G, inner = qh % a.G, block = a.per < a.G ? inner / a.per : 0;
+    const int hb = a.apart > 1 ? kvh * a.apart + block : kvh, beside = a.beside > 1 ? block : 0;
     const int first = plan.x + hb * (plan.y + TURN), w0 = first / share, S = min((first + plan.y - 1) / share, a.shares - 1) - w0 + 1;
     if (S < 2) return;
     const int lane = threadIdx.x & 63, c = lane % TPS, sg = lane / TPS;
-    auto slot_of = [&](int i) { return (size_t)(2 * (w0 + i) + (i == 0 ? 1 : 0)) * per + inner % 16; };
+    auto slot_of = [&](int i) { return (size_t)(2 * ((w0 + i) * a.beside + beside) + (i == 0 ? 1 : 0)) * a.per + inner - block * a.per; };
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.0f;
     for (int s0 = 0; s0 < S; s0 += 4 * CG) {
@@ -620,33 +658,46 @@ __global__ __launch_bounds__(256) void paged_rope_append_kernel(const paged::App
 
 // ------------------------------------------------------------------------------------------
 namespace {
-struct Grid { int heads, per, shares; uint64_t waves; };      // kv heads times blocks of 16 query heads; heads of a slot; waves of the launch
-Grid paged_grid(int64_t B, int Hq, int Hkv, int64_t cap, int64_t window, int64_t sinks) {
+struct Grid { int per, apart, beside, shares; uint64_t groups; };         // as in Args; workgroups of the launch
+Grid paged_grid(int64_t B, int Hq, int Hkv, int D, int e4m3, int64_t cap, int64_t window, int64_t sinks) {
     using namespace paged;
-    const int G = Hq / Hkv, heads = Hkv * ((G + 15) / 16);
     // a window and the sinks may each begin and end inside a tile
     const int64_t rows = window > 0 ? std::min(cap, window + 2 * TILE + sinks + 2 * TILE) : cap;
     const int64_t steps = std::max<int64_t>(1, (rows + STEP - 1) / STEP);
-    Grid g{heads, std::min(G, 16), 0, (uint64_t)B * heads};
+    const int G = Hq / Hkv;
+    Grid g{std::min(G, 16), (G + 15) / 16, 1, 0, 0};
+    if (G > 16) {
+        if (D == 128 && !e4m3) {
+            if (steps > WHOLE && g.apart <= SIDE_BY_SIDE) g.beside = g.apart, g.apart = 1;
+        } else if (B * Hkv * g.apart * steps >= WIDE) {
+            g.per = std::min(G, 32), g.apart = (G + 31) / 32;
+        }
+    }
+    g.groups = (uint64_t)B * Hkv * g.apart;
     if (steps > WHOLE) {
-        g.shares = (int)std::min<int64_t>(SHARES, (B * heads * (steps + TURN) + MIN_SHARE - 1) / MIN_SHARE);
-        g.waves = g.shares + 1;
+        const int64_t most = g.beside == 1 ? SHARES : std::min(SHARES / 2, 256 * (8 / g.beside));
+        g.shares = (int)std::min<int64_t>(most, ((int64_t)g.groups * (steps + TURN) + MIN_SHARE - 1) / MIN_SHARE);
+        g.groups = g.shares + 1;
     }
     return g;
 }
+size_t plan_bytes(int B) { return ((size_t)(B + 1) * sizeof(int2) + 15) / 16 * 16; }
 }  // namespace
 
 size_t paged_decode_workspace_bytes(int B, int Hq, int Hkv, int D, int64_t cap) {
-    const Grid g = paged_grid(B, Hq, Hkv, cap, 0, 0);       // with a window there are as many waves at most
-    if (!g.shares) return 0;
-    return (size_t)g.shares * 2 * g.per * (D + 2) * sizeof(float) + ((size_t)(B + 1) * sizeof(int2) + 15) / 16 * 16;
+    size_t most = 0;                                        // of both formats; a window makes it no more
+    for (int e4m3 = 0; e4m3 < 2; ++e4m3) {
+        const Grid g = paged_grid(B, Hq, Hkv, D, e4m3, cap, 0, 0);
+        if (g.shares) most = std::max(most, plan_bytes(B) + (size_t)g.shares * g.beside * 2 * g.per * (D + 2) * sizeof(float));
+    }
+    return most;
 }
 
 int launch_paged_decode(const void* q, const void* k_pages, const void* v_pages, const int* page_table, const int* kv_lens,
                         const float* k_scale, const float* v_scale, void* o, float* lse, int B, int Hq, int Hkv, int D, int pages,
                         int page_size, int width, int window, int sinks, int e4m3, float scale, void* workspace, hipStream_t stream) {
     using namespace paged;
-    const Grid g = paged_grid(B, Hq, Hkv, (int64_t)width * page_size, window, sinks);
+    const Grid g = paged_grid(B, Hq, Hkv, D, e4m3, (int64_t)width * page_size, window, sinks);
     Args a{};
     a.q = static_cast<const uint16_t*>(q);
     a.k = k_pages, a.v = v_pages;
@@ -655,22 +706,26 @@ int launch_paged_decode(const void* q, const void* k_pages, const void* v_pages,
     a.o = static_cast<uint16_t*>(o), a.lse = lse;
     if (g.shares) {
         a.plan = static_cast<int2*>(workspace);
-        a.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + ((size_t)(B + 1) * sizeof(int2) + 15) / 16 * 16);
-        a.part_m = a.part_o + (size_t)g.shares * 2 * g.per * D;
-        a.part_l = a.part_m + (size_t)g.shares * 2 * g.per;
+        const size_t slots = (size_t)g.shares * g.beside * 2 * g.per;
+        a.part_o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + plan_bytes(B));
+        a.part_m = a.part_o + slots * D;
+        a.part_l = a.part_m + slots;
     }
-    a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv, a.blocks = (a.G + 15) / 16;
+    a.B = B, a.Hq = Hq, a.Hkv = Hkv, a.G = Hq / Hkv;
+    a.per = g.per, a.apart = g.apart, a.beside = g.beside;
     a.width = width, a.page_tiles = page_size / TILE, a.pages = pages;
     a.cap = width * page_size, a.window = window, a.sinks = sinks, a.shares = g.shares;
     a.scale_log2 = scale * LOG2E;
-    const dim3 grid((unsigned)((g.waves + WAVES - 1) / WAVES));
-    auto kernel = D == 128 ? (e4m3 ? &paged_decode_kernel<128, true> : &paged_decode_kernel<128, false>)
-                           : (e4m3 ? &paged_decode_kernel<64, true> : &paged_decode_kernel<64, false>);
-    launch_kernel(kernel, grid, dim3(THREADS), 0, stream, a);
+    auto pick = [&](auto qb) {
+        return D == 128 ? &paged_decode_kernel<128, true, qb(), false> : e4m3 ? &paged_decode_kernel<64, true, qb(), false> : &paged_decode_kernel<64, false, qb(), false>;
+    };
+    auto kernel = D == 128 && !e4m3 ? (g.beside > 1 ? &paged_decode_kernel<128, false, 1, true> : &paged_decode_kernel<128, false, 1, false>)
+                                    : g.per > 16 ? pick(std::integral_constant<int, 2>{}) : pick(std::integral_constant<int, 1>{});
+    launch_kernel(kernel, dim3((unsigned)g.groups), dim3(64 * g.beside), 0, stream, a);
     if (hipGetLastError() != hipSuccess) return -1;
     if (!g.shares) return 0;
     const size_t heads = (size_t)B * Hq;
-    if ((int64_t)B * g.heads < MANY_HEADS)
+    if ((int64_t)B * Hkv * g.apart * g.beside < MANY_HEADS)
         launch_kernel(D == 128 ? &paged_join_kernel<128> : &paged_join_kernel<64>, dim3((unsigned)heads), dim3(256), 0, stream, a);
     else
         launch_kernel(D == 128 ? &paged_join_few_kernel<128> : &paged_join_few_kernel<64>, dim3((unsigned)((heads + 3) / 4)), dim3(256), 0, stream, a);
