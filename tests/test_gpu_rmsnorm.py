@@ -142,6 +142,14 @@ def test_backward(rows, d):
         assert all(torch.equal(a, b) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("rows,d", [(1, 2560), (2, 2056), (3, 2304), (4, 2560), (771, 2088), (1601, 2560), (1, 5120), (257, 4104), (4095, 4616), (4097, 5120)])
+def test_backward_of_rows_of_five_and_ten_waves(rows, d):
+    import tyr_amd
+    (h, g, dr), w = _data(rows, d, 14, 3)
+    for r in (dr, None):
+        _check_grads(tyr_amd.rmsnorm_residual_bwd(g, h, w, 1e-6, d_resid=r), g, h, w, 1e-6, r)
+
+
 @pytest.mark.parametrize("d", [64, 1000, 16384])
 @pytest.mark.parametrize("size", [1e-15, 1e15])
 def test_backward_of_large_and_small_rows(d, size):

@@ -160,7 +160,7 @@ __global__ __launch_bounds__(S::THREADS) void rmsnorm_residual_kernel(
     }
 }
 
-// Gradients.  Workgroups of 16 waves: as many row slots as fit, slot s of workgroup i takes the rows ROWS (i + k gridDim.x) + s, the
+// Gradients.  Workgroups of 16 waves (or as many of them as whole rows need): as many row slots as fit, slot s of workgroup i takes the rows ROWS (i + k gridDim.x) + s, the
 // next one's loads under way while it works on one, and keeps dw of its rows in registers.  The slots are added through LDS at the
 // end, half of them to the other half at a time, and the workgroup writes one row of part [gridDim.x][d_model].
 // 65536 x 1024 85 us of reading and writing 537 MB and 5 us for the parts; 2000 x 4096 12.5 and 3.  (1024 workgroups of four waves: 91 and
@@ -268,9 +268,10 @@ __global__ __launch_bounds__(1024) void rmsnorm_residual_bwd_kernel(
         now = next;
     }
 #pragma unroll
-    for (int half = ROWS / 2; half > 0; half /= 2) {
+    for (int n = ROWS; n > 1; n = (n + 1) / 2) {
+        const int half = (n + 1) / 2;
         __syncthreads();
-        if (slot >= half && slot < 2 * half)
+        if (slot >= half && slot < n)
 #pragma unroll
             for (int p = 0; p < P; ++p)
                 if (has[p]) {
@@ -279,7 +280,7 @@ __global__ __launch_bounds__(1024) void rmsnorm_residual_bwd_kernel(
                     s[1] = f32x4{dw[p][4], dw[p][5], dw[p][6], dw[p][7]};
                 }
         __syncthreads();
-        if (slot < half)
+        if (slot < n - half)
 #pragma unroll
             for (int p = 0; p < P; ++p)
                 if (has[p]) {
@@ -320,7 +321,8 @@ __global__ __launch_bounds__(256) void rmsnorm_dweight_kernel(const float* __res
 
 // ------------------------------------------------------------------------------------------
 namespace {
-// Of the backward: one piece a lane, whose values, weights and sums fill the registers, as long as 16 waves hold a row so.
+// Of the backward: one piece a lane, whose values, weights and sums fill the registers, as long as 16 waves hold a row so.  Of waves without
+// work there are fewer with five to a row (22880 x 2080 87 us with eight, 69 so; 1000 x 2560 10.1, 10.5) and ten, two workgroups a CU.
 template <class F>
 void with_bwd_shape(int d_model, F go) {
     using namespace rms;
@@ -330,7 +332,9 @@ void with_bwd_shape(int d_model, F go) {
     else if (d_model <= 512) go(Shape<64, 1, 1>{});
     else if (d_model <= 1024) go(Shape<64, 2, 1>{});
     else if (d_model <= 2048) go(Shape<64, 4, 1>{});
+    else if (d_model <= 2560) go(Shape<64, 5, 1>{});
     else if (d_model <= 4096) go(Shape<64, 8, 1>{});
+    else if (d_model <= 5120) go(Shape<64, 10, 1>{});
     else if (d_model <= 8192) go(Shape<64, 16, 1>{});
     else go(Shape<64, 16, 2>{});
 }
@@ -348,12 +352,13 @@ void with_shape(int d_model, F go) {
     else go(Shape<64, 16, 2>{});
 }
 
-// workgroups of a backward: parts of dw
+// workgroups of a backward: parts of dw.  One a CU; of ten waves two, where the rows outweigh the parts (5700 x 4400 51.7 us with one, 47.5 so;
+// 2000 x 5120 20.0, 21.2).
 template <class S>
 size_t bwd_parts(size_t rows) {
     constexpr int ROWS = 1024 / (S::LPR * S::WPR);
-    const size_t groups = (rows + ROWS - 1) / ROWS;
-    return groups < 256 ? groups : 256;
+    const size_t groups = (rows + ROWS - 1) / ROWS, most = S::WPR == 10 && rows >= 4096 ? 512 : 256;
+    return groups < most ? groups : most;
 }
 }  // namespace
 
@@ -398,9 +403,10 @@ int launch_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const vo
     with_bwd_shape(d_model, [&](auto shape) {
         using S = decltype(shape);
         parts = bwd_parts<S>(rows);
-        const size_t lds = (size_t)(512 / (S::LPR * S::WPR)) * d_model * sizeof(float);        // at most 32 KB
+        constexpr int ROWS = 1024 / (S::LPR * S::WPR);
+        const size_t lds = (size_t)(ROWS / 2) * d_model * sizeof(float);        // at most 32 KB
         auto go = [&](auto in_cache, auto with_resid) {
-            launch_kernel((rmsnorm_residual_bwd_kernel<S, in_cache(), with_resid()>), dim3((unsigned)parts), dim3(1024), lds, stream,
+            launch_kernel((rmsnorm_residual_bwd_kernel<S, in_cache(), with_resid()>), dim3((unsigned)parts), dim3(S::LPR * S::WPR * ROWS), lds, stream,
                           static_cast<const uint16_t*>(d_out), static_cast<const uint16_t*>(d_resid), static_cast<const uint16_t*>(resid),
                           static_cast<const uint16_t*>(weight), static_cast<uint16_t*>(dx), static_cast<float*>(workspace), rows, d_model, eps);
         };
