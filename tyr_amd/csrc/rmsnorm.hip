@@ -168,7 +168,7 @@ __global__ __launch_bounds__(S::THREADS) void rmsnorm_residual_kernel(
 template <class S, bool CACHED, bool RESID>
 __global__ __launch_bounds__(1024) void rmsnorm_residual_bwd_kernel(
     const uint16_t* __restrict__ d_out, const uint16_t* __restrict__ d_resid, const uint16_t* __restrict__ resid,
-    const uint16_t* __restrict__ weight, uint16_t* __restrict__ dx, float* __restrict__ dw_part, size_t rows, int d_model, float eps) {
+    const uint16_t* __restrict__ weight, uint16_t* __restrict__ dx, float* __restrict__ dw_part, uint16_t* __restrict__ dw_out, size_t rows, int d_model, float eps) {
     using namespace rms;
     constexpr int LPR = S::LPR, WPR = S::WPR, P = S::P, ROWS = 1024 / (LPR * WPR);
     __shared__ float2 part[2][ROWS][WPR];
@@ -292,7 +292,8 @@ __global__ __launch_bounds__(1024) void rmsnorm_residual_bwd_kernel(
     if (slot == 0)
 #pragma unroll
         for (int p = 0; p < P; ++p)
-            if (has[p]) {
+            if (has[p] && dw_out) st_global_16(dw_out + pc[p], pack8(dw[p]));      // the only workgroup
+            else if (has[p]) {
                 f32x4* s = reinterpret_cast<f32x4*>(dw_part + (size_t)blockIdx.x * d_model + pc[p]);
                 s[0] = f32x4{dw[p][0], dw[p][1], dw[p][2], dw[p][3]};
                 s[1] = f32x4{dw[p][4], dw[p][5], dw[p][6], dw[p][7]};
@@ -352,12 +353,15 @@ void with_shape(int d_model, F go) {
     else go(Shape<64, 16, 2>{});
 }
 
+// Rows of so many groups at most are one workgroup's, which then has dw: 2 rows of 2048 5.7 us by two launches, 3.3 so; two groups 5.9, 4.5;
+// three 5.7, 6.7.
+constexpr size_t ALONE = 2;
 // workgroups of a backward: parts of dw.  One a CU; of ten waves two, where the rows outweigh the parts (5700 x 4400 51.7 us with one, 47.5 so;
 // 2000 x 5120 20.0, 21.2).
 template <class S>
 size_t bwd_parts(size_t rows) {
     constexpr int ROWS = 1024 / (S::LPR * S::WPR);
-    const size_t groups = (rows + ROWS - 1) / ROWS, most = S::WPR == 10 && rows >= 4096 ? 512 : 256;
+    const size_t groups = (rows + ROWS - 1) / ROWS, most = groups <= ALONE ? 1 : S::WPR == 10 && rows >= 4096 ? 512 : 256;
     return groups < most ? groups : most;
 }
 }  // namespace
@@ -408,12 +412,14 @@ int launch_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const vo
         auto go = [&](auto in_cache, auto with_resid) {
             launch_kernel((rmsnorm_residual_bwd_kernel<S, in_cache(), with_resid()>), dim3((unsigned)parts), dim3(S::LPR * S::WPR * ROWS), lds, stream,
                           static_cast<const uint16_t*>(d_out), static_cast<const uint16_t*>(d_resid), static_cast<const uint16_t*>(resid),
-                          static_cast<const uint16_t*>(weight), static_cast<uint16_t*>(dx), static_cast<float*>(workspace), rows, d_model, eps);
+                          static_cast<const uint16_t*>(weight), static_cast<uint16_t*>(dx), static_cast<float*>(workspace),
+                          parts == 1 ? static_cast<uint16_t*>(dweight) : nullptr, rows, d_model, eps);
         };
         if (d_resid) { if (cached) go(std::true_type{}, std::true_type{}); else go(std::false_type{}, std::true_type{}); }
         else { if (cached) go(std::true_type{}, std::false_type{}); else go(std::false_type{}, std::false_type{}); }
     });
     if (hipGetLastError() != hipSuccess) return -1;
+    if (parts == 1) return 0;
     launch_kernel(rmsnorm_dweight_kernel, dim3((unsigned)((d_model + 31) / 32)), dim3(256), 0, stream, static_cast<const float*>(workspace),
                   static_cast<uint16_t*>(dweight), (int)parts, d_model);
     return hipGetLastError() == hipSuccess ? 0 : -1;
