@@ -492,6 +492,44 @@ def test_captured_step_follows_lengths_and_pages():
         assert torch.equal(o, want[0]) and torch.equal(lse, want[1]) and torch.equal(kg, ke) and torch.equal(vg, ve), replay
 
 
+@pytest.mark.parametrize("Hq,D,e4m3,width", [(32, 128, False, 200), (33, 128, False, 200), (32, 128, True, 9000), (40, 64, False, 9000), (32, 128, True, 200)])
+def test_captured_decode_of_many_query_heads(Hq, D, e4m3, width):
+    """One captured call replayed, on a side stream too, while lengths and the table change in place; pages that are not there, NaN in
+    rows that are not seen."""
+    import tyr_amd
+    B, page, full = 64, 16, 200 * 16
+    g = _gen(31 + Hq)
+    (k, v), table, ks, vs = _cache(g, [full] * B, page, 1, D, e4m3, width=width)
+    table[3, 5], table[4, :200] = -7, k.shape[0]
+    k[table[6, 1].long(), :, 9:] = float("nan")      # behind 25 rows of sequence 6
+    v[table[6, 1].long(), :, 9:] = float("nan")
+    q = torch.randn(B, Hq, 1, D, generator=g, device="cuda").bfloat16()
+    lens = torch.full((B,), 25, dtype=torch.int32, device="cuda")
+
+    def call(**kw):
+        return tyr_amd.paged_decode(q, k, v, table, lens, k_scale=ks, v_scale=vs, **kw)
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, lse = call()
+    side = torch.cuda.Stream()
+    for replay, (shortest, longest) in enumerate(((25, 25), (0, full), (full - 40, full), (0, 70), (0, full))):
+        n = torch.randint(shortest, longest + 1, (B,), generator=g, device="cuda", dtype=torch.int32)
+        n[6] = 25
+        lens.copy_(n)
+        want = call()
+        side.wait_stream(torch.cuda.current_stream())
+        beside = call(stream=side)
+        o.zero_()
+        lse.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for got in ((o, lse), beside):
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), replay
+        _check(o, lse, q, k, v, table, lens.tolist(), 1 / math.sqrt(D), ks=ks, vs=vs, only=(0, 3, 4, 5, 6, 63))
+
+
 def test_on_a_side_stream():
     import tyr_amd
     g = _gen(22)

@@ -14,7 +14,7 @@
 //   32 sequences of 8192 bf16 rows 182, 172 so.)
 //   Heads that several waves have a part of are joined by a second launch from partial results (O, m, l), as
 //     m = max m_s ; l = sum l_s 2^(m_s-m) ; O = sum O_s 2^(m_s-m) / l ; LSE = ln l + m ln 2.
-// HBM-bound: each visible row of K and V is read once a block of query heads, straight into MFMA operand registers (16x16x32 bf16):
+// HBM-bound: each visible row of K and V is read once a block of 16 query heads, or two, straight into MFMA operand registers (16x16x32 bf16):
 //   S^T (16 rows x 16 q) = K x Q^T and O^T_j (16 d x 16 q) += V^T x P^T, j = 0..7, the layouts of the contiguous decode:
 //   lane l = (x = l % 16, g = l / 16) holds row x of K and, of V, the columns 8x..8x+7 of the rows 4g..4g+3 whose probabilities the
 //   accumulator of S^T leaves in it, so P^T needs no movement; V is transposed 8x8 in registers.
@@ -437,7 +437,7 @@ __global__ __launch_bounds__(64 * (AGAIN ? paged::SIDE_BY_SIDE : 1), 2) void pag
     // One way out, behind both halves' loads: with one between them the compiler would take s1's for the last ones made, and wait for
     // s0's with them.
     do {
-        if constexpr (AGAIN) __builtin_amdgcn_s_barrier();
+        if constexpr (AGAIN) __builtin_amdgcn_s_barrier();       // the waves side by side ask for the same rows together
         load(s1);
         compute(s0);
         if constexpr (AGAIN) __builtin_amdgcn_s_barrier();
