@@ -18,8 +18,8 @@
 //   S^T (16 rows x 16 q) = K x Q^T and O^T_j (16 d x 16 q) += V^T x P^T, j = 0..7, the layouts of the contiguous decode:
 //   lane l = (x = l % 16, g = l / 16) holds row x of K and, of V, the columns 8x..8x+7 of the rows 4g..4g+3 whose probabilities the
 //   accumulator of S^T leaves in it, so P^T needs no movement; V is transposed 8x8 in registers.
-//   P is given as bf16 twice, its rounding and what that left: products with the second cost matrix time that is idle here, and
-//   the result is as exact as with f32 probabilities.
+//   P is given as bf16 twice, its rounding and what that left (below 2^-16 of it is lost): products with the second cost matrix time that
+//   is idle here, and the result is as exact as with f32 probabilities.
 #include "common.hpp"
 #include "launch.hpp"
 
@@ -139,6 +139,8 @@ template <bool AGAIN> __device__ __forceinline__ u32x4 load_tile_16(__amdgpu_buf
 template <bool AGAIN> __device__ __forceinline__ u32x2 load_tile_8(__amdgpu_buffer_rsrc_t t, int at) {
     return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(t, at, 0, AGAIN ? 0 : 2));
 }
+
+__device__ __forceinline__ float last_bit_set(float x) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) | 1u); }
 
 __device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t four, bool upper) {
     const bf16x2 r = upper ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(four, 1.0f, false);
@@ -408,7 +410,15 @@ __global__ __launch_bounds__(64 * (AGAIN ? paged::SIDE_BY_SIDE : 1), 2) void pag
             lsum[c] = lsum[c] * alpha + psum;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                hi[c][i] = pack_bf16(pv[2 * i], pv[2 * i + 1]);
+                if constexpr (FP8) {
+                    hi[c][i] = pack_bf16(pv[2 * i], pv[2 * i + 1]);
+                } else {
+                    // bf16 V may be infinite, so both parts of a probability are positive: the first rounded down, the other not 0 (the
+                    // least bit of the 24 is set).  Rounded to nearest, the other is 0 or negative half of the time, and inf + 0 inf is NaN.
+                    pv[2 * i] = last_bit_set(pv[2 * i]);
+                    pv[2 * i + 1] = last_bit_set(pv[2 * i + 1]);
+                    hi[c][i] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, pv[2 * i + 1]), __builtin_bit_cast(uint32_t, pv[2 * i]), 0x07060302u);
+                }
                 lo[c][i] = pack_bf16(pv[2 * i] - bf16_lo(hi[c][i]), pv[2 * i + 1] - bf16_hi(hi[c][i]));
             }
         }
