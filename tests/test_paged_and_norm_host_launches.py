@@ -1,0 +1,77 @@
+"""What the host code of the paged and RMS norm entry points decides, on the CPU: as tests/test_host_launches.py, every signed overflow an
+abort, launches recorded instead of made (tests/host_launches)."""
+import os
+import re
+import subprocess
+from concurrent.futures import ThreadPoolExecutor
+
+import pytest
+
+from tests.test_host_launches import CHECKED, ROOT
+
+SHAPE, WS = "-2", "-5"
+
+
+@pytest.fixture(scope="module")
+def ask(tmp_path_factory):
+    tmp = tmp_path_factory.mktemp("host")
+
+    def compile_(name):
+        obj = str(tmp / (name + ".o"))
+        subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "--offload-host-only", "-O1", "-std=c++17", "-w", *CHECKED, "-c",
+                               os.path.join(ROOT, "tyr_amd", "csrc", name + ".hip"), "-o", obj])
+        return obj
+    with ThreadPoolExecutor() as pool:
+        objs = list(pool.map(compile_, ("capi", "paged", "rmsnorm")))
+    main, exe = str(tmp / "recorder.o"), str(tmp / "recorder")
+    subprocess.check_call(["g++", "-O1", "-std=c++17", "-D__HIP_PLATFORM_AMD__=1", "-isystem", "/opt/rocm/include", "-c",
+                           os.path.join(ROOT, "tests", "host_launches", "paged_recorder.cpp"), "-o", main])
+    # what the other kernel files and the fat binaries would define is never reached
+    subprocess.check_call(["/opt/rocm/llvm/bin/clang++", main, *objs, "-fsanitize=signed-integer-overflow", "-fsanitize-minimal-runtime",
+                           "-Wl,--unresolved-symbols=ignore-all", "-o", exe])
+
+    def run(lines):
+        r = subprocess.run([exe], input="\n".join(lines) + "\n", capture_output=True, text=True)
+        got = r.stdout.splitlines()
+        assert r.returncode == 0 and len(got) == len(lines), (lines[min(len(got), len(lines) - 1)], r.returncode, r.stderr[-300:])
+        return got
+    return run
+
+
+def test_the_scratch_query_knows_the_shapes_that_a_call_refuses(ask):
+    """It overflowed for some and asked for terabytes; callers allocate by it before the call can refuse."""
+    shapes = [(1, 2147483633, 1, 128, 16, 100), (1, 2147483632, 1, 128, 16, 100), (1, 2 ** 31 - 1, 1, 64, 16, 1), (1, 1 << 26, 1, 64, 16, 1),
+              (1 << 26, 1, 1, 64, 16, 1), (2 ** 31 - 1, 1, 1, 128, 16, 1), (1 << 16, 1, 1, 128, 16, 1 << 15), (1, 1, 1, 128, 16, (1 << 27) - 1),
+              (16, 1, 1, 128, 16, (1 << 27) - 1), (1 << 25, 1, 1, 128, 16, 60), (1 << 12, 1 << 13, 1, 64, 16, 1 << 12), (3, 34, 2, 64, 48, 999)]
+    for s in shapes:
+        need, = ask([f"decode_bytes {' '.join(map(str, s))}"])
+        for e4m3 in (0, 1):
+            with_it, = ask([f"decode {' '.join(map(str, s))} 0 0 {e4m3} {int(need) or 1 << 50}"])
+            if with_it.startswith("0 "):
+                assert int(need) <= 1 << 33 and (int(need) == 0 or ask([f"decode {' '.join(map(str, s))} 0 0 {e4m3} {int(need) - 1}"]) == [WS])
+            else:
+                assert (with_it, need) == (SHAPE, "0"), s
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,Hkv", [(1, 1), (8, 2), (17, 1), (32, 1), (33, 1), (66, 2), (128, 1), (130, 1), (1200, 600)])
+def test_the_scratch_of_a_decode_holds_what_any_window_writes(ask, Hq, Hkv, D):
+    """The query knows neither the window nor the pages' format.  A launch of shares has one workgroup more than there are; a wave writes
+    at most two partial results of each of its query heads: D numbers, a maximum and a sum."""
+    G = Hq // Hkv
+    for B in (1, 3, 70, 2000):
+        for page, width in ((16, 1), (16, 16), (16, 17), (48, 30), (256, 40), (64, 2000)):
+            shape = f"{B} {Hq} {Hkv} {D} {page} {width}"
+            need, = ask([f"decode_bytes {shape}"])
+            calls = [f"decode {shape} {window} {sinks} {e4m3} {need}" for window in (0, 1, 100, 225, 1000, 1 << 40) for sinks in (0, 4, 300, 1 << 40)
+                     for e4m3 in (0, 1)]
+            for call, got in zip(calls, ask(calls)):
+                if got == SHAPE:                         # too many steps, whatever the window
+                    assert need == "0"
+                    continue
+                m = re.fullmatch(r"0 paged_decode_kernel<\d+,(?:true|false),(\d),(true|false)>:(\d+)( paged_join\w*<\d+>:\d+)?", got)
+                assert m, (call, got)
+                if m[4]:
+                    beside = -(-G // 16) if m[2] == "true" else 1
+                    waves = (int(m[3]) - 1) * beside
+                    assert int(need) >= 8 * (B + 1) + waves * 2 * min(G, 16 * int(m[1])) * (D + 2) * 4, (call, got)

@@ -466,6 +466,14 @@ static int page_extents(uint64_t B, uint64_t Hq, uint64_t Hkv, uint64_t D, uint6
         return TYR_HIP_ERR_BAD_SHAPE;
     return TYR_HIP_OK;
 }
+// what a decode asks of it beyond that, and its scratch query with it
+static int decode_extents(uint64_t B, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t num_pages, uint64_t page_size, uint64_t table_width) {
+    const int rc = page_extents(B, Hq, Hkv, D, num_pages, page_size, table_width);
+    if (rc != TYR_HIP_OK) return rc;
+    if (B * Hq >= (uint64_t)1 << 26) return TYR_HIP_ERR_BAD_SHAPE;            // waves of a launch
+    if (B * Hkv * ((Hq / Hkv + 15) / 16) > ((uint64_t)1 << 30) / (table_width * page_size / 32 + 8)) return TYR_HIP_ERR_BAD_SHAPE;      // steps of all heads
+    return TYR_HIP_OK;
+}
 // page scales belong to e4m3 pages
 static int page_format(int cache_dtype, const float* k_scale, const float* v_scale) {
     if (cache_dtype != TYR_HIP_CACHE_BF16 && cache_dtype != TYR_HIP_CACHE_E4M3) return TYR_HIP_ERR_UNSUPPORTED;
@@ -496,7 +504,7 @@ int tyr_hip_paged_rope_append(const void* q, const void* k_new, const void* v_ne
 }
 
 size_t tyr_hip_paged_decode_workspace_bytes(uint64_t B, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t page_size, uint64_t table_width) {
-    if (page_extents(B, Hq, Hkv, D, 1, page_size, table_width) != TYR_HIP_OK) return 0;
+    if (decode_extents(B, Hq, Hkv, D, 1, page_size, table_width) != TYR_HIP_OK) return 0;
     return tyr::paged_decode_workspace_bytes((int)B, (int)Hq, (int)Hkv, (int)D, (int64_t)(table_width * page_size));
 }
 
@@ -505,14 +513,12 @@ int tyr_hip_paged_decode(const void* q, const void* k_pages, const void* v_pages
                          uint64_t D, uint64_t num_pages, uint64_t page_size, uint64_t table_width, uint64_t window, uint64_t sinks,
                          int cache_dtype, float scale, void* workspace, size_t workspace_bytes, void* stream) {
     if (!q || !k_pages || !v_pages || !page_table || !kv_lens || !o) return TYR_HIP_ERR_NULL_POINTER;
-    int rc = page_extents(B, Hq, Hkv, D, num_pages, page_size, table_width);
+    int rc = decode_extents(B, Hq, Hkv, D, num_pages, page_size, table_width);
     if (rc != TYR_HIP_OK) return rc;
     rc = page_format(cache_dtype, k_scale, v_scale);
     if (rc != TYR_HIP_OK) return rc;
     if (!(scale > 0.0f) || scale > 3.0e38f) return TYR_HIP_ERR_UNSUPPORTED;
     const uint64_t cap = table_width * page_size;
-    if (B * Hq >= (uint64_t)1 << 26) return TYR_HIP_ERR_BAD_SHAPE;            // waves of a launch
-    if (B * Hkv * ((Hq / Hkv + 15) / 16) > ((uint64_t)1 << 30) / (cap / 32 + 8)) return TYR_HIP_ERR_BAD_SHAPE;      // steps of all heads
     if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(o) || !aligned4(page_table) || !aligned4(kv_lens) || !aligned4(lse))
         return TYR_HIP_ERR_MISALIGNED;
     const size_t need = tyr_hip_paged_decode_workspace_bytes(B, Hq, Hkv, D, page_size, table_width);
