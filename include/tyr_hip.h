@@ -476,7 +476,8 @@ int tyr_hip_paged_rope_append(const void* q, const void* k_new, const void* v_ne
  * between replays.  Results are reproducible for the same lengths.
  *   workspace : tyr_hip_paged_decode_workspace_bytes(...) bytes, 16-byte aligned, contents arbitrary; calls that overlap in time need
  *               one each (may be NULL where that is 0)
- * Supported additionally: B * Hq < 2^26; steps of 32 rows of all heads, counted with table_width * page_size rows a sequence, < 2^30.
+ * Supported additionally: B * Hq < 2^26; steps of 32 rows of all heads (a head: a kv head of a sequence and a block of 16 of its query
+ * heads), counted with table_width * page_size rows a sequence, < 2^30.
  */
 size_t tyr_hip_paged_decode_workspace_bytes(uint64_t B, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t page_size, uint64_t table_width);
 int tyr_hip_paged_decode(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table, const int32_t* kv_lens,

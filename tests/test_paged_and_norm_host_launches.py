@@ -75,3 +75,18 @@ def test_the_scratch_of_a_decode_holds_what_any_window_writes(ask, Hq, Hkv, D):
                     beside = -(-G // 16) if m[2] == "true" else 1
                     waves = (int(m[3]) - 1) * beside
                     assert int(need) >= 8 * (B + 1) + waves * 2 * min(G, 16 * int(m[1])) * (D + 2) * 4, (call, got)
+
+
+def test_a_decode_takes_every_shape_below_its_documented_limits(ask):
+    """B Hq < 2^26, and steps of 32 rows of all heads (blocks of 16 query heads) < 2^30: the rest is refused."""
+    for B, Hq, Hkv, page, width in ((1 << 25, 1, 1, 16, 60), (1 << 25, 1, 1, 16, 63), (1 << 25, 1, 1, 16, 62), (1 << 25, 2, 1, 16, 1), ((1 << 26) - 1, 1, 1, 16, 1),
+                                    (1 << 26, 1, 1, 16, 1), ((1 << 26) - 1, 1, 1, 16, 31), (1 << 16, 1, 1, 16, 1 << 15), ((1 << 16) - 1, 1, 1, 16, 1 << 15),
+                                    (15, 1, 1, 16, (1 << 27) - 1), (16, 1, 1, 16, (1 << 27) - 1), (15, 16, 1, 16, (1 << 27) - 1), (15, 17, 1, 16, (1 << 27) - 1),
+                                    (1, (1 << 26) - 1, 1, 16, 16), (7, 170, 17, 48, 1000)):
+        fits = B * Hq < 1 << 26 and B * Hkv * -(-(Hq // Hkv) // 16) * -(-page * width // 32) < 1 << 30
+        for D in (64, 128):
+            shape = f"{B} {Hq} {Hkv} {D} {page} {width}"
+            need, = ask([f"decode_bytes {shape}"])
+            for e4m3 in (0, 1):
+                got, = ask([f"decode {shape} 0 0 {e4m3} {need}"])
+                assert got.startswith("0 paged_decode_kernel") if fits else (got, need) == (SHAPE, "0"), (shape, got)

@@ -471,7 +471,8 @@ static int decode_extents(uint64_t B, uint64_t Hq, uint64_t Hkv, uint64_t D, uin
     const int rc = page_extents(B, Hq, Hkv, D, num_pages, page_size, table_width);
     if (rc != TYR_HIP_OK) return rc;
     if (B * Hq >= (uint64_t)1 << 26) return TYR_HIP_ERR_BAD_SHAPE;            // waves of a launch
-    if (B * Hkv * ((Hq / Hkv + 15) / 16) > ((uint64_t)1 << 30) / (table_width * page_size / 32 + 8)) return TYR_HIP_ERR_BAD_SHAPE;      // steps of all heads
+    // steps of all heads; with those that going from head to head counts as, three each, they are below 2^31
+    if (B * Hkv * ((Hq / Hkv + 15) / 16) * ((table_width * page_size + 31) / 32) >= (uint64_t)1 << 30) return TYR_HIP_ERR_BAD_SHAPE;
     return TYR_HIP_OK;
 }
 // page scales belong to e4m3 pages
