@@ -9,7 +9,7 @@ import pytest
 
 from tests.test_host_launches import CHECKED, ROOT
 
-SHAPE, WS = "-2", "-5"
+NULL, SHAPE, MISAL, WS = "-1", "-2", "-4", "-5"
 
 
 @pytest.fixture(scope="module")
@@ -90,3 +90,10 @@ def test_a_decode_takes_every_shape_below_its_documented_limits(ask):
             for e4m3 in (0, 1):
                 got, = ask([f"decode {shape} 0 0 {e4m3} {need}"])
                 assert got.startswith("0 paged_decode_kernel") if fits else (got, need) == (SHAPE, "0"), (shape, got)
+
+
+def test_row_scales_of_a_bf16_norm_are_not_looked_at(ask):
+    for residual in (0, 1):
+        assert ask([f"norm 4 64 {residual} 0 {at}" for at in (0, 2, 4096)]) == ask([f"norm 4 64 {residual} 0 0"]) * 3
+        assert ask([f"norm 4 64 {residual} 0 2"])[0].startswith("0 rmsnorm_residual_kernel")
+        assert ask([f"norm 4 64 {residual} 1 {at}" for at in (0, 2)]) == [NULL, MISAL]

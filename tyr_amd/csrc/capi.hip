@@ -428,7 +428,8 @@ int tyr_hip_rmsnorm_residual(const void* x, const void* residual, const void* we
     if ((out_dtype != TYR_HIP_OUT_BF16 && out_dtype != TYR_HIP_OUT_E4M3) || !(eps >= 0.0f)) return TYR_HIP_ERR_UNSUPPORTED;
     if (!tyr::rmsnorm_residual_fits((size_t)rows, (int)d_model)) return TYR_HIP_ERR_BAD_SHAPE;
     if (out_dtype == TYR_HIP_OUT_E4M3 && !row_scale) return TYR_HIP_ERR_NULL_POINTER;
-    if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(out) || !aligned16(out_resid) || !aligned4(row_scale))
+    if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(out) || !aligned16(out_resid) ||
+        (out_dtype == TYR_HIP_OUT_E4M3 && !aligned4(row_scale)))
         return TYR_HIP_ERR_MISALIGNED;
     rc = tyr::launch_rmsnorm_residual(x, residual, weight, out, out_resid, row_scale, (size_t)rows, (int)d_model, eps,
                                       out_dtype == TYR_HIP_OUT_E4M3, static_cast<hipStream_t>(stream));
