@@ -409,7 +409,8 @@ int tyr_hip_gemm_fp8_ws(const void* aq, const void* bq, void* c,
  *   out       = bf16(y)                                   out_dtype = TYR_HIP_OUT_BF16
  *   out       = e4m3(y / row_scale), row_scale = max |y| of the row / 448     out_dtype = TYR_HIP_OUT_E4M3
  * The e4m3 output and its row scales are the `aq` and `row_scale` of tyr_hip_gemm_fp8_ex.  A row whose largest |y| is below 2^-100
- * (a zero row among them) takes the scale 1.  Statistics are f32 over the whole row of the rounded out_resid.
+ * (a zero row among them) takes the scale 1.  Statistics are f32 over the whole row of the rounded out_resid; rows whose squares f32 does
+ * not hold (2^64 and more, or 2^-35 and less where eps is as small) are scaled by a power of two for them, here and in the gradients.
  *
  *   x, residual, out_resid : bf16 [rows, d_model]; residual and out_resid both given or both NULL; outputs overlap no input
  *   weight : bf16 [d_model]     out : bf16 or e4m3 [rows, d_model]     row_scale : f32 [rows] (e4m3), not looked at for bf16
