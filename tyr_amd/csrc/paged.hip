@@ -46,6 +46,7 @@ constexpr int SIDE_BY_SIDE = 8;             // of them at most: as many as have 
 constexpr int TURN = 3;                     // steps that going from one head to the next is counted as
 constexpr int MANY_HEADS = 64;              // heads of a launch from which one wave joins each, not four (1024 heads of 3-22 steps 40.7 us, 37.4 so;
                                             // with 8 heads of 128 parts four waves have more of them under way)
+constexpr int LONG = 32;                    // parts of a head up to which that is so
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -90,7 +91,7 @@ struct Args {
     const float *k_scale, *v_scale;
     uint16_t* o;
     float *lse, *part_o, *part_m, *part_l;
-    int2* plan;                             // [B] first step of each sequence's first head, steps of a head; [B]: steps of a wave
+    int2* plan;                             // [B] first step of each sequence's first head, steps of a head; [B]: steps of a wave, of the longest head
     int B, Hq, Hkv, G;                      // G = query heads of a kv head
     int per, apart, beside;                 // query heads of a block; blocks that are heads of their own; blocks of waves side by side
     int width, page_tiles, pages;           // pages of a table row; tiles of a page; pages of the pool
@@ -186,7 +187,7 @@ __global__ __launch_bounds__(64 * (AGAIN ? paged::SIDE_BY_SIDE : 1), 2) void pag
         // one wave more than there are shares writes down the plan, for the launch that joins
         const bool scribe = place == a.shares;
         if (scribe && side > 0) return;
-        if (scribe && lane == 0) a.plan[a.B] = int2{share, 0};
+        int longest = 0;                                 // steps of a head
         at = min((int64_t)place * share, (int64_t)all);
         end = min(at + share, all);
         if (!scribe && at >= end) return;
@@ -194,13 +195,19 @@ __global__ __launch_bounds__(64 * (AGAIN ? paged::SIDE_BY_SIDE : 1), 2) void pag
         int base = 0;
         for (;;) {
             const int upto = base + round.total() * heads, b0 = round.b0 + lane;
-            if (scribe) { if (b0 < a.B) a.plan[b0] = int2{base + (round.upto - round.steps - TURN) * heads, round.steps}; }
-            else if (at < upto) break;
+            if (scribe) {
+                if (b0 < a.B) a.plan[b0] = int2{base + (round.upto - round.steps - TURN) * heads, round.steps};
+                longest = max(longest, round.steps);
+            } else if (at < upto) break;
             base = upto;
             if (round.b0 + 64 >= a.B) break;
             round.read(a, round.b0 + 64, lane);
         }
-        if (scribe) return;
+        if (scribe) {
+            for (int d = 32; d > 0; d /= 2) longest = max(longest, __shfl_xor(longest, d));
+            if (lane == 0) a.plan[a.B] = int2{share, longest};
+            return;
+        }
         // the first lane whose sequence ends behind `at`; none if the lengths changed under the two readings of them
         const uint64_t behind = __builtin_amdgcn_ballot_w64(at < base + round.upto * heads);
         if (behind == 0 || at < base) return;
@@ -457,34 +464,39 @@ __global__ __launch_bounds__(64 * (AGAIN ? paged::SIDE_BY_SIDE : 1), 2) void pag
     finish(now, now_last);
 }
 
-// Joins the parts of a head: one workgroup per (sequence, query head), D/4 threads of 4 elements a part, several side by side.  It is all
-// latency, 3-4 us (m, l and the weights of 64 parts by the lanes of a wave instead, no serial step: as long).
-template <int D>
-__global__ __launch_bounds__(256) void paged_join_kernel(const paged::Args a) {
-    using namespace paged;
-    constexpr int TPS = D / 4, CG = 256 / TPS;
-    __shared__ f32x4 so[CG][TPS];
-    __shared__ float sm[CG], sl[CG];
-    const int b = blockIdx.x / (unsigned)a.Hq, qh = blockIdx.x % (unsigned)a.Hq;
-    const int2 plan = a.plan[b];
-    const int share = a.plan[a.B].x;
-    const int kvh = qh / a.G, inner = qh % a.G, block = a.per < a.G ? inner / a.per : 0;
-    const int hb = a.apart > 1 ? kvh * a.apart + block : kvh, beside = a.beside > 1 ? block : 0;
-    // the waves that had a part of this head's steps
-    const int first = plan.x + hb * (plan.y + TURN), w0 = first / share, S = min((first + plan.y - 1) / share, a.shares - 1) - w0 + 1;
-    if (S < 2) return;
-    const int t = threadIdx.x, c = t % TPS, sg = t / TPS;
+namespace paged {
+// The parts of a query head: the partial results of the waves that had some of its steps.
+struct Parts {
+    int w0, S, beside, inner;               // the first of the waves, their number; which of the waves side by side; the head's place in its block
+    size_t head;
+    __device__ __forceinline__ Parts(const Args& a, int b, int qh) {
+        const int2 plan = a.plan[b];
+        const int share = a.plan[a.B].x;
+        const int kvh = qh / a.G, block = a.per < a.G ? (qh - kvh * a.G) / a.per : 0;
+        inner = qh - kvh * a.G - block * a.per;
+        const int hb = a.apart > 1 ? kvh * a.apart + block : kvh;
+        beside = a.beside > 1 ? block : 0;
+        const int first = plan.x + hb * (plan.y + TURN);
+        w0 = first / share;
+        S = min((first + plan.y - 1) / share, a.shares - 1) - w0 + 1;
+        head = (size_t)b * a.Hq + qh;
+    }
     // of the first wave: the head that goes on behind it; of the others the one that began before them
-    auto slot_of = [&](int i) { return (size_t)(2 * ((w0 + i) * a.beside + beside) + (i == 0 ? 1 : 0)) * a.per + inner - block * a.per; };
+    __device__ __forceinline__ size_t slot(const Args& a, int i) const { return (size_t)(2 * ((w0 + i) * a.beside + beside) + (i == 0 ? 1 : 0)) * a.per + inner; }
+};
+// Four elements of O, and m and l, of parts g, g + groups, ...: four under way at a time.
+struct Sum { f32x4 o; float m, l; };
+template <int D>
+__device__ __forceinline__ Sum join_every(const Args& a, const Parts& p, int c, int g, int groups) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.0f;
-    for (int s0 = sg; s0 < S; s0 += 4 * CG) {
+    for (int s0 = g; s0 < p.S; s0 += 4 * groups) {
         f32x4 os[4];
         float ms[4], ls[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const size_t slot = slot_of(min(s0 + i * CG, S - 1));
-            ms[i] = s0 + i * CG < S ? a.part_m[slot] : -INFINITY;
+            const size_t slot = p.slot(a, min(s0 + i * groups, p.S - 1));
+            ms[i] = s0 + i * groups < p.S ? a.part_m[slot] : -INFINITY;
             ls[i] = a.part_l[slot];
             os[i] = *reinterpret_cast<const f32x4*>(a.part_o + slot * D + 4 * c);
         }
@@ -495,87 +507,92 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const paged::Args a) {
         m = mn;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (s0 + i * CG < S) {
+            if (s0 + i * groups < p.S) {
                 const float wgt = fast_exp2(ms[i] - ref);
                 o += os[i] * wgt;
                 l += ls[i] * wgt;
             }
     }
-    so[sg][c] = o;
-    if (c == 0) { sm[sg] = m; sl[sg] = l; }
+    return Sum{o, m, l};
+}
+template <int D>
+__device__ __forceinline__ void store_head(const Args& a, const Parts& p, int c, const Sum& t) {
+    const float inv = t.l == 0.0f ? 0.0f : 1.0f / t.l;
+    reinterpret_cast<u32x2*>(a.o + p.head * D)[c] = u32x2{pack_bf16(t.o[0] * inv, t.o[1] * inv), pack_bf16(t.o[2] * inv, t.o[3] * inv)};
+    if (a.lse && c == 0) a.lse[p.head] = t.l == 0.0f ? -INFINITY : logf(t.l) + t.m * LN2;
+}
+// A head by a workgroup of 256 threads: D/4 threads of 4 elements a part, several parts side by side.
+template <int D> struct Side { f32x4 o[1024 / D][D / 4]; float m[1024 / D], l[1024 / D]; };
+template <int D>
+__device__ __forceinline__ void join_by_all(const Args& a, const Parts& p, Side<D>& side) {
+    constexpr int TPS = D / 4, CG = 256 / TPS;
+    const int t = threadIdx.x, c = t % TPS, g = t / TPS;
+    Sum x = join_every<D>(a, p, c, g, CG);
+    side.o[g][c] = x.o;
+    if (c == 0) { side.m[g] = x.m; side.l[g] = x.l; }
     __syncthreads();
     if (t >= TPS) return;
-    const int n = min(CG, S);
+    const int n = min(CG, p.S);
     for (int i = 1; i < n; ++i) {
-        const float mn = fmaxf(m, sm[i]), ref = mn == -INFINITY ? 0.0f : mn, f = fast_exp2(m - ref), wgt = fast_exp2(sm[i] - ref);
-        o = o * f + so[i][c] * wgt;
-        l = l * f + sl[i] * wgt;
-        m = mn;
+        const float mn = fmaxf(x.m, side.m[i]), ref = mn == -INFINITY ? 0.0f : mn, f = fast_exp2(x.m - ref), wgt = fast_exp2(side.m[i] - ref);
+        x.o = x.o * f + side.o[i][c] * wgt;
+        x.l = x.l * f + side.l[i] * wgt;
+        x.m = mn;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const size_t head = (size_t)b * a.Hq + qh;
-    reinterpret_cast<u32x2*>(a.o + head * D)[c] = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
-    if (a.lse && c == 0) a.lse[head] = l == 0.0f ? -INFINITY : logf(l) + m * LN2;
+    store_head<D>(a, p, c, x);
+}
+}  // namespace paged
+
+// Joins the parts of a head: one workgroup per (sequence, query head).  It is all latency, 3-4 us (m, l and the weights of 64 parts by the
+// lanes of a wave instead, no serial step: as long).
+template <int D>
+__global__ __launch_bounds__(256) void paged_join_kernel(const paged::Args a) {
+    using namespace paged;
+    __shared__ Side<D> side;
+    const Parts p(a, blockIdx.x / (unsigned)a.Hq, blockIdx.x % (unsigned)a.Hq);
+    if (p.S >= 2) join_by_all<D>(a, p, side);
 }
 
-// The same with a wave a head, for launches of many heads, whose heads have few parts.
+// The same with a wave a head, for launches of many heads, most of which have few parts.  Where the longest head has more than LONG, what has
+// more is one for all waves of a workgroup after all, in workgroups far apart, so that the heads of a sequence do not wait for each other.  64
+// heads of 8 query heads each, one of 100000 rows and 63 of 20: 35.8 us, 84.8 with a wave for each; 64 of 1 to 32768 rows 33.0, 39.2.  It
+// costs 0.9 of 73 us where 2048 short sequences are joined.
 template <int D>
 __global__ __launch_bounds__(256) void paged_join_few_kernel(const paged::Args a) {
     using namespace paged;
     constexpr int TPS = D / 4, CG = 64 / TPS;
-    const int id = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + threadIdx.x / 64));
-    const int b = id / a.Hq, qh = id - b * a.Hq;
-    if (b >= a.B) return;
-    const int2 plan = a.plan[b];
-    const int share = a.plan[a.B].x;
-    const int kvh = qh / a.G, inner = qh % a.G, block = a.per < a.G ? inner / a.per : 0;
-    const int hb = a.apart > 1 ? kvh * a.apart + block : kvh, beside = a.beside > 1 ? block : 0;
-    const int first = plan.x + hb * (plan.y + TURN), w0 = first / share, S = min((first + plan.y - 1) / share, a.shares - 1) - w0 + 1;
-    if (S < 2) return;
-    const int lane = threadIdx.x & 63, c = lane % TPS, sg = lane / TPS;
-    auto slot_of = [&](int i) { return (size_t)(2 * ((w0 + i) * a.beside + beside) + (i == 0 ? 1 : 0)) * a.per + inner - block * a.per; };
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.0f;
-    for (int s0 = 0; s0 < S; s0 += 4 * CG) {
-        f32x4 os[4];
-        float ms[4], ls[4];
+    __shared__ Side<D> side;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x / 64)), id = blockIdx.x * 4 + wave;
+    const int b = id / a.Hq, lane = threadIdx.x & 63;
+    const Parts p(a, min(b, a.B - 1), id - b * a.Hq);
+    const int S = b < a.B ? p.S : 0;
+    const int2 all = a.plan[a.B];
+    const bool far = all.y > all.x * (LONG - 2);                  // the same for the whole launch
+    if (S >= 2 && !(far && S > LONG)) {
+        const int c = lane % TPS, g = lane / TPS;
+        Sum x = join_every<D>(a, p, c, g, CG);
+        // the groups of lanes together
+        float m = max_xor32(x.m);
+        if constexpr (CG == 4) m = max_xor16(m);
+        const float f = fast_exp2(x.m - (m == -INFINITY ? 0.0f : m));
+        auto sum = [&](float y) {
+            y = sum_xor32(y * f);
+            if constexpr (CG == 4) y = sum_xor16(y);
+            return y;
+        };
+        x.m = m;
+        x.l = sum(x.l);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const size_t slot = slot_of(min(s0 + i * CG + sg, S - 1));
-            ms[i] = s0 + i * CG + sg < S ? a.part_m[slot] : -INFINITY;
-            ls[i] = a.part_l[slot];
-            os[i] = *reinterpret_cast<const f32x4*>(a.part_o + slot * D + 4 * c);
-        }
-        const float mn = fmaxf(fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3])), m), ref = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = fast_exp2(m - ref);
-        o *= alpha;
-        l *= alpha;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (s0 + i * CG + sg < S) {
-                const float wgt = fast_exp2(ms[i] - ref);
-                o += os[i] * wgt;
-                l += ls[i] * wgt;
-            }
+        for (int i = 0; i < 4; ++i) x.o[i] = sum(x.o[i]);
+        if (g == 0) store_head<D>(a, p, c, x);
     }
-    // the groups of lanes together
-    float all = max_xor32(m);
-    if constexpr (CG == 4) all = max_xor16(all);
-    const float f = fast_exp2(m - (all == -INFINITY ? 0.0f : all));
-    auto sum = [&](float x) {
-        x = sum_xor32(x * f);
-        if constexpr (CG == 4) x = sum_xor16(x);
-        return x;
-    };
-    l = sum(l);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = sum(o[i]);
-    if (sg != 0) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const size_t head = (size_t)b * a.Hq + qh;
-    reinterpret_cast<u32x2*>(a.o + head * D)[c] = u32x2{pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv)};
-    if (a.lse && c == 0) a.lse[head] = l == 0.0f ? -INFINITY : logf(l) + all * LN2;
+    if (!far) return;
+    for (int i = blockIdx.x; i < a.B * a.Hq; i += gridDim.x) {    // at most four
+        const Parts of(a, i / a.Hq, i % a.Hq);
+        if (of.S <= LONG) continue;
+        join_by_all<D>(a, of, side);
+        __syncthreads();                                          // the next one writes what this one reads
+    }
 }
 
 // ---- new tokens into the pages ---------------------------------------------------------------
