@@ -16,6 +16,7 @@
 #include "common.hpp"
 #include "launch.hpp"
 #include <type_traits>
+#include <utility>
 
 namespace tyr {
 
@@ -33,6 +34,13 @@ __device__ __forceinline__ u32x4 pack8(const float (&f)[8]) {
     for (int i = 0; i < 4; ++i) v[i] = pack_bf16(f[2 * i], f[2 * i + 1]);
     return v;
 }
+
+// f(0), f(1), ... f(N - 1), each with its own type: an array that they index is registers from the start.  (As loops, beside the branch for rows
+// beyond f32, the weights became one block of registers, and the second piece was asked for when the first was there.)
+template <int... I, class F>
+__device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F f) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, class F>
+__device__ __forceinline__ void each(F f) { each_of(std::make_integer_sequence<int, N>{}, f); }
 
 template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
@@ -52,7 +60,7 @@ __device__ __forceinline__ float over_lanes(float x, F op) {
 }
 // bf16 holds rows whose squares f32 does not.  Where a row's mean square, eps with it, is outside of [LEAST, infinity), its statistics are
 // taken again from h 2^k (and eps 2^2k): y is the same for every k.  Such a row is read twice more, by each of its waves alone: no barrier.
-// What the test costs the others: 65536 x 1024 87.3 us without it, 87.8 so; its gradients 92.1, 92.8; 2000 x 4096 16.1, 16.2.
+// What the test costs the others: 65536 x 1024 87.7 us without it, 87.9 so; its gradients 89.7, 90.7; 2000 x 4096 16.0, 16.0.
 constexpr float LEAST = 0x1p-70f;
 __device__ __forceinline__ bool beyond(float mean) {                // or NaN
     return __builtin_bit_cast(uint32_t, mean) - __builtin_bit_cast(uint32_t, LEAST) >= 0x7f800000u - __builtin_bit_cast(uint32_t, LEAST);
@@ -110,20 +118,19 @@ __global__ __launch_bounds__(S::THREADS) void rmsnorm_residual_kernel(
     const int pieces = row < rows ? d_model / 8 : 0;
     const size_t at = row * d_model;
     u32x4 a[P], b[P], w[P];
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
+    each<P>([&](auto p) {
         const int pc = lane + LPR * (wr + WPR * p);
         if (pc < pieces) {
             a[p] = ld_stream_16<CACHED>(x + at + pc * 8);
             if constexpr (RESIDUAL) b[p] = ld_stream_16<CACHED>(res + at + pc * 8);
             w[p] = ld_global_16(weight + pc * 8);
+            __builtin_amdgcn_sched_barrier(0);                      // all are asked for before one is waited for
         }
-    }
+    });
     float h[P][8], sq = 0.0f, top = 0.0f;
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
+    each<P>([&](auto p) {
         const int pc = lane + LPR * (wr + WPR * p);
-        if (pc >= pieces) continue;
+        if (pc >= pieces) return;
         unpack8(a[p], h[p]);
         if constexpr (RESIDUAL) {
             float f[8];
@@ -142,7 +149,7 @@ __global__ __launch_bounds__(S::THREADS) void rmsnorm_residual_kernel(
             h[p][i] *= wf[i];
             if constexpr (E4M3) top = fmaxf(top, fabsf(h[p][i]));
         }
-    }
+    });
     sq = over_lanes<LPR>(sq, Add{});
     if constexpr (E4M3) top = over_lanes<LPR>(top, Max{});
     if constexpr (WPR > 1) {
@@ -191,37 +198,34 @@ __global__ __launch_bounds__(S::THREADS) void rmsnorm_residual_kernel(
         sq = over_lanes<LPR>(sq, Add{});
         top = over_lanes<LPR>(top, Max{});
         rho = rsqrtf(sq / (float)d_model + eps * k * k);
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
+        each<P>([&](auto p) {
             const int pc = lane + LPR * (wr + WPR * p);
-            if (pc >= pieces) continue;
+            if (pc >= pieces) return;
             element(pc, h[p]);
             unpack8(ld_global_16(weight + pc * 8), wf);
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[p][i] = h[p][i] * k * wf[i];
-        }
+        });
     }
     if constexpr (E4M3) {
         top *= rho;                                                 // max |y|: rho is positive
         const float s = top < TINY ? 1.0f : top / E4M3_MAX, f = rho / s;
         if (lane == 0 && wr == 0 && pieces) row_scale[row] = s;
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
+        each<P>([&](auto p) {
             const int pc = lane + LPR * (wr + WPR * p);
             if (pc < pieces)
                 st_global_8(static_cast<uint8_t*>(out) + at + pc * 8,
                             u32x2{pack_e4m3(f32x4{h[p][0], h[p][1], h[p][2], h[p][3]} * f), pack_e4m3(f32x4{h[p][4], h[p][5], h[p][6], h[p][7]} * f)});
-        }
+        });
     } else {
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
+        each<P>([&](auto p) {
             const int pc = lane + LPR * (wr + WPR * p);
-            if (pc >= pieces) continue;
+            if (pc >= pieces) return;
             float o[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) o[i] = h[p][i] * rho;
             st_global_16_nt(static_cast<uint16_t*>(out) + at + pc * 8, pack8(o));
-        }
+        });
     }
 }
 
