@@ -97,3 +97,14 @@ def test_row_scales_of_a_bf16_norm_are_not_looked_at(ask):
         assert ask([f"norm 4 64 {residual} 0 {at}" for at in (0, 2, 4096)]) == ask([f"norm 4 64 {residual} 0 0"]) * 3
         assert ask([f"norm 4 64 {residual} 0 2"])[0].startswith("0 rmsnorm_residual_kernel")
         assert ask([f"norm 4 64 {residual} 1 {at}" for at in (0, 2)]) == [NULL, MISAL]
+
+
+def test_the_scratch_of_a_norm_s_gradients_holds_their_parts(ask):
+    """A workgroup of the main launch writes a row of d_model numbers for dweight, unless it is the only one."""
+    for d in (8, 64, 512, 1032, 2048, 2560, 4096, 5120, 8192, 16384):
+        for rows in (1, 2, 3, 100, 4095, 4096, 65536, 2 ** 31 - 1):
+            need = int(ask([f"norm_bwd_bytes {rows} {d}"])[0])
+            for resid in (0, 1):
+                got, less = ask([f"norm_bwd {rows} {d} {resid} {need}", f"norm_bwd {rows} {d} {resid} {need - 1}"])
+                m = re.fullmatch(r"0 rmsnorm_residual_bwd_kernel<.*>:(\d+)( rmsnorm_dweight_kernel:\d+)?", got)
+                assert m and less == WS and need >= int(m[1]) * d * 4 and (m[2] is None) == (m[1] == "1"), (rows, d, got)
