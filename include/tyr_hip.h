@@ -472,7 +472,8 @@ int tyr_hip_paged_rope_append(const void* q, const void* k_new, const void* v_ne
  *   sinks   : first rows that stay visible outside the window (without a window: no effect)
  * Pages without a visible row are not looked at, and their table entries may hold anything.  A sequence that sees no row gets O = 0,
  * LSE = -inf.  What the rows that are not visible hold, NaN included, does not matter.  An infinite V in a visible row makes its column
- * of O that infinity (NaN where both signs meet) if the row's probability is above 2^-100 of the largest; below, it may be NaN.
+ * of O that infinity (NaN where both signs meet) if the row's probability is above 2^-100 of the largest; below, it may be NaN.  Sums are
+ * f32 and divided at the end: finite |V| times the visible rows has to stay below 2^128.
  * The batch is cut into pieces on the device, by the lengths that are there: a captured call follows lengths and tables that change
  * between replays.  Results are reproducible for the same lengths.
  *   workspace : tyr_hip_paged_decode_workspace_bytes(...) bytes, 16-byte aligned, contents arbitrary; calls that overlap in time need

@@ -37,7 +37,7 @@ constexpr int WHOLE = 8;                    // sequences of so many steps at mos
 // More than 16 query heads of a kv head are several blocks.  Where each block is a head of its own, its rows come from memory once a block.
 // Two other ways have them come once for two blocks, or for all:
 //   - a wave takes two blocks (bf16 rows of 128 leave no registers for that).  Its steps take longer, so only launches that have many of
-//     them, by their tables' width: 128 sequences of 8192 e4m3 rows, 32 query heads of one kv head 98.7 us, 63.8 so; 64 of 4000 29.1, 30.4.
+//     them, by their tables' width: 128 sequences of 8192 e4m3 rows, 32 query heads of one kv head 98.7 us, 63 so; 64 of 4000 29.1, 30.4.
 constexpr int WIDE = 32768;                 // steps of all blocks from which
 //   - waves side by side in a workgroup take a block each of the same steps and keep together by a barrier, so that all but the first find
 //     the rows in the caches: bf16 rows of 128 where sequences are cut.  128 sequences of 8192 rows, 32 heads 182 us, 118 so (1024 shares

@@ -520,7 +520,7 @@ int launch_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const vo
         using S = decltype(shape);
         parts = bwd_parts<S>(rows);
         constexpr int ROWS = 1024 / (S::LPR * S::WPR);
-        const size_t lds = (size_t)(ROWS / 2) * d_model * sizeof(float);        // at most 32 KB
+        const size_t lds = (size_t)(ROWS / 2) * d_model * sizeof(float);        // at most 16 KB
         auto go = [&](auto in_cache, auto with_resid) {
             launch_kernel((rmsnorm_residual_bwd_kernel<S, in_cache(), with_resid()>), dim3((unsigned)parts), dim3(S::LPR * S::WPR * ROWS), lds, stream,
                           static_cast<const uint16_t*>(d_out), static_cast<const uint16_t*>(d_resid), static_cast<const uint16_t*>(resid),
