@@ -476,8 +476,8 @@ int tyr_hip_paged_rope_append(const void* q, const void* k_new, const void* v_ne
  * f32 and divided at the end: finite |V| times the visible rows has to stay below 2^128.
  * The batch is cut into pieces on the device, by the lengths that are there: a captured call follows lengths and tables that change
  * between replays.  Results are reproducible for the same lengths.
- *   workspace : tyr_hip_paged_decode_workspace_bytes(...) bytes, 16-byte aligned, contents arbitrary; calls that overlap in time need
- *               one each (may be NULL where that is 0)
+ *   workspace : tyr_hip_paged_decode_workspace_bytes(...) bytes (0 also for shapes that the call refuses), 16-byte aligned, contents
+ *               arbitrary; calls that overlap in time need one each (may be NULL where that is 0)
  * Supported additionally: B * Hq < 2^26; steps of 32 rows of all heads (a head: a kv head of a sequence and a block of 16 of its query
  * heads), counted with table_width * page_size rows a sequence, < 2^30.
  */
