@@ -292,11 +292,30 @@ int tyr_hip_rope_fwd(const void* x, const float* cos, const float* sin, void* y,
  *   out       = bf16((out_resid - mean) * rsqrt(var + eps) * weight + bias)
  * with mean / var over the whole row of the rounded out_resid, in f32.
  *
+ * Without a residual (residual and out_resid both NULL) out_resid is x itself and nothing is written; without a bias (NULL) none is added.
+ * Rows whose differences from the mean have squares that f32 does not hold are scaled by a power of two for the statistics, here and in
+ * the gradients.
+ *
  *   x, residual, out, out_resid : bf16 [rows, d_model]      weight, bias : bf16 [d_model]
+ * Supported: a launch of fewer than 2^32 threads: rows * (elements of a row, rounded up to 64 * 2^n) < 2^35, twice that above 512.
  */
 int tyr_hip_layernorm_residual(const void* x, const void* residual, const void* weight,
                                const void* bias, void* out, void* out_resid,
                                uint64_t rows, uint64_t d_model, float eps, void* stream);
+
+/* Its gradients.  With n = (resid - mean) rho, rho = rsqrt(var + eps), g = d_out * weight:
+ *   dx      = bf16(rho (g - mean(g) - n mean(g n)) + d_resid)     the gradient of x and of residual alike
+ *   dweight = bf16(sum over rows of d_out n)      dbias = bf16(sum over rows of d_out), NULL = not wanted
+ *   resid   : the forward's out_resid (its x where there was no residual), bf16 [rows, d_model]
+ *   d_out   : gradient of out, bf16 [rows, d_model]
+ *   d_resid : gradient that reaches out_resid by other ways, bf16 [rows, d_model], or NULL
+ *   dx      : bf16 [rows, d_model]      dweight, dbias : bf16 [d_model]      (they overlap no input)
+ *   workspace : tyr_hip_layernorm_residual_bwd_workspace_bytes(rows, d_model) bytes, 16-byte aligned, contents arbitrary
+ * The result is deterministic (no atomic accumulation).  Shapes as the forward. */
+size_t tyr_hip_layernorm_residual_bwd_workspace_bytes(uint64_t rows, uint64_t d_model);
+int tyr_hip_layernorm_residual_bwd(const void* d_out, const void* d_resid, const void* resid, const void* weight, void* dx,
+                                   void* dweight, void* dbias, uint64_t rows, uint64_t d_model, float eps, void* workspace,
+                                   size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Device-to-device copy kernel.
@@ -432,6 +451,67 @@ size_t tyr_hip_rmsnorm_residual_bwd_workspace_bytes(uint64_t rows, uint64_t d_mo
 int tyr_hip_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const void* resid, const void* weight, void* dx,
                                  void* dweight, uint64_t rows, uint64_t d_model, float eps, void* workspace,
                                  size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Embedding: rows of a table by token, and the gradient of the table.
+ *
+ *   out[i] = scale * table[ids[i]];  a token outside of [0, vocab) (padding) gives a row of zeros
+ *   ids   : int32 (TYR_HIP_I32) or int64 (TYR_HIP_I64) [n]      table : [vocab, d_model]      out : [n, d_model], overlaps no input
+ *   dtype : of table and out, TYR_HIP_F32 or TYR_HIP_BF16
+ * Supported: d_model % 8 == 0 (bf16) / % 4 == 0 (f32) up to 2^20; n and vocab < 2^31; n * (16-byte pieces of a row, rounded up to a power of
+ * two, at most 256) < 2^32 - 256.
+ */
+enum tyr_hip_index_dtype { TYR_HIP_I32 = 0, TYR_HIP_I64 = 1 };
+int tyr_hip_embedding(const void* ids, int ids_dtype, const void* table, void* out, uint64_t n, uint64_t vocab, uint64_t d_model,
+                      float scale, int dtype, void* stream);
+
+/* The gradient of the table:
+ *   d_table[v] = scale * sum over i with ids[i] = v of d_out[i]          accumulate = 0: every row is written, those of no token with zeros
+ *   d_table[v] = d_table[v] + that sum                                   accumulate = 1: rows of no token are not touched
+ * Sums are f32 and rounded once.  Tokens outside of [0, vocab) add nothing; what their rows of d_out hold does not matter.  The tokens are
+ * sorted first: the result is deterministic (no atomic accumulation).
+ *   d_out : [n, d_model]      d_table : [vocab, d_model], overlaps no input; both of dtype
+ *   workspace : tyr_hip_embedding_bwd_workspace_bytes(...) bytes (0 for shapes that the call refuses), 16-byte aligned, contents arbitrary;
+ *               calls that overlap in time need one each
+ * Supported: as the lookup, and n <= 2^30; with pieces of 8 tokens (32 above 8192 tokens) and blocks of 64 16-byte pieces of a row,
+ * pieces * blocks < 2^23 and pieces * blocks + vocab / 16 < 2^26. */
+size_t tyr_hip_embedding_bwd_workspace_bytes(uint64_t n, uint64_t vocab, uint64_t d_model, int dtype);
+int tyr_hip_embedding_bwd(const void* d_out, const void* ids, int ids_dtype, void* d_table, uint64_t n, uint64_t vocab, uint64_t d_model,
+                          float scale, int accumulate, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Log probabilities of given tokens, with the entropy and the most likely alternatives of each row, and their gradient.
+ *
+ *   lse[r]     = ln sum over v < vocab of exp(x[r, v])
+ *   logp[r]    = x[r, targets[r]] - lse[r];  0 for a target outside of [0, vocab) (padding)
+ *   entropy[r] = -sum p ln p, p = exp(x - lse)                            NULL: not computed
+ *   top_logp, top_ids [rows, top] : the `top` largest x - lse and their places, largest first, equal ones by place      top = 0: none
+ *   logits  : x, bf16 or f32 [rows, width], at any element; the columns from vocab on (padding of the head's product) are not looked at
+ *   targets : int32 or int64 [rows]      logp, lse, entropy : f32 [rows]      top_logp : f32, top_ids : int32
+ * All sums are f32 about the row's largest logit.  Logits of -infinity have no probability; a row of nothing else has lse = logp = -infinity,
+ * entropy 0 and its first `top` places as alternatives, of -infinity each.  A row with a NaN or +infinity has NaN in all of its results (logp
+ * of padding apart); among the alternatives NaN stands with the -infinities.
+ *   workspace : tyr_hip_token_logprobs_workspace_bytes(...) bytes (0 also for shapes that the call refuses), 16-byte aligned, contents
+ *               arbitrary; calls that overlap in time need one each (may be NULL where that is 0)
+ * Supported: top <= vocab and <= TYR_HIP_TOKEN_LOGPROBS_MAX_TOP; vocab < 2^30, width < 2^31; rows and, with 16 KB of a row each, the
+ * gradient's workgroups rows * ceil(vocab / (8192 bf16, 4096 f32)) < 2^24.
+ */
+#define TYR_HIP_TOKEN_LOGPROBS_MAX_TOP 64
+size_t tyr_hip_token_logprobs_workspace_bytes(uint64_t rows, uint64_t vocab, uint64_t top, int dtype);
+int tyr_hip_token_logprobs(const void* logits, const void* targets, int targets_dtype, float* logp, float* lse, float* entropy,
+                           float* top_logp, int32_t* top_ids, uint64_t rows, uint64_t vocab, uint64_t width, uint64_t top, int dtype,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gradient with respect to the logits, from those of logp, entropy and lse:
+ *   d_logits[r, v] = p (d_lse - d_logp - d_entropy (ln p + entropy)) + d_logp [v = targets[r]],   p = exp(x - lse);  0 from vocab on
+ *   logits, targets : the forward's      lse, entropy : its results (entropy only with d_entropy)
+ *   d_logp, d_entropy, d_lse : f32 [rows], NULL = zeros; d_logp of a target outside of [0, vocab) counts as zero
+ *   d_logits : as logits; may be logits itself (fastest where both begin at the same place of 16 bytes)
+ * A row whose gradients are all zero, or whose lse is -infinity, gets zeros whatever else it holds.  p has the precision of lse:
+ * |lse| 2^-24 of its size. */
+int tyr_hip_token_logprobs_bwd(const void* logits, const void* targets, int targets_dtype, const float* lse, const float* entropy,
+                               const float* d_logp, const float* d_entropy, const float* d_lse, void* d_logits, uint64_t rows,
+                               uint64_t vocab, uint64_t width, int dtype, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Key-value cache in pages.

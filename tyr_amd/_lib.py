@@ -20,6 +20,8 @@ SYMBOLS = (
     "tyr_hip_decode_rope_append", "tyr_hip_rope_fwd", "tyr_hip_layernorm_residual", "tyr_hip_copy", "tyr_hip_mfma_sustain", "tyr_hip_mse_loss_grad_workspace_bytes", "tyr_hip_mse_loss_grad", "tyr_hip_sgd_step",
     "tyr_hip_rmsnorm_residual", "tyr_hip_rmsnorm_residual_bwd_workspace_bytes", "tyr_hip_rmsnorm_residual_bwd", "tyr_hip_paged_rope_append",
     "tyr_hip_paged_decode_workspace_bytes", "tyr_hip_paged_decode",
+    "tyr_hip_layernorm_residual_bwd_workspace_bytes", "tyr_hip_layernorm_residual_bwd", "tyr_hip_embedding", "tyr_hip_embedding_bwd_workspace_bytes",
+    "tyr_hip_embedding_bwd", "tyr_hip_token_logprobs_workspace_bytes", "tyr_hip_token_logprobs", "tyr_hip_token_logprobs_bwd",
 )
 
 BINDING_PATH = os.path.join(_HERE, "lib", "_tyr_torch.so")
@@ -142,5 +144,21 @@ def load() -> ctypes.CDLL:
     L.tyr_hip_paged_decode_workspace_bytes.restype = sz
     L.tyr_hip_paged_decode.argtypes = [vp] * 9 + [u64] * 9 + [ci, f32, vp, sz, vp]
     L.tyr_hip_paged_decode.restype = ci
+    L.tyr_hip_layernorm_residual_bwd_workspace_bytes.argtypes = [u64, u64]
+    L.tyr_hip_layernorm_residual_bwd_workspace_bytes.restype = sz
+    L.tyr_hip_layernorm_residual_bwd.argtypes = [vp] * 7 + [u64, u64, f32, vp, sz, vp]
+    L.tyr_hip_layernorm_residual_bwd.restype = ci
+    L.tyr_hip_embedding.argtypes = [vp, ci, vp, vp, u64, u64, u64, f32, ci, vp]
+    L.tyr_hip_embedding.restype = ci
+    L.tyr_hip_embedding_bwd_workspace_bytes.argtypes = [u64] * 3 + [ci]
+    L.tyr_hip_embedding_bwd_workspace_bytes.restype = sz
+    L.tyr_hip_embedding_bwd.argtypes = [vp, vp, ci, vp, u64, u64, u64, f32, ci, ci, vp, sz, vp]
+    L.tyr_hip_embedding_bwd.restype = ci
+    L.tyr_hip_token_logprobs_workspace_bytes.argtypes = [u64] * 3 + [ci]
+    L.tyr_hip_token_logprobs_workspace_bytes.restype = sz
+    L.tyr_hip_token_logprobs.argtypes = [vp, vp, ci] + [vp] * 5 + [u64] * 4 + [ci, vp, sz, vp]
+    L.tyr_hip_token_logprobs.restype = ci
+    L.tyr_hip_token_logprobs_bwd.argtypes = [vp, vp, ci] + [vp] * 6 + [u64] * 3 + [ci, vp]
+    L.tyr_hip_token_logprobs_bwd.restype = ci
     _lib = L
     return L

@@ -397,18 +397,49 @@ int tyr_hip_rope_fwd(const void* x, const float* cos, const float* sin, void* y,
     return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
 }
 
+// layer norms of rows of at most 8192
+static bool layernorm_extents(uint64_t rows, uint64_t d_model, int* rc) {
+    if (rows == 0 || d_model == 0) *rc = TYR_HIP_ERR_BAD_SHAPE;
+    else if (d_model % 8 != 0 || d_model > 8192) *rc = TYR_HIP_ERR_UNSUPPORTED;
+    else if (rows > (uint64_t)INT_MAX || !tyr::layernorm_residual_fits((size_t)rows, (int)d_model)) *rc = TYR_HIP_ERR_BAD_SHAPE;
+    else return true;
+    return false;
+}
+
 int tyr_hip_layernorm_residual(const void* x, const void* residual, const void* weight, const void* bias,
                                void* out, void* out_resid, uint64_t rows, uint64_t d_model, float eps,
                                void* stream) {
-    if (!x || !residual || !weight || !bias || !out || !out_resid) return TYR_HIP_ERR_NULL_POINTER;
-    if (rows == 0 || d_model == 0) return TYR_HIP_ERR_BAD_SHAPE;
-    if (d_model % 8 != 0 || d_model > 8192 || !(eps >= 0.0f)) return TYR_HIP_ERR_UNSUPPORTED;
-    if ((rows + 3) / 4 > (uint64_t)INT_MAX) return TYR_HIP_ERR_BAD_SHAPE;
+    if (!x || !weight || !out || (residual != nullptr) != (out_resid != nullptr)) return TYR_HIP_ERR_NULL_POINTER;
+    int rc;
+    if (!layernorm_extents(rows, d_model, &rc)) return rc;
+    if (!(eps >= 0.0f)) return TYR_HIP_ERR_UNSUPPORTED;
     if (!aligned16(x) || !aligned16(residual) || !aligned16(weight) || !aligned16(bias) || !aligned16(out) ||
         !aligned16(out_resid))
         return TYR_HIP_ERR_MISALIGNED;
-    const int rc = tyr::launch_layernorm_residual(x, residual, weight, bias, out, out_resid, (size_t)rows,
-                                                  (int)d_model, eps, static_cast<hipStream_t>(stream));
+    rc = tyr::launch_layernorm_residual(x, residual, weight, bias, out, out_resid, (size_t)rows,
+                                        (int)d_model, eps, static_cast<hipStream_t>(stream));
+    return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
+}
+
+size_t tyr_hip_layernorm_residual_bwd_workspace_bytes(uint64_t rows, uint64_t d_model) {
+    int rc;
+    return layernorm_extents(rows, d_model, &rc) ? tyr::layernorm_residual_bwd_workspace_bytes((size_t)rows, (int)d_model) : 0;
+}
+
+int tyr_hip_layernorm_residual_bwd(const void* d_out, const void* d_resid, const void* resid, const void* weight, void* dx, void* dweight,
+                                   void* dbias, uint64_t rows, uint64_t d_model, float eps, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+    if (!d_out || !resid || !weight || !dx || !dweight) return TYR_HIP_ERR_NULL_POINTER;
+    int rc;
+    if (!layernorm_extents(rows, d_model, &rc)) return rc;
+    if (!(eps >= 0.0f)) return TYR_HIP_ERR_UNSUPPORTED;
+    if (!aligned16(d_out) || !aligned16(d_resid) || !aligned16(resid) || !aligned16(weight) || !aligned16(dx) || !aligned16(dweight) ||
+        !aligned16(dbias))
+        return TYR_HIP_ERR_MISALIGNED;
+    if (!workspace || workspace_bytes < tyr::layernorm_residual_bwd_workspace_bytes((size_t)rows, (int)d_model)) return TYR_HIP_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return TYR_HIP_ERR_MISALIGNED;
+    rc = tyr::launch_layernorm_residual_bwd(d_out, d_resid, resid, weight, dx, dweight, dbias, (size_t)rows, (int)d_model, eps, workspace,
+                                            static_cast<hipStream_t>(stream));
     return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
 }
 
@@ -453,6 +484,113 @@ int tyr_hip_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const v
     if (!aligned16(workspace)) return TYR_HIP_ERR_MISALIGNED;
     rc = tyr::launch_rmsnorm_residual_bwd(d_out, d_resid, resid, weight, dx, dweight, (size_t)rows, (int)d_model, eps, workspace,
                                           static_cast<hipStream_t>(stream));
+    return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
+}
+
+static bool is_index(int dtype) { return dtype == TYR_HIP_I32 || dtype == TYR_HIP_I64; }
+static bool is_float(int dtype) { return dtype == TYR_HIP_F32 || dtype == TYR_HIP_BF16; }
+static bool aligned_index(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == TYR_HIP_I64 ? 7u : 3u)) == 0; }
+
+// what both calls on an embedding ask
+static int embedding_extents(uint64_t n, uint64_t vocab, uint64_t d_model, int dtype) {
+    if (n == 0 || vocab == 0 || d_model == 0) return TYR_HIP_ERR_BAD_SHAPE;
+    if (!is_float(dtype) || d_model % (dtype == TYR_HIP_BF16 ? 8 : 4) != 0 || d_model > (uint64_t)1 << 20) return TYR_HIP_ERR_UNSUPPORTED;
+    if (!fits_int(n) || !fits_int(vocab)) return TYR_HIP_ERR_BAD_SHAPE;
+    return TYR_HIP_OK;
+}
+
+int tyr_hip_embedding(const void* ids, int ids_dtype, const void* table, void* out, uint64_t n, uint64_t vocab, uint64_t d_model, float scale,
+                      int dtype, void* stream) {
+    if (!ids || !table || !out) return TYR_HIP_ERR_NULL_POINTER;
+    int rc = embedding_extents(n, vocab, d_model, dtype);
+    if (rc != TYR_HIP_OK) return rc;
+    if (!is_index(ids_dtype)) return TYR_HIP_ERR_UNSUPPORTED;
+    const int bf16 = dtype == TYR_HIP_BF16;
+    if (!tyr::embedding_fits((size_t)n, (int)d_model, bf16 ? 2 : 4)) return TYR_HIP_ERR_BAD_SHAPE;
+    if (!aligned_index(ids, ids_dtype) || !aligned16(table) || !aligned16(out)) return TYR_HIP_ERR_MISALIGNED;
+    rc = tyr::launch_embedding(ids, ids_dtype == TYR_HIP_I64, table, out, (size_t)n, (size_t)vocab, (int)d_model, scale, bf16,
+                               static_cast<hipStream_t>(stream));
+    return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
+}
+
+static int embedding_bwd_extents(uint64_t n, uint64_t vocab, uint64_t d_model, int dtype) {
+    const int rc = embedding_extents(n, vocab, d_model, dtype);
+    if (rc != TYR_HIP_OK) return rc;
+    return n <= (uint64_t)1 << 30 && tyr::embedding_bwd_fits((size_t)n, (size_t)vocab, (int)d_model, dtype == TYR_HIP_BF16) ? TYR_HIP_OK : TYR_HIP_ERR_BAD_SHAPE;
+}
+
+size_t tyr_hip_embedding_bwd_workspace_bytes(uint64_t n, uint64_t vocab, uint64_t d_model, int dtype) {
+    return embedding_bwd_extents(n, vocab, d_model, dtype) == TYR_HIP_OK
+               ? tyr::embedding_bwd_workspace_bytes((size_t)n, (size_t)vocab, (int)d_model, dtype == TYR_HIP_BF16) : 0;
+}
+
+int tyr_hip_embedding_bwd(const void* d_out, const void* ids, int ids_dtype, void* d_table, uint64_t n, uint64_t vocab, uint64_t d_model,
+                          float scale, int accumulate, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!d_out || !ids || !d_table) return TYR_HIP_ERR_NULL_POINTER;
+    int rc = embedding_bwd_extents(n, vocab, d_model, dtype);
+    if (rc != TYR_HIP_OK) return rc;
+    if (!is_index(ids_dtype)) return TYR_HIP_ERR_UNSUPPORTED;
+    if (!aligned_index(ids, ids_dtype) || !aligned16(d_out) || !aligned16(d_table)) return TYR_HIP_ERR_MISALIGNED;
+    const int bf16 = dtype == TYR_HIP_BF16;
+    if (!workspace || workspace_bytes < tyr::embedding_bwd_workspace_bytes((size_t)n, (size_t)vocab, (int)d_model, bf16)) return TYR_HIP_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return TYR_HIP_ERR_MISALIGNED;
+    rc = tyr::launch_embedding_bwd(d_out, ids, ids_dtype == TYR_HIP_I64, d_table, (size_t)n, (size_t)vocab, (int)d_model, scale, accumulate, bf16,
+                                   workspace, static_cast<hipStream_t>(stream));
+    return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
+}
+
+// what the calls on logits ask of them
+static int logits_extents(uint64_t rows, uint64_t vocab, uint64_t width, int dtype) {
+    if (rows == 0 || vocab == 0 || width < vocab) return TYR_HIP_ERR_BAD_SHAPE;
+    if (!is_float(dtype)) return TYR_HIP_ERR_UNSUPPORTED;
+    if (vocab >= (uint64_t)1 << 30 || width >= (uint64_t)1 << 31 || rows > (uint64_t)INT_MAX ||
+        !tyr::token_logprobs_fits((size_t)rows, (int)vocab, dtype == TYR_HIP_BF16))
+        return TYR_HIP_ERR_BAD_SHAPE;
+    return TYR_HIP_OK;
+}
+static bool aligned_logits(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == TYR_HIP_BF16 ? 1u : 3u)) == 0; }
+static int top_extents(uint64_t vocab, uint64_t top) {
+    if (top > vocab) return TYR_HIP_ERR_BAD_SHAPE;
+    return top > TYR_HIP_TOKEN_LOGPROBS_MAX_TOP ? TYR_HIP_ERR_UNSUPPORTED : TYR_HIP_OK;
+}
+
+size_t tyr_hip_token_logprobs_workspace_bytes(uint64_t rows, uint64_t vocab, uint64_t top, int dtype) {
+    if (logits_extents(rows, vocab, vocab, dtype) != TYR_HIP_OK || top_extents(vocab, top) != TYR_HIP_OK) return 0;
+    return tyr::token_logprobs_workspace_bytes((size_t)rows, (int)vocab, (int)top, dtype == TYR_HIP_BF16);
+}
+
+int tyr_hip_token_logprobs(const void* logits, const void* targets, int targets_dtype, float* logp, float* lse, float* entropy, float* top_logp,
+                           int32_t* top_ids, uint64_t rows, uint64_t vocab, uint64_t width, uint64_t top, int dtype, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+    if (!logits || !targets || !logp || !lse || (top != 0 && (!top_logp || !top_ids))) return TYR_HIP_ERR_NULL_POINTER;
+    int rc = logits_extents(rows, vocab, width, dtype);
+    if (rc == TYR_HIP_OK) rc = top_extents(vocab, top);
+    if (rc != TYR_HIP_OK) return rc;
+    if (!is_index(targets_dtype)) return TYR_HIP_ERR_UNSUPPORTED;
+    if (!aligned_logits(logits, dtype) || !aligned_index(targets, targets_dtype) || !aligned4(logp) || !aligned4(lse) || !aligned4(entropy) ||
+        (top != 0 && (!aligned4(top_logp) || !aligned4(top_ids))))
+        return TYR_HIP_ERR_MISALIGNED;
+    const int bf16 = dtype == TYR_HIP_BF16;
+    const size_t need = tyr::token_logprobs_workspace_bytes((size_t)rows, (int)vocab, (int)top, bf16);
+    if (need && (!workspace || workspace_bytes < need)) return TYR_HIP_ERR_WORKSPACE;
+    if (need && !aligned16(workspace)) return TYR_HIP_ERR_MISALIGNED;
+    rc = tyr::launch_token_logprobs(logits, targets, targets_dtype == TYR_HIP_I64, logp, lse, entropy, top_logp, top_ids, (size_t)rows, (int)vocab,
+                                    (size_t)width, (int)top, bf16, workspace, static_cast<hipStream_t>(stream));
+    return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
+}
+
+int tyr_hip_token_logprobs_bwd(const void* logits, const void* targets, int targets_dtype, const float* lse, const float* entropy,
+                               const float* d_logp, const float* d_entropy, const float* d_lse, void* d_logits, uint64_t rows, uint64_t vocab,
+                               uint64_t width, int dtype, void* stream) {
+    if (!logits || !targets || !lse || !d_logits || (d_entropy && !entropy)) return TYR_HIP_ERR_NULL_POINTER;
+    int rc = logits_extents(rows, vocab, width, dtype);
+    if (rc != TYR_HIP_OK) return rc;
+    if (!is_index(targets_dtype)) return TYR_HIP_ERR_UNSUPPORTED;
+    if (!aligned_logits(logits, dtype) || !aligned_logits(d_logits, dtype) || !aligned_index(targets, targets_dtype) || !aligned4(lse) || !aligned4(entropy) ||
+        !aligned4(d_logp) || !aligned4(d_entropy) || !aligned4(d_lse))
+        return TYR_HIP_ERR_MISALIGNED;
+    rc = tyr::launch_token_logprobs_bwd(logits, targets, targets_dtype == TYR_HIP_I64, lse, entropy, d_logp, d_entropy, d_lse, d_logits, (size_t)rows,
+                                        (int)vocab, (size_t)width, dtype == TYR_HIP_BF16, static_cast<hipStream_t>(stream));
     return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;
 }
 

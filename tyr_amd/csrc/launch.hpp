@@ -48,8 +48,13 @@ int launch_rope_fwd(const void* x, const float* cosp, const float* sinp, void* y
 int launch_decode_rope_append(const void* q, const void* k_new, const void* v_new, const float* cosp,
                               const float* sinp, void* q_out, void* k_cache, void* v_cache, int B, int Hq, int Hkv,
                               int D, size_t kv_stride, size_t pos, hipStream_t stream);
+// residual and out_resid: both or neither; bias may be null
+bool layernorm_residual_fits(size_t rows, int d_model);    // a launch has fewer than 2^32 threads
 int launch_layernorm_residual(const void* x, const void* residual, const void* weight, const void* bias, void* out,
                               void* out_resid, size_t rows, int d_model, float eps, hipStream_t stream);
+size_t layernorm_residual_bwd_workspace_bytes(size_t rows, int d_model);
+int launch_layernorm_residual_bwd(const void* d_out, const void* d_resid, const void* resid, const void* weight, void* dx, void* dweight,
+                                  void* dbias, size_t rows, int d_model, float eps, void* workspace, hipStream_t stream);
 // residual and out_resid: both or neither; row_scale [rows] with e4m3
 bool rmsnorm_residual_fits(size_t rows, int d_model);      // a launch has fewer than 2^32 threads
 int launch_rmsnorm_residual(const void* x, const void* residual, const void* weight, void* out, void* out_resid, float* row_scale,
@@ -57,6 +62,23 @@ int launch_rmsnorm_residual(const void* x, const void* residual, const void* wei
 size_t rmsnorm_residual_bwd_workspace_bytes(size_t rows, int d_model);
 int launch_rmsnorm_residual_bwd(const void* d_out, const void* d_resid, const void* resid, const void* weight, void* dx, void* dweight,
                                 size_t rows, int d_model, float eps, void* workspace, hipStream_t stream);
+
+bool embedding_fits(size_t n, int d_model, int elem_bytes);
+int launch_embedding(const void* ids, int ids64, const void* table, void* out, size_t n, size_t vocab, int d_model, float scale, int bf16,
+                     hipStream_t stream);
+bool embedding_bwd_fits(size_t n, size_t vocab, int d_model, int bf16);
+size_t embedding_bwd_workspace_bytes(size_t n, size_t vocab, int d_model, int bf16);
+int launch_embedding_bwd(const void* d_out, const void* ids, int ids64, void* table, size_t n, size_t vocab, int d_model, float scale, int into,
+                         int bf16, void* workspace, hipStream_t stream);
+
+// entropy and, for top = 0, top_logp and top_ids may be null
+bool token_logprobs_fits(size_t rows, int vocab, int bf16);
+size_t token_logprobs_workspace_bytes(size_t rows, int vocab, int top, int bf16);
+int launch_token_logprobs(const void* logits, const void* targets, int targets64, float* logp, float* lse, float* entropy, float* top_logp,
+                          int32_t* top_ids, size_t rows, int vocab, size_t width, int top, int bf16, void* workspace, hipStream_t stream);
+int launch_token_logprobs_bwd(const void* logits, const void* targets, int targets64, const float* lse, const float* entropy, const float* d_logp,
+                              const float* d_entropy, const float* d_lse, void* d_logits, size_t rows, int vocab, size_t width, int bf16,
+                              hipStream_t stream);
 
 // The cache in pages; cap = rows that a table row can name.  k_scale / v_scale [Hkv] may be null.
 size_t paged_decode_workspace_bytes(int B, int Hq, int Hkv, int D, int64_t cap);

@@ -1,0 +1,515 @@
+// Log probabilities of given tokens, with entropy and the largest alternatives, and their gradient (gfx950).
+//
+// Of a row x of `vocab` logits, m its largest, s = sum e^(x - m), t = sum (x - m) e^(x - m):
+//   lse = m + ln s,   logp = x[target] - m - ln s,   entropy = ln s - t / s,   alternatives: the `top` largest x, equal ones by place.
+// Gradient, with p = e^(x - lse) and the gradients of logp, entropy and lse that arrive:
+//   dx = p (d_lse - d_logp - d_entropy (ln p + entropy)) + d_logp [at the target]
+//
+// One pass over the row: every lane keeps m, s and t of its own elements and scales them when its m grows; they are joined at the end, in f32.
+// The alternatives need no second pass: the `top`-th largest of the lanes' m is no larger than the `top`-th largest element, so only the
+// elements of lanes that reach it are read once more, and of those the ones that reach it are few.
+//
+// Bound by HBM (bf16: and nearly by the vector units, 7 to 9 instructions an element, of which the exponential counts as four).
+//
+// A row begins at any element: up to 16 bytes' worth at its two ends are taken one by one, what lies between in pieces of 16 bytes.
+#include <algorithm>
+#include <type_traits>
+
+#include "common.hpp"
+#include "launch.hpp"
+
+namespace tyr {
+
+namespace lp {
+constexpr int THREADS = 256, WAVES = THREADS / 64;
+constexpr int AT_ONCE = 4;                        // pieces a lane asks for together
+constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
+constexpr float LEAST = -3.402823466e38f;         // m of no element: the smallest finite number
+// sizes of m, and of the least element, up to which an element's exponent is one multiplication and addition
+constexpr float TAME = 1024.0f, FAR = 1e30f;
+constexpr int MAX_TOP = 64;
+constexpr int KEPT = 512;                         // candidates that stay when the list is cut
+
+template <class T> struct Elem;
+template <> struct Elem<uint16_t> {
+    static constexpr int E = 8;
+    static __device__ __forceinline__ float one(uint16_t v) { return __builtin_bit_cast(float, (uint32_t)v << 16); }
+    static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { f[2 * i] = bf16_lo(v[i]); f[2 * i + 1] = bf16_hi(v[i]); }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
+        return u32x4{pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7])};
+    }
+    static __device__ __forceinline__ void put(uint16_t* p, float v) { *p = (uint16_t)pack_bf16(v, 0.0f); }
+};
+template <> struct Elem<float> {
+    static constexpr int E = 4;
+    static __device__ __forceinline__ float one(float v) { return v; }
+    static __device__ __forceinline__ void unpack(u32x4 v, float (&f)[4]) {
+        const f32x4 x = __builtin_bit_cast(f32x4, v);              // (a bit cast of one element of a vector reads the first)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = x[i];
+    }
+    static __device__ __forceinline__ u32x4 pack(const float (&f)[4]) {
+        return __builtin_bit_cast(u32x4, f32x4{f[0], f[1], f[2], f[3]});
+    }
+    static __device__ __forceinline__ void put(float* p, float v) { *p = v; }
+};
+
+// A stretch of a row, [begin, end) in elements of the row: `head` single elements, `pieces` of E, `tail` single ones.
+template <class T>
+struct Stretch {
+    const T* row;
+    int begin, head, pieces, tail;
+    __device__ __forceinline__ Stretch(const T* row_, int begin_, int end) : row(row_), begin(begin_) {
+        constexpr int E = Elem<T>::E;
+        const int off = (int)((reinterpret_cast<uintptr_t>(row + begin) / sizeof(T)) % E);
+        head = min(end - begin, off ? E - off : 0);
+        pieces = (end - begin - head) / E;
+        tail = end - begin - head - pieces * E;
+    }
+    __device__ __forceinline__ const T* piece(int p) const { return row + begin + head + p * Elem<T>::E; }
+    __device__ __forceinline__ int place(int p) const { return begin + head + p * Elem<T>::E; }
+    // the single element of a thread, or -1: threads [0, E) the head's, [E, 2 E) the tail's
+    __device__ __forceinline__ int single(int thread) const {
+        constexpr int E = Elem<T>::E;
+        if (thread < head) return begin + thread;
+        if (thread >= E && thread < E + tail) return begin + head + pieces * E + thread - E;
+        return -1;
+    }
+};
+
+// m, s and t (in units of log2) of some elements
+struct Sum { float m, s, t; };
+__device__ __forceinline__ Sum join(Sum a, Sum b) {
+    const float m = fmaxf(a.m, b.m);
+    // differences of lowest and largest numbers overflow: at -2^20 the factor is 0 already
+    const float da = fmaxf((a.m - m) * LOG2E, -0x1p20f), db = fmaxf((b.m - m) * LOG2E, -0x1p20f);
+    const float ea = fast_exp2(da), eb = fast_exp2(db);
+    return {m, a.s * ea + b.s * eb, (a.t + da * a.s) * ea + (b.t + db * b.s) * eb};
+}
+// N elements joined to a sum.  Where m is large the rounding of m log2(e) weighs more than a difference taken first, and where an element is
+// -infinity or near it 0 * infinity is not 0: differences are taken first there, and bounded.
+template <bool ENTROPY, int N>
+__device__ __forceinline__ void add(Sum& a, const float (&x)[N]) {
+    float most = x[0], least = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+        most = fmaxf(most, x[i]);
+        if constexpr (ENTROPY) least = fminf(least, x[i]);
+    }
+    if (most > a.m) {
+        const float d = fmaxf((a.m - most) * LOG2E, -0x1p20f), e = fast_exp2(d);
+        if constexpr (ENTROPY) a.t = (a.t + d * a.s) * e;
+        a.s *= e;
+        a.m = most;
+    }
+    const bool tame = fabsf(a.m) < TAME && (!ENTROPY || least > -FAR);
+    if (__builtin_amdgcn_ballot_w64(!tame) == 0) {
+        // relative to c, which is m log2(e) but for its rounding: that much is put right for the sums
+        const float c = a.m * LOG2E, off = -fmaf(a.m, LOG2E, -c), off_ln = off * LN2;
+        float s = 0.0f, t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float y = fmaf(x[i], LOG2E, -c), e = fast_exp2(y);
+            s += e;
+            if constexpr (ENTROPY) t = fmaf(y, e, t);
+        }
+        if constexpr (ENTROPY) a.t += t + fmaf(off, s, off_ln * t);
+        a.s += fmaf(s, off_ln, s);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float y = (x[i] - a.m) * LOG2E, e = fast_exp2(y);
+            a.s += e;
+            if constexpr (ENTROPY) a.t = fmaf(fmaxf(y, -0x1p20f), e, a.t);
+        }
+    }
+}
+
+// Elements in the order of the alternatives: larger first, equal ones by place; -0 is 0, and NaN the least.
+__device__ __forceinline__ uint64_t rank_of(float x, uint32_t place) {
+    x = x == x ? x + 0.0f : -__builtin_inff();
+    const uint32_t b = __builtin_bit_cast(uint32_t, x);
+    return (uint64_t)(b >> 31 ? ~b : b | 0x80000000u) << 32 | (uint32_t)~place;
+}
+__device__ __forceinline__ float value_of(uint64_t rank) {
+    const uint32_t b = (uint32_t)(rank >> 32);
+    return __builtin_bit_cast(float, b >> 31 ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ uint32_t place_of(uint64_t rank) { return ~(uint32_t)rank; }
+
+// What may still be among the alternatives.
+struct Candidates {
+    uint64_t list[KEPT + THREADS * 8];            // what stays, and what the threads add in a turn
+    uint64_t chosen[MAX_TOP];
+    uint64_t best[WAVES];
+    int count;
+};
+__device__ __forceinline__ uint64_t largest(uint64_t v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t w = __shfl_xor((unsigned long long)v, o, 64);
+        v = w > v ? w : v;
+    }
+    return v;
+}
+// c.chosen = the `top` largest of the first `count` of the list, in order, 0 behind the last; all threads call it.  A few by counting how many
+// are larger than each, many by one search for each of the chosen.
+__device__ __forceinline__ void choose(Candidates& c, int count, int top) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (count <= KEPT) {
+        for (int i = threadIdx.x; i < top; i += THREADS)
+            if (i >= count) c.chosen[i] = 0;
+        for (int i = threadIdx.x; i < count; i += THREADS) {
+            const uint64_t mine = c.list[i];
+            int front = 0;
+#pragma unroll 8
+            for (int j = 0; j < count; ++j) front += c.list[j] > mine;
+            if (front < top) c.chosen[front] = mine;
+        }
+    } else {
+        uint64_t limit = ~(uint64_t)0;
+        for (int j = 0; j < top; ++j) {
+            uint64_t v = 0;
+            for (int i = threadIdx.x; i < count; i += THREADS) {
+                const uint64_t w = c.list[i];
+                if (w < limit && w > v) v = w;
+            }
+            v = largest(v);
+            if (lane == 0) c.best[wave] = v;
+            __syncthreads();
+            limit = c.best[0];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) limit = c.best[w] > limit ? c.best[w] : limit;
+            if (threadIdx.x == 0) c.chosen[j] = limit;
+            __syncthreads();
+        }
+    }
+    __syncthreads();
+}
+// What one workgroup's stretch of a row comes to where rows are cut; its alternatives stand apart.
+struct Part { float m, s, t, unused; };
+
+struct Out {
+    float *logp, *lse, *entropy, *top_logp;
+    int32_t* top_ids;
+};
+// One thread writes a row's results, `top` threads its alternatives.
+template <class T, bool ENTROPY>
+__device__ __forceinline__ void write_row(const Out& out, size_t row, const T* x, int64_t target, int vocab, const Sum& a, float ls) {
+    const bool none = a.s == 0.0f;                                // every logit is -infinity
+    out.lse[row] = none ? -__builtin_inff() : a.m + ls;
+    out.logp[row] = (uint64_t)target >= (uint64_t)vocab ? 0.0f : none ? -__builtin_inff() : (Elem<T>::one(x[target]) - a.m) - ls;
+    if constexpr (ENTROPY) {
+        const float h = ls - a.t * LN2 / a.s;
+        out.entropy[row] = none || h < 0.0f ? 0.0f : h;
+    }
+}
+__device__ __forceinline__ void write_top(const Out& out, size_t row, const Candidates& c, int top, const Sum& a, float ls) {
+    const int j = threadIdx.x;
+    if (j >= top) return;
+    const uint64_t r = c.chosen[j];
+    out.top_logp[row * top + j] = a.s == 0.0f ? -__builtin_inff() : (value_of(r) - a.m) - ls;
+    out.top_ids[row * top + j] = (int32_t)place_of(r);
+}
+__device__ __forceinline__ int64_t target_of(const void* targets, int is64, size_t row) {
+    return is64 ? static_cast<const int64_t*>(targets)[row] : static_cast<const int32_t*>(targets)[row];
+}
+}  // namespace lp
+
+// Workgroup (row, part of it).  Rows of one part are finished here, others leave a Part and their alternatives.
+template <class T, bool CACHED, bool ENTROPY, bool TOP>
+__global__ __launch_bounds__(lp::THREADS) void token_logprobs_kernel(const T* __restrict__ logits, const void* __restrict__ targets, int targets64,
+                                                                     lp::Out out, lp::Part* __restrict__ parts, uint64_t* __restrict__ part_tops,
+                                                                     int vocab, size_t width, int cut, int each, int top) {
+    using namespace lp;
+    constexpr int E = Elem<T>::E;
+    __shared__ Sum sums[WAVES];
+    const size_t row = blockIdx.x / cut;
+    const int part = blockIdx.x % cut, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const T* x = logits + row * width;
+    const int begin = min(vocab, part * each), end = min(vocab, begin + each);
+    const Stretch<T> st(x, begin, end);
+    Sum a{LEAST, 0.0f, 0.0f};
+    const int alone = st.single(threadIdx.x);
+    const float single[1] = {alone >= 0 ? Elem<T>::one(x[alone]) : -__builtin_inff()};
+    int p = threadIdx.x;
+    for (; p + (AT_ONCE - 1) * THREADS < st.pieces; p += AT_ONCE * THREADS) {
+        u32x4 v[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) v[u] = ld_stream_16<CACHED>(st.piece(p + u * THREADS));
+        float f[AT_ONCE * E];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+            float g[E];
+            Elem<T>::unpack(v[u], g);
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[u * E + i] = g[i];
+        }
+        add<ENTROPY>(a, f);
+    }
+    for (; p < st.pieces; p += THREADS) {
+        float f[E];
+        Elem<T>::unpack(ld_stream_16<CACHED>(st.piece(p)), f);
+        add<ENTROPY>(a, f);
+    }
+    if (alone >= 0) add<ENTROPY>(a, single);
+    const float mine = a.m;                                       // the largest of this thread's elements
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) a = join(a, Sum{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64)});
+    if (lane == 0) sums[wave] = a;
+    __syncthreads();
+    a = sums[0];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) a = join(a, sums[w]);
+    const float ls = logf(a.s);
+    if (threadIdx.x == 0) {
+        if (cut > 1) parts[blockIdx.x] = Part{a.m, a.s, a.t, 0.0f};
+        else write_row<T, ENTROPY>(out, row, x, target_of(targets, targets64, row), vocab, a, ls);
+    }
+    if constexpr (TOP) {
+        __shared__ Candidates c;
+        __shared__ float most[THREADS];
+        __shared__ uint8_t who[THREADS];
+        __shared__ int whos;
+        most[threadIdx.x] = mine;
+        if (threadIdx.x == 0) c.count = whos = 0;
+        __syncthreads();
+        // the top-th largest of the threads' largest (or a little less): bit by bit in the order of whole numbers, every wave by itself
+        uint32_t key[WAVES], found = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) key[w] = (uint32_t)(rank_of(most[w * 64 + lane], 0) >> 32);
+        for (uint32_t bit = 0x80000000u; bit >= (sizeof(T) == 4 ? 1u : 0x10000u); bit >>= 1) {
+            int n = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[w] >= (found | bit)));
+            if (n >= top) found |= bit;
+            if (bit == 1) break;
+        }
+        const float limit = value_of((uint64_t)found << 32);
+        // no limit where fewer than `top` threads have elements that are numbers
+        const bool all = !(limit > LEAST);
+        if (all || mine >= limit) who[atomicAdd(&whos, 1)] = (uint8_t)threadIdx.x;
+        __syncthreads();
+        // their elements, a piece a thread in a turn, and the single ones in a last turn
+        const int threads = whos, items = threads * ((st.pieces + THREADS - 1) / THREADS), turns = (items + THREADS - 1) / THREADS;
+        uint64_t least = 0;                                       // only what is larger can still be among the alternatives
+        for (int turn = 0; turn <= turns; ++turn) {
+            if (turn < turns) {
+                const int item = turn * THREADS + threadIdx.x, piece = item < items ? who[item % threads] + item / threads * THREADS : st.pieces;
+                if (piece < st.pieces) {
+                    float f[E];
+                    Elem<T>::unpack(ld_global_16(st.piece(piece)), f);
+#pragma unroll
+                    for (int i = 0; i < E; ++i)
+                        if (all || f[i] >= limit) {
+                            const uint64_t r = rank_of(f[i], st.place(piece) + i);
+                            if (r > least) c.list[atomicAdd(&c.count, 1)] = r;
+                        }
+                }
+            } else if (alone >= 0 && (all || single[0] >= limit)) {
+                const uint64_t r = rank_of(single[0], alone);
+                if (r > least) c.list[atomicAdd(&c.count, 1)] = r;
+            }
+            __syncthreads();
+            const int count = c.count;
+            __syncthreads();
+            if (turn == turns || count > KEPT) choose(c, count, top);
+            if (turn < turns && count > KEPT) {                   // many are as large: the first of them go on
+                least = c.chosen[top - 1];
+                if (threadIdx.x < top) c.list[threadIdx.x] = c.chosen[threadIdx.x];
+                if (threadIdx.x == 0) c.count = top;
+                __syncthreads();
+            }
+        }
+        if (cut > 1) {
+            if (threadIdx.x < top) part_tops[(size_t)blockIdx.x * top + threadIdx.x] = c.chosen[threadIdx.x];
+        } else {
+            write_top(out, row, c, top, a, ls);
+        }
+    }
+}
+
+// Rows that were cut: a workgroup a row.
+template <class T, bool ENTROPY, bool TOP>
+__global__ __launch_bounds__(lp::THREADS) void token_logprobs_join_kernel(const T* __restrict__ logits, const void* __restrict__ targets, int targets64,
+                                                                          lp::Out out, const lp::Part* __restrict__ parts,
+                                                                          const uint64_t* __restrict__ part_tops, int vocab, size_t width, int cut, int top) {
+    using namespace lp;
+    const size_t row = blockIdx.x;
+    const int lane = threadIdx.x & 63;
+    const T* x = logits + row * width;
+    Sum a{LEAST, 0.0f, 0.0f};
+    for (int i = lane; i < cut; i += 64) {                        // every wave by itself
+        const Part q = parts[row * cut + i];
+        a = join(a, Sum{q.m, q.s, q.t});
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) a = join(a, Sum{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64)});
+    const float ls = logf(a.s);
+    if (threadIdx.x == 0) write_row<T, ENTROPY>(out, row, x, target_of(targets, targets64, row), vocab, a, ls);
+    if constexpr (TOP) {
+        __shared__ Candidates c;
+        const int count = cut * top;                              // at most the list's length
+        for (int i = threadIdx.x; i < count; i += THREADS) c.list[i] = part_tops[row * count + i];
+        __syncthreads();
+        choose(c, count, top);
+        write_top(out, row, c, top, a, ls);
+    }
+}
+
+// The gradient: workgroup (row, part of it).  logits and d_logits may be the same memory: a thread writes where it alone has read.
+template <class T, bool CACHED, bool ENTROPY>
+__global__ __launch_bounds__(lp::THREADS) void token_logprobs_bwd_kernel(const T* logits, const void* __restrict__ targets, int targets64,
+                                                                         const float* __restrict__ lse, const float* __restrict__ entropy,
+                                                                         const float* __restrict__ d_logp, const float* __restrict__ d_entropy,
+                                                                         const float* __restrict__ d_lse, T* d_logits, int vocab, size_t width,
+                                                                         int cut, int each) {
+    using namespace lp;
+    constexpr int E = Elem<T>::E;
+    const size_t row = blockIdx.x / cut;
+    const int part = blockIdx.x % cut;
+    const T* x = logits + row * width;
+    T* dx = d_logits + row * width;
+    const int begin = min(vocab, part * each), end = min(vocab, begin + each);
+    const Stretch<T> st(x, begin, end);
+    const int64_t given = target_of(targets, targets64, row);
+    const bool has_target = (uint64_t)given < (uint64_t)vocab && d_logp;
+    const int target = has_target ? (int)given : -1;
+    const float g = has_target ? d_logp[row] : 0.0f, gh = ENTROPY ? d_entropy[row] : 0.0f, l = lse[row];
+    float k = (d_lse ? d_lse[row] : 0.0f) - g, kh = -gh * LN2;    // dx = p (k + kh log2 p)
+    if constexpr (ENTROPY) k -= gh * entropy[row];
+    // a row without a gradient, or without a logit above -infinity
+    const bool zero = (g == 0.0f && k == 0.0f && gh == 0.0f) || l == -__builtin_inff();
+    // dx = e (k + kh y) with e = 2^y; y is relative to c, which is lse log2(e) but for its rounding: that much goes into k and kh
+    const bool tame = fabsf(l) < 0x1p20f;
+    const float c = l * LOG2E;
+    if (tame) {
+        const float off = -fmaf(l, LOG2E, -c), e = fast_exp2(off);
+        k = fmaf(kh, off, k) * e;
+        kh *= e;
+    }
+    auto slope = [&](float v) {
+        const float y = tame ? fmaf(v, LOG2E, -c) : (v - l) * LOG2E;
+        const float e = fast_exp2(y);
+        if constexpr (ENTROPY) return e * fmaf(fmaxf(y, -0x1p20f), kh, k);
+        else return e * k;
+    };
+    auto with_target = [&](float v, bool there) {                 // the same bits wherever an element is computed
+#pragma clang fp contract(off)
+        return there ? v + g : v;
+    };
+    auto put = [&](int i) { Elem<T>::put(dx + i, zero ? 0.0f : with_target(slope(Elem<T>::one(x[i])), i == target)); };
+    // pieces of 16 bytes where both tensors have them at the same elements
+    if ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(d_logits)) % 16 != 0) {
+        for (int i = begin + threadIdx.x; i < end; i += THREADS) put(i);
+    } else {
+        const int alone = st.single(threadIdx.x);
+        if (alone >= 0) put(alone);
+        for (int p0 = threadIdx.x; p0 < st.pieces; p0 += AT_ONCE * THREADS) {
+            u32x4 v[AT_ONCE];
+            if (!zero) {
+#pragma unroll
+                for (int u = 0; u < AT_ONCE; ++u) v[u] = ld_stream_16<CACHED>(st.piece(min(p0 + u * THREADS, st.pieces - 1)));
+            }
+#pragma unroll
+            for (int u = 0; u < AT_ONCE; ++u) {
+                const int p = p0 + u * THREADS;
+                if (p >= st.pieces) break;
+                float f[E];
+                if (zero) {
+#pragma unroll
+                    for (int i = 0; i < E; ++i) f[i] = 0.0f;
+                } else {
+                    Elem<T>::unpack(v[u], f);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) f[i] = slope(f[i]);
+                    const int at = target - st.place(p);
+                    if ((unsigned)at < (unsigned)E) {
+#pragma unroll
+                        for (int i = 0; i < E; ++i) f[i] = with_target(f[i], i == at);
+                    }
+                }
+                st_global_16_nt(dx + st.place(p), Elem<T>::pack(f));
+            }
+        }
+    }
+    if (part == cut - 1)
+        for (size_t i = vocab + threadIdx.x; i < width; i += THREADS) Elem<T>::put(dx + i, 0.0f);
+}
+
+// ------------------------------------------------------------------------------------------
+namespace {
+using namespace lp;
+// Parts of a row, so that few rows fill the device: up to 1024 workgroups of 8 KB of a row or more; what the parts leave for the alternatives fits
+// the list that joins them.
+struct Cut { int parts, each; };
+Cut cut_of(size_t rows, int vocab, int elem_bytes, int top) {
+    size_t n = 1024 / rows;
+    n = std::min(n, (size_t)vocab * elem_bytes / 8192);
+    if (top) n = std::min(n, (size_t)2048 / top);
+    n = std::max(n, (size_t)1);
+    const int each = (int)(((vocab + n - 1) / n + 127) / 128 * 128);
+    return {(vocab + each - 1) / each, each};
+}
+// of the gradient: a workgroup's threads go round once
+int bwd_each(int elem_bytes) { return THREADS * AT_ONCE * 16 / elem_bytes; }
+}  // namespace
+
+bool token_logprobs_fits(size_t rows, int vocab, int bf16) {
+    const int each = bwd_each(bf16 ? 2 : 4);
+    return rows < ((size_t)1 << 24) && rows * ((vocab + each - 1) / each) < ((size_t)1 << 24);      // workgroups of 256 threads
+}
+
+size_t token_logprobs_workspace_bytes(size_t rows, int vocab, int top, int bf16) {
+    const Cut c = cut_of(rows, vocab, bf16 ? 2 : 4, top);
+    return c.parts > 1 ? rows * c.parts * (sizeof(Part) + 8 * (size_t)top) : 0;
+}
+
+int launch_token_logprobs(const void* logits, const void* targets, int targets64, float* logp, float* lse, float* entropy, float* top_logp,
+                          int32_t* top_ids, size_t rows, int vocab, size_t width, int top, int bf16, void* workspace, hipStream_t stream) {
+    const Cut c = cut_of(rows, vocab, bf16 ? 2 : 4, top);
+    const Out out{logp, lse, entropy, top_logp, top_ids};
+    Part* parts = static_cast<Part*>(workspace);
+    uint64_t* tops = reinterpret_cast<uint64_t*>(parts + (c.parts > 1 ? rows * c.parts : 0));
+    const bool cached = rows * vocab * (bf16 ? 2 : 4) <= kStreamCached;
+    auto go = [&](auto elem, auto in_cache, auto with_entropy, auto with_top) {
+        using T = decltype(elem);
+        const T* x = static_cast<const T*>(logits);
+        launch_kernel((token_logprobs_kernel<T, in_cache(), with_entropy(), with_top()>), dim3((unsigned)(rows * c.parts)), dim3(THREADS), 0, stream, x,
+                      targets, targets64, out, parts, tops, vocab, width, c.parts, c.each, top);
+        if (c.parts > 1)
+            launch_kernel((token_logprobs_join_kernel<T, with_entropy(), with_top()>), dim3((unsigned)rows), dim3(THREADS), 0, stream, x, targets, targets64,
+                          out, parts, tops, vocab, width, c.parts, top);
+    };
+    auto outputs = [&](auto elem, auto in_cache) {
+        if (entropy) { if (top) go(elem, in_cache, std::true_type{}, std::true_type{}); else go(elem, in_cache, std::true_type{}, std::false_type{}); }
+        else { if (top) go(elem, in_cache, std::false_type{}, std::true_type{}); else go(elem, in_cache, std::false_type{}, std::false_type{}); }
+    };
+    auto pick = [&](auto elem) { if (cached) outputs(elem, std::true_type{}); else outputs(elem, std::false_type{}); };
+    if (bf16) pick(uint16_t{}); else pick(float{});
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+int launch_token_logprobs_bwd(const void* logits, const void* targets, int targets64, const float* lse, const float* entropy, const float* d_logp,
+                              const float* d_entropy, const float* d_lse, void* d_logits, size_t rows, int vocab, size_t width, int bf16,
+                              hipStream_t stream) {
+    const int each = bwd_each(bf16 ? 2 : 4), cut = (vocab + each - 1) / each;
+    const bool cached = rows * vocab * (bf16 ? 4 : 8) <= kStreamCached;
+    auto go = [&](auto elem, auto in_cache, auto with_entropy) {
+        using T = decltype(elem);
+        launch_kernel((token_logprobs_bwd_kernel<T, in_cache(), with_entropy()>), dim3((unsigned)(rows * cut)), dim3(THREADS), 0, stream,
+                      static_cast<const T*>(logits), targets, targets64, lse, entropy, d_logp, d_entropy, d_lse, static_cast<T*>(d_logits), vocab, width, cut,
+                      each);
+    };
+    auto pick = [&](auto elem) {
+        if (cached) { if (d_entropy) go(elem, std::true_type{}, std::true_type{}); else go(elem, std::true_type{}, std::false_type{}); }
+        else { if (d_entropy) go(elem, std::false_type{}, std::true_type{}); else go(elem, std::false_type{}, std::false_type{}); }
+    };
+    if (bf16) pick(uint16_t{}); else pick(float{});
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+
+}  // namespace tyr

@@ -1,5 +1,5 @@
 // Memory-bound row kernels around the attention path (gfx950): device copy, rotary embedding,
-// fused residual + LayerNorm, and the decode step's "rotate q and k, append k and v to the cache".
+// and the decode step's "rotate q and k, append k and v to the cache".
 //
 // Reference semantics restated here:
 //   copy           Tyr/GPU/Kernels/Copy.lean:16-27 (copy64x64: out = in, one f32 tile per block)
@@ -7,15 +7,11 @@
 //                  halves along head_dim, y1 = x1 cos - x2 sin, y2 = x1 sin + x2 cos, cos / sin
 //                  [seq, head_dim/2] f32 broadcast over batch and heads, arithmetic in f32, result in
 //                  x's dtype; DSL twin Tyr/GPU/Kernels/Rotary.lean:13-66 (rotaryFwd, f32 64x64).
-//   layernorm      Tyr/GPU/Kernels/FusedLayerNorm.lean:28-140 (tkFusedLayerNormResidual1024):
-//                  out_resid = bf16(x + residual); statistics of the rounded out_resid in f32 over the
-//                  whole row; out = bf16((r - mean) * rsqrt(var + eps) * weight + bias); expected
-//                  values Examples/GPU/RunLayerNorm.lean:27-33 (torch layer_norm of x + residual).
 //   decode append  Tyr/Model/Qwen/Attention.lean:172-196 (forwardStep): applyRotaryEmb on the
 //                  single-token q and k, then sliceScatter of k and v into row `seq` of the
 //                  [batch, kv_heads, maxLen, head_dim] cache.
 //
-// All four are bound by HBM bandwidth: every lane moves 16-byte pieces, consecutive lanes touch
+// All of them are bound by HBM bandwidth: every lane moves 16-byte pieces, consecutive lanes touch
 // consecutive addresses, and the grids have many more workgroups than the device has CUs.
 #include "common.hpp"
 #include "launch.hpp"
@@ -143,111 +139,6 @@ __global__ __launch_bounds__(rw::THREADS) void decode_rope_append_kernel(
     st_global_16(dst + D / 2 + e0, b);
 }
 
-// WPR waves per row; a lane holds P <= 2 pieces (8 bf16) of it, lane, lane + 64 * WPR, so that all loads of a row, weights
-// included, are under way at once and many waves share the chip (one wave per row, up to 16 pieces a lane: 2222 x 4096
-// 16.8 us, 300 x 8192 17; so 13.1 and 7.1).
-template <int WPR, int P, bool CACHED>
-__global__ __launch_bounds__(WPR > 4 ? 64 * WPR : 256) void layernorm_residual_kernel(
-    const uint16_t* __restrict__ x, const uint16_t* __restrict__ res, const uint16_t* __restrict__ weight,
-    const uint16_t* __restrict__ bias, uint16_t* __restrict__ out, uint16_t* __restrict__ out_resid, size_t rows,
-    int d_model, float eps) {
-    constexpr int RPB = WPR > 4 ? 1 : 4 / WPR;
-    __shared__ float2 part[RPB][WPR];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = wave % WPR;
-    const size_t row = (size_t)blockIdx.x * RPB + wave / WPR;
-    const bool live = row < rows;
-    if (WPR == 1 && !live) return;
-    const int pieces = live ? d_model / 8 : 0;
-    const size_t at = row * d_model;
-    float v[P][8];
-    u32x4 a[P], b[P], w[P], bi[P];
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const int pc = lane + 64 * (wr + WPR * p);
-        if (pc < pieces) {
-            a[p] = ld_stream_16<CACHED>(x + at + pc * 8);
-            b[p] = ld_stream_16<CACHED>(res + at + pc * 8);
-        }
-    }
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const int pc = lane + 64 * (wr + WPR * p);
-        if (pc < pieces) {
-            w[p] = ld_global_16(weight + pc * 8);
-            bi[p] = ld_global_16(bias + pc * 8);
-        }
-    }
-    float sum = 0.0f;
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const int pc = lane + 64 * (wr + WPR * p);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[p][i] = 0.0f;
-        if (pc < pieces) {
-            float f[8], g[8];
-            rw::unpack8(a[p], f);
-            rw::unpack8(b[p], g);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] += g[i];
-            const u32x4 r16 = rw::pack8(f);                     // out_resid is the bf16-rounded sum ...
-            st_global_16_nt(out_resid + at + pc * 8, r16);
-            rw::unpack8(r16, v[p]);                             // ... and the statistics are taken from it
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum += v[p][i];
-        }
-    }
-    auto wave_sum = [](float s) {
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) s += __shfl_xor(s, o, 64);
-        return sum_xor32(s);
-    };
-    // mean and sum of squares about it: of each wave's elements, then of the row's waves together
-    auto elements = [&](int i) {                                // of wave i
-        int c = 0;
-#pragma unroll
-        for (int p = 0; p < P; ++p) c += max(0, min(64, pieces - 64 * (i + WPR * p)));
-        return 8.0f * (float)c;
-    };
-    float mean = wave_sum(sum) / fmaxf(elements(wr), 1.0f);
-    float sq = 0.0f;
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-        if (lane + 64 * (wr + WPR * p) < pieces) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) { const float c = v[p][i] - mean; sq += c * c; }
-        }
-    sq = wave_sum(sq);
-    if constexpr (WPR > 1) {
-        if (lane == 0) part[wave / WPR][wr] = float2{mean, sq};
-        __syncthreads();
-        if (!live) return;
-        float2 q[WPR];
-        float total = 0.0f;
-#pragma unroll
-        for (int i = 0; i < WPR; ++i) {
-            q[i] = part[wave / WPR][i];
-            total += q[i].x * elements(i);
-        }
-        mean = total / (float)d_model;
-        sq = 0.0f;
-#pragma unroll
-        for (int i = 0; i < WPR; ++i) { const float d = q[i].x - mean; sq += q[i].y + elements(i) * d * d; }
-    }
-    const float inv_std = rsqrtf(sq / (float)d_model + eps);
-#pragma unroll
-    for (int p = 0; p < P; ++p) {
-        const int pc = lane + 64 * (wr + WPR * p);
-        if (pc < pieces) {
-            float wf[8], bf[8], o[8];
-            rw::unpack8(w[p], wf);
-            rw::unpack8(bi[p], bf);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = (v[p][i] - mean) * inv_std * wf[i] + bf[i];
-            st_global_16_nt(out + at + pc * 8, rw::pack8(o));
-        }
-    }
-}
-
 // ------------------------------------------------------------------------------------------
 int launch_copy(const void* src, void* dst, size_t bytes, hipStream_t stream) {
     const size_t n16 = bytes / 16;
@@ -291,25 +182,6 @@ int launch_decode_rope_append(const void* q, const void* k_new, const void* v_ne
                        static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_new),
                        static_cast<const uint16_t*>(v_new), cosp, sinp, static_cast<uint16_t*>(q_out),
                        static_cast<uint16_t*>(k_cache), static_cast<uint16_t*>(v_cache), nq, nkv, D, kv_stride, pos);
-    return hipGetLastError() == hipSuccess ? 0 : -1;
-}
-
-int launch_layernorm_residual(const void* x, const void* residual, const void* weight, const void* bias, void* out,
-                              void* out_resid, size_t rows, int d_model, float eps, hipStream_t stream) {
-    auto go = [&](auto wpr, auto p) {
-        constexpr int W = wpr(), RPB = W > 4 ? 1 : 4 / W;       // rows per workgroup
-        auto kernel = rows * d_model * 8 <= kStreamCached ? &layernorm_residual_kernel<W, p(), true> : &layernorm_residual_kernel<W, p(), false>;
-        launch_kernel(kernel, dim3((unsigned)((rows + RPB - 1) / RPB)), dim3(W > 4 ? 64 * W : 256), 0, stream,
-                           static_cast<const uint16_t*>(x), static_cast<const uint16_t*>(residual), static_cast<const uint16_t*>(weight),
-                           static_cast<const uint16_t*>(bias), static_cast<uint16_t*>(out), static_cast<uint16_t*>(out_resid), rows,
-                           d_model, eps);
-    };
-    using std::integral_constant;
-    if (d_model <= 512) go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-    else if (d_model <= 1024) go(integral_constant<int, 1>{}, integral_constant<int, 2>{});
-    else if (d_model <= 2048) go(integral_constant<int, 2>{}, integral_constant<int, 2>{});
-    else if (d_model <= 4096) go(integral_constant<int, 4>{}, integral_constant<int, 2>{});
-    else go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
     return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 

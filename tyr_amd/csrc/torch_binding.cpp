@@ -71,7 +71,10 @@ public:
     X(tyr_hip_copy) X(tyr_hip_gemm_workspace_bytes) X(tyr_hip_gemm_bf16_batched_ws) X(tyr_hip_gemm_fp8_ws)                    \
     X(tyr_hip_mse_loss_grad_workspace_bytes) X(tyr_hip_mse_loss_grad) X(tyr_hip_sgd_step)                                    \
     X(tyr_hip_rmsnorm_residual) X(tyr_hip_rmsnorm_residual_bwd_workspace_bytes) X(tyr_hip_rmsnorm_residual_bwd)              \
-    X(tyr_hip_paged_rope_append) X(tyr_hip_paged_decode_workspace_bytes) X(tyr_hip_paged_decode)
+    X(tyr_hip_paged_rope_append) X(tyr_hip_paged_decode_workspace_bytes) X(tyr_hip_paged_decode)                             \
+    X(tyr_hip_layernorm_residual_bwd_workspace_bytes) X(tyr_hip_layernorm_residual_bwd) X(tyr_hip_embedding)                 \
+    X(tyr_hip_embedding_bwd_workspace_bytes) X(tyr_hip_embedding_bwd) X(tyr_hip_token_logprobs_workspace_bytes)              \
+    X(tyr_hip_token_logprobs) X(tyr_hip_token_logprobs_bwd)
 const struct Api {
 #define X(f) Symbol<decltype(&::f)> f{#f};
     TYR_ENTRY_POINTS(X)
@@ -137,7 +140,7 @@ double real(PyObject* o) {
 }
 float attn_scale(PyObject* o, int64_t D) { return (float)(o == Py_None ? 1.0 / std::sqrt((double)D) : real(o)); }
 
-PyObject* wrap(at::Tensor t) { return THPVariable_Wrap(std::move(t)); }
+PyObject* wrap(at::Tensor t) { return THPVariable_Wrap(std::move(t)); }      // a tensor that was not made is None
 template <class... T>
 PyObject* wrap_tuple(T&&... t) {
     PyObject* items[] = {wrap(std::forward<T>(t))...};
@@ -310,28 +313,6 @@ PyObject* rope_fwd(PyObject* const* a) {
     return wrap(std::move(y));
 }
 
-// (x, residual, weight, bias, eps)
-PyObject* layernorm_residual(PyObject* const* a) {
-    const at::Tensor &x = checked(a[0], "x", at::kBFloat16), &res = checked(a[1], "residual", at::kBFloat16),
-                     &w = checked(a[2], "weight", at::kBFloat16), &b = checked(a[3], "bias", at::kBFloat16);
-    const float eps = (float)real(a[4]);
-    if (x.dim() == 0) fail("x must have dim >= 1");
-    const int64_t d = x.size(-1);
-    if (res.sizes() != x.sizes() || w.dim() != 1 || w.size(0) != d || b.dim() != 1 || b.size(0) != d)
-        fail("residual must match x, weight and bias must be [d_model]");
-    at::Tensor out, out_resid;
-    int rc;
-    {
-        NoGil nogil;
-        out = empty_like(x);
-        out_resid = empty_like(x);
-        rc = api.tyr_hip_layernorm_residual(x.data_ptr(), res.data_ptr(), w.data_ptr(), b.data_ptr(), out.data_ptr(), out_resid.data_ptr(),
-                                            d ? x.numel() / d : 0, d, eps, stream());
-    }
-    check_status(rc, "fusedLayerNormResidual");
-    return wrap_tuple(std::move(out), std::move(out_resid));
-}
-
 // (src)
 PyObject* copy(PyObject* const* a) {
     const at::Tensor& src = tensor(a[0], "input");
@@ -373,6 +354,61 @@ const at::Tensor* optional(PyObject* o, const char* name, at::ScalarType dtype, 
     return o == Py_None ? nullptr : &checked(o, name, dtype, ndim);
 }
 void* pointer(const at::Tensor* t) { return t ? t->data_ptr() : nullptr; }
+
+// (x, residual, weight, bias, eps, stream_given)
+PyObject* layernorm_residual(PyObject* const* a) {
+    const at::Tensor& x = checked(a[0], "x", at::kBFloat16);
+    const at::Tensor* res = optional(a[1], "residual", at::kBFloat16);
+    const at::Tensor& w = checked(a[2], "weight", at::kBFloat16);
+    const at::Tensor* b = optional(a[3], "bias", at::kBFloat16);
+    const float eps = (float)real(a[4]);
+    if (x.dim() == 0) fail("x must have dim >= 1");
+    const int64_t d = x.size(-1);
+    if ((res && res->sizes() != x.sizes()) || w.dim() != 1 || w.size(0) != d || (b && (b->dim() != 1 || b->size(0) != d)))
+        fail("residual must match x, weight and bias must be [d_model]");
+    not_empty({&x}, "fusedLayerNormResidual");
+    const OnDevice on(x, {res, &w, b}, truth(a[5]));
+    at::Tensor out, out_resid;
+    int rc;
+    {
+        NoGil nogil;
+        out = empty_like(x);
+        out_resid = res ? empty_like(x) : x;
+        rc = api.tyr_hip_layernorm_residual(x.data_ptr(), pointer(res), w.data_ptr(), pointer(b), out.data_ptr(),
+                                            res ? out_resid.data_ptr() : nullptr, d ? x.numel() / d : 0, d, eps, stream());
+    }
+    check_status(rc, "fusedLayerNormResidual");
+    return wrap_tuple(std::move(out), std::move(out_resid));
+}
+
+// (d_out, resid, weight, eps, d_resid, bias, stream_given) -> (dx, dweight, dbias or None)
+PyObject* layernorm_residual_bwd(PyObject* const* a) {
+    const at::Tensor &g = checked(a[0], "dOut", at::kBFloat16), &h = checked(a[1], "resid", at::kBFloat16),
+                     &w = checked(a[2], "weight", at::kBFloat16, 1);
+    const float eps = (float)real(a[3]);
+    const at::Tensor* dr = optional(a[4], "dResid", at::kBFloat16);
+    const bool bias = truth(a[5]);
+    if (h.dim() == 0) fail("resid must have dim >= 1");
+    const int64_t d = h.size(-1);
+    if (g.sizes() != h.sizes() || (dr && dr->sizes() != h.sizes()) || w.size(0) != d)
+        fail("dOut and dResid must match resid, weight must be [d_model]");
+    not_empty({&h}, "layerNormResidualBwd");
+    const OnDevice on(h, {&g, &w, dr}, truth(a[6]));
+    at::Tensor dx, dw, db;
+    int rc;
+    {
+        NoGil nogil;
+        dx = empty_like(h);
+        dw = empty_like(w);
+        if (bias) db = empty_like(w);
+        const int64_t rows = d ? h.numel() / d : 0;
+        const at::Tensor ws = scratch(api.tyr_hip_layernorm_residual_bwd_workspace_bytes(rows, d), h);
+        rc = api.tyr_hip_layernorm_residual_bwd(g.data_ptr(), pointer(dr), h.data_ptr(), w.data_ptr(), dx.data_ptr(), dw.data_ptr(),
+                                                bias ? db.data_ptr() : nullptr, rows, d, eps, ws.data_ptr(), ws.numel(), stream());
+    }
+    check_status(rc, "layerNormResidualBwd");
+    return wrap_tuple(std::move(dx), std::move(dw), std::move(db));
+}
 
 // (x, residual, weight, eps, e4m3, stream_given) -> (out, out_resid) or (out, row_scale, out_resid)
 PyObject* rmsnorm_residual(PyObject* const* a) {
@@ -518,6 +554,146 @@ PyObject* paged_decode(PyObject* const* a) {
     }
     check_status(rc, "pagedDecode");
     return wrap_tuple(std::move(o), std::move(lse));
+}
+
+// ---- tokens: embedding and log probabilities
+int index_dtype(const at::Tensor& t, const char* name) {
+    if (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong) fail(std::string(name) + " must have dtype torch.int32 or torch.int64");
+    check(t, name, t.scalar_type());
+    return t.scalar_type() == at::kInt ? TYR_HIP_I32 : TYR_HIP_I64;
+}
+int float_dtype(const at::Tensor& t, const char* name, int ndim = -1) {
+    if (t.scalar_type() != at::kFloat && t.scalar_type() != at::kBFloat16) fail(std::string(name) + " must have dtype torch.float32 or torch.bfloat16");
+    check(t, name, t.scalar_type(), ndim);
+    return t.scalar_type() == at::kFloat ? TYR_HIP_F32 : TYR_HIP_BF16;
+}
+
+// (ids, table, scale, stream_given)
+PyObject* embedding(PyObject* const* a) {
+    const at::Tensor &ids = tensor(a[0], "ids"), &table = tensor(a[1], "table");
+    const int index = index_dtype(ids, "ids"), dtype = float_dtype(table, "table", 2);
+    const float scale = (float)real(a[2]);
+    if (ids.dim() > 3) fail("ids must have dim <= 3");
+    const int64_t vocab = table.size(0), d = table.size(1);
+    not_empty({&ids, &table}, "embedding");
+    const OnDevice on(ids, {&table}, truth(a[3]));
+    at::DimVector sizes(ids.sizes().begin(), ids.sizes().end());
+    sizes.push_back(d);
+    at::Tensor out;
+    int rc;
+    {
+        NoGil nogil;
+        out = empty(sizes, table.scalar_type(), table);
+        rc = api.tyr_hip_embedding(ids.data_ptr(), index, table.data_ptr(), out.data_ptr(), ids.numel(), vocab, d, scale, dtype, stream());
+    }
+    check_status(rc, "embedding");
+    return wrap(std::move(out));
+}
+
+// (d_out, ids, vocab, scale, into, stream_given)
+PyObject* embedding_bwd(PyObject* const* a) {
+    const at::Tensor &g = tensor(a[0], "dOut"), &ids = tensor(a[1], "ids");
+    const int dtype = float_dtype(g, "dOut"), index = index_dtype(ids, "ids");
+    const int64_t vocab = count(a[2], "vocab");
+    const float scale = (float)real(a[3]);
+    if (g.dim() != ids.dim() + 1 || g.sizes().slice(0, ids.dim()) != ids.sizes()) fail("dOut must have the shape of ids and d_model behind it");
+    const int64_t d = g.size(-1);
+    const at::Tensor* into = optional(a[4], "into", g.scalar_type(), 2);
+    if (into && (into->size(0) != vocab || into->size(1) != d)) fail("into must be [vocab, d_model]");
+    not_empty({&ids, &g}, "embeddingBwd");
+    const OnDevice on(g, {&ids, into}, truth(a[5]));
+    at::Tensor table;
+    int rc;
+    {
+        NoGil nogil;
+        const size_t bytes = api.tyr_hip_embedding_bwd_workspace_bytes(ids.numel(), vocab, d, dtype);
+        // a shape that the call refuses is not allocated for
+        if (into) table = *into;
+        else if (bytes) table = empty({vocab, d}, g.scalar_type(), g);
+        const at::Tensor ws = scratch(bytes, g);
+        rc = api.tyr_hip_embedding_bwd(g.data_ptr(), ids.data_ptr(), index, bytes ? table.data_ptr() : ws.data_ptr(), ids.numel(), vocab, d, scale,
+                                       into != nullptr, dtype, ws.data_ptr(), ws.numel(), stream());
+    }
+    check_status(rc, "embeddingBwd");
+    return wrap(std::move(table));
+}
+
+// logits [..., width], one target and one number of each output a row
+struct Logits {
+    const at::Tensor &x, &targets;
+    int dtype, index;
+    int64_t width, vocab, rows;
+    Logits(PyObject* px, PyObject* pt, PyObject* pv) : x(tensor(px, "logits")), targets(tensor(pt, "targets")) {
+        dtype = float_dtype(x, "logits");
+        index = index_dtype(targets, "targets");
+        if (x.dim() == 0 || x.sizes().slice(0, x.dim() - 1) != targets.sizes()) fail("targets must have the shape of logits without the last extent");
+        width = x.size(-1);
+        vocab = pv == Py_None ? width : count(pv, "vocab");
+        if (vocab > width) fail("vocab must not exceed the logits' last extent");
+        rows = targets.numel();
+    }
+    const at::Tensor& row_values(PyObject* o, const char* name) const {
+        const at::Tensor& t = checked(o, name, at::kFloat);
+        if (t.sizes() != targets.sizes()) fail(std::string(name) + " must have the shape of targets");
+        return t;
+    }
+    const at::Tensor* optional_values(PyObject* o, const char* name) const { return o == Py_None ? nullptr : &row_values(o, name); }
+};
+
+// (logits, targets, vocab, top, entropy, stream_given) -> (logp, lse, entropy or None, top_logp or None, top_ids or None)
+PyObject* token_logprobs(PyObject* const* a) {
+    const Logits l(a[0], a[1], a[2]);
+    const int64_t top = count(a[3], "top");
+    const bool with_entropy = truth(a[4]);
+    not_empty({&l.x}, "tokenLogprobs");
+    if (l.vocab == 0 || top > l.vocab) check_status(TYR_HIP_ERR_BAD_SHAPE, "tokenLogprobs");
+    if (top > TYR_HIP_TOKEN_LOGPROBS_MAX_TOP) check_status(TYR_HIP_ERR_UNSUPPORTED, "tokenLogprobs");
+    const OnDevice on(l.x, {&l.targets}, truth(a[5]));
+    at::Tensor logp, lse, entropy, top_logp, top_ids;
+    int rc;
+    {
+        NoGil nogil;
+        logp = empty(l.targets.sizes(), at::kFloat, l.x);
+        lse = empty(l.targets.sizes(), at::kFloat, l.x);
+        if (with_entropy) entropy = empty(l.targets.sizes(), at::kFloat, l.x);
+        if (top) {
+            at::DimVector sizes(l.targets.sizes().begin(), l.targets.sizes().end());
+            sizes.push_back(top);
+            top_logp = empty(sizes, at::kFloat, l.x);
+            top_ids = empty(sizes, at::kInt, l.x);
+        }
+        const size_t bytes = api.tyr_hip_token_logprobs_workspace_bytes(l.rows, l.vocab, top, l.dtype);
+        at::Tensor ws;
+        if (bytes) ws = scratch(bytes, l.x);
+        rc = api.tyr_hip_token_logprobs(l.x.data_ptr(), l.targets.data_ptr(), l.index, (float*)logp.data_ptr(), (float*)lse.data_ptr(),
+                                        with_entropy ? (float*)entropy.data_ptr() : nullptr, top ? (float*)top_logp.data_ptr() : nullptr,
+                                        top ? (int32_t*)top_ids.data_ptr() : nullptr, l.rows, l.vocab, l.width, top, l.dtype,
+                                        bytes ? ws.data_ptr() : nullptr, bytes, stream());
+    }
+    check_status(rc, "tokenLogprobs");
+    return wrap_tuple(std::move(logp), std::move(lse), std::move(entropy), std::move(top_logp), std::move(top_ids));
+}
+
+// (d_logp, logits, targets, lse, vocab, entropy, d_entropy, d_lse, in_place, stream_given)
+PyObject* token_logprobs_bwd(PyObject* const* a) {
+    const Logits l(a[1], a[2], a[4]);
+    const at::Tensor *g = l.optional_values(a[0], "dLogp"), &lse = l.row_values(a[3], "lse"), *entropy = l.optional_values(a[5], "entropy"),
+                     *gh = l.optional_values(a[6], "dEntropy"), *gl = l.optional_values(a[7], "dLse");
+    const bool in_place = truth(a[8]);
+    if (gh && !entropy) fail("dEntropy needs the forward's entropy");
+    not_empty({&l.x}, "tokenLogprobsBwd");
+    const OnDevice on(l.x, {&l.targets, g, &lse, entropy, gh, gl}, truth(a[9]));
+    at::Tensor d;
+    int rc;
+    {
+        NoGil nogil;
+        d = in_place ? l.x : empty_like(l.x);
+        rc = api.tyr_hip_token_logprobs_bwd(l.x.data_ptr(), l.targets.data_ptr(), l.index, (const float*)lse.data_ptr(), (const float*)pointer(entropy),
+                                            (const float*)pointer(g), (const float*)pointer(gh), (const float*)pointer(gl), d.data_ptr(), l.rows,
+                                            l.vocab, l.width, l.dtype, stream());
+    }
+    check_status(rc, "tokenLogprobsBwd");
+    return wrap(std::move(d));
 }
 
 // ---- products
@@ -693,10 +869,11 @@ PyObject* load(PyObject*, PyObject* args) {
 PyMethodDef methods[] = {
     {"load", load, METH_VARARGS, nullptr},
     TYR_METHOD(flash_attn_fwd, 8), TYR_METHOD(flash_attn_bwd, 11), TYR_METHOD(gqa_decode, 8), TYR_METHOD(decode_rope_append, 8),
-    TYR_METHOD(rope_fwd, 3), TYR_METHOD(layernorm_residual, 5), TYR_METHOD(copy, 1), TYR_METHOD(gemm_bf16, 3),
+    TYR_METHOD(rope_fwd, 3), TYR_METHOD(layernorm_residual, 6), TYR_METHOD(copy, 1), TYR_METHOD(gemm_bf16, 3),
     TYR_METHOD(matmul_bf16, 3), TYR_METHOD(gemm_fp8, 5), TYR_METHOD(gemm_fp8_scaled, 7), TYR_METHOD(mse_loss_grad, 2),
     TYR_METHOD(sgd_step, 4), TYR_METHOD(rmsnorm_residual, 6), TYR_METHOD(rmsnorm_residual_bwd, 6), TYR_METHOD(paged_rope_append, 13),
-    TYR_METHOD(paged_decode, 11), {nullptr, nullptr, 0, nullptr}};
+    TYR_METHOD(paged_decode, 11), TYR_METHOD(layernorm_residual_bwd, 7), TYR_METHOD(embedding, 4), TYR_METHOD(embedding_bwd, 6),
+    TYR_METHOD(token_logprobs, 6), TYR_METHOD(token_logprobs_bwd, 10), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tyr_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -29,6 +29,8 @@ _n = _lib.load_binding(TyrGpuError)
 _flash_attn_fwd, _flash_attn_bwd, _gqa_decode, _decode_rope_append = _n.flash_attn_fwd, _n.flash_attn_bwd, _n.gqa_decode, _n.decode_rope_append
 _rope_fwd, _layernorm_residual, _copy, _matmul_bf16, _gemm_bf16 = _n.rope_fwd, _n.layernorm_residual, _n.copy, _n.matmul_bf16, _n.gemm_bf16
 _gemm_fp8, _gemm_fp8_scaled, _mse_loss_grad, _sgd_step = _n.gemm_fp8, _n.gemm_fp8_scaled, _n.mse_loss_grad, _n.sgd_step
+_layernorm_residual_bwd, _embedding, _embedding_bwd = _n.layernorm_residual_bwd, _n.embedding, _n.embedding_bwd
+_token_logprobs, _token_logprobs_bwd = _n.token_logprobs, _n.token_logprobs_bwd
 _rmsnorm_residual, _rmsnorm_residual_bwd, _paged_rope_append, _paged_decode = _n.rmsnorm_residual, _n.rmsnorm_residual_bwd, _n.paged_rope_append, _n.paged_decode
 
 
@@ -129,10 +131,21 @@ def rope_fwd(x, cos, sin, stream=None):
 
 
 def layernorm_residual(x, residual, weight, bias, eps: float = 1e-5, stream=None):
-    """(out, outResid) = fusedLayerNormResidual x residual weight bias.  bf16; x, residual [..., d]; weight, bias [d]."""
+    """(out, outResid) = fusedLayerNormResidual x residual weight bias.  bf16; x, residual [..., d]; weight, bias [d].
+    Without a residual (None) outResid is x itself; without a bias (None) none is added."""
     if stream is None:
-        return _layernorm_residual(x, residual, weight, bias, eps)
-    return _on_stream(stream, _layernorm_residual, x, residual, weight, bias, eps)
+        return _layernorm_residual(x, residual, weight, bias, eps, False)
+    return _on_stream(stream, _layernorm_residual, x, residual, weight, bias, eps, True)
+
+
+def layernorm_residual_bwd(d_out, resid, weight, eps: float = 1e-5, d_resid=None, bias: bool = True, stream=None):
+    """(dX, dWeight, dBias) = layerNormResidualBwd dOut resid weight: gradients of layernorm_residual, bf16.  resid [..., d] is
+    the outResid that the forward returned, d_out the gradient of its out and d_resid (or None) the one that reaches outResid
+    from the layers behind.  dX [..., d] is the gradient of x and of the residual alike; dWeight, dBias [d] (``bias`` False:
+    dBias is None)."""
+    if stream is None:
+        return _layernorm_residual_bwd(d_out, resid, weight, eps, d_resid, bias, False)
+    return _on_stream(stream, _layernorm_residual_bwd, d_out, resid, weight, eps, d_resid, bias, True)
 
 
 def rmsnorm_residual(x, residual, weight, eps: float = 1e-6, stream=None):
@@ -189,6 +202,47 @@ def paged_decode(q, k_pages, v_pages, page_table, kv_lens, scale: float | None =
     if stream is None:
         return _paged_decode(q, k_pages, v_pages, page_table, kv_lens, scale, window, sinks, k_scale, v_scale, False)
     return _on_stream(stream, _paged_decode, q, k_pages, v_pages, page_table, kv_lens, scale, window, sinks, k_scale, v_scale, True)
+
+
+def embedding(ids, table, scale: float = 1.0, stream=None):
+    """out = embedding ids table scale: out[..., :] = scale * table[ids[...]].  ids int32 or int64, any extents up to three;
+    table bf16 or f32 [vocab, d] -> [..., d] of its type.  An id outside of [0, vocab) (padding) gives zeros."""
+    if stream is None:
+        return _embedding(ids, table, scale, False)
+    return _on_stream(stream, _embedding, ids, table, scale, True)
+
+
+def embedding_bwd(d_out, ids, vocab: int, scale: float = 1.0, into=None, stream=None):
+    """dTable = embeddingBwd dOut ids: row v is scale times the sum of the rows of d_out whose id is v, zero where there are
+    none.  d_out bf16 or f32 [..., d]; ids int32 or int64 [...]; -> [vocab, d] of d_out's type.  Ids outside of [0, vocab) add
+    nothing.  With ``into`` (a gradient that is there, [vocab, d] of d_out's type: tied weights, accumulated batches) the sums
+    are added to its rows, in place, and it is returned.  The result is reproducible."""
+    if stream is None:
+        return _embedding_bwd(d_out, ids, vocab, scale, into, False)
+    return _on_stream(stream, _embedding_bwd, d_out, ids, vocab, scale, into, True)
+
+
+def token_logprobs(logits, targets, vocab: int | None = None, top: int = 0, entropy: bool = True, stream=None):
+    """(logp, lse, entropy, topLogp, topIds) = tokenLogprobs logits targets: for every row of logits (bf16 or f32 [..., width])
+    the log of the sum of exponentials, the log probability of its target (int32 or int64 [...]; 0 for one outside of
+    [0, vocab): padding), the entropy, and the ``top`` (up to 64) largest log probabilities with their ids (int32), largest
+    first, equal ones by id.  The first ``vocab`` columns count (None: all); the others are the padding of the product that
+    made the logits.  logp, lse, entropy f32 [...]; topLogp, topIds [..., top]; what was not asked for is None.  Logits of
+    -infinity have no probability; a row of nothing else has logp = lse = -infinity and entropy 0."""
+    if stream is None:
+        return _token_logprobs(logits, targets, vocab, top, entropy, False)
+    return _on_stream(stream, _token_logprobs, logits, targets, vocab, top, entropy, True)
+
+
+def token_logprobs_bwd(d_logp, logits, targets, lse, vocab: int | None = None, entropy=None, d_entropy=None, d_lse=None,
+                       in_place: bool = False, stream=None):
+    """dLogits = tokenLogprobsBwd dLogp logits targets lse: the gradient of token_logprobs' logp, entropy and lse with respect
+    to the logits, of their type and shape (zeros in the columns from ``vocab`` on).  lse and, with d_entropy, entropy are the
+    forward's; d_logp, d_entropy, d_lse f32 [...] or None (zeros).  ``in_place`` overwrites the logits instead of
+    allocating."""
+    if stream is None:
+        return _token_logprobs_bwd(d_logp, logits, targets, lse, vocab, entropy, d_entropy, d_lse, in_place, False)
+    return _on_stream(stream, _token_logprobs_bwd, d_logp, logits, targets, lse, vocab, entropy, d_entropy, d_lse, in_place, True)
 
 
 def copy(src, stream=None):
