@@ -493,8 +493,8 @@ int tyr_hip_embedding_bwd(const void* d_out, const void* ids, int ids_dtype, voi
  * of padding apart); among the alternatives NaN stands with the -infinities.
  *   workspace : tyr_hip_token_logprobs_workspace_bytes(...) bytes (0 also for shapes that the call refuses), 16-byte aligned, contents
  *               arbitrary; calls that overlap in time need one each (may be NULL where that is 0)
- * Supported: top <= vocab and <= TYR_HIP_TOKEN_LOGPROBS_MAX_TOP; vocab < 2^30, width < 2^31; rows and, with 16 KB of a row each, the
- * gradient's workgroups rows * ceil(vocab / (8192 bf16, 4096 f32)) < 2^24.
+ * Supported: top <= vocab and <= TYR_HIP_TOKEN_LOGPROBS_MAX_TOP; vocab < 2^30, width < 2^31; rows and the
+ * gradient's workgroups rows * ceil(vocab / (4096 bf16, 2048 f32)) < 2^24.
  */
 #define TYR_HIP_TOKEN_LOGPROBS_MAX_TOP 64
 size_t tyr_hip_token_logprobs_workspace_bytes(uint64_t rows, uint64_t vocab, uint64_t top, int dtype);

@@ -6,8 +6,9 @@
 //   dx = p (d_lse - d_logp - d_entropy (ln p + entropy)) + d_logp [at the target]
 //
 // One pass over the row: every lane keeps m, s and t of its own elements and scales them when its m grows; they are joined at the end, in f32.
-// The alternatives need no second pass: the `top`-th largest of the lanes' m is no larger than the `top`-th largest element, so only the
-// elements of lanes that reach it are read once more, and of those the ones that reach it are few.
+// The alternatives need no second pass: the `top`-th largest of the lanes' m is no larger than the `top`-th largest element.  Every lane keeps
+// the maxima of its blocks of 64 bytes, too, and only the blocks that reach that limit are read once more (all of such a lane's elements:
+// each 16 bytes of them another cache line, with 20 alternatives nearly the whole row again, 4096 x 50001 108 us, 82 so).
 //
 // Bound by HBM (bf16: and nearly by the vector units, 7 to 9 instructions an element, of which the exponential counts as four).
 //
@@ -15,20 +16,25 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "common.hpp"
 #include "launch.hpp"
+#include "rows.hpp"
 
 namespace tyr {
 
 namespace lp {
 constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int AT_ONCE = 4;                        // pieces a lane asks for together
+constexpr int BWD_THREADS = 256, BWD_AT_ONCE = 2; // of the gradient
 constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 constexpr float LEAST = -3.402823466e38f;         // m of no element: the smallest finite number
-// sizes of m, and of the least element, up to which an element's exponent is one multiplication and addition
-constexpr float TAME = 1024.0f, FAR = 1e30f;
+constexpr float TAME = 1024.0f;                   // size of m up to which an element's exponent is one multiplication and addition
 constexpr int MAX_TOP = 64;
 constexpr int KEPT = 512;                         // candidates that stay when the list is cut
+constexpr int TURN = 128;                         // threads that add to it in a turn
+constexpr int LIST = KEPT + TURN * 8;
+constexpr int SLOTS = 16;                         // maxima of blocks a thread; block b is in slot b % SLOTS
+constexpr int MOST_BLOCKS = 1024;
+constexpr int JOINED = 256;                       // alternatives of all parts together that the join looks for its limit among
 
 template <class T> struct Elem;
 template <> struct Elem<uint16_t> {
@@ -89,50 +95,53 @@ __device__ __forceinline__ Sum join(Sum a, Sum b) {
     const float ea = fast_exp2(da), eb = fast_exp2(db);
     return {m, a.s * ea + b.s * eb, (a.t + da * a.s) * ea + (b.t + db * b.s) * eb};
 }
-// N elements joined to a sum.  Where m is large the rounding of m log2(e) weighs more than a difference taken first, and where an element is
-// -infinity or near it 0 * infinity is not 0: differences are taken first there, and bounded.
+// N elements joined to a sum; the largest of them.  Where m is large the rounding of m log2(e) weighs more than a difference taken first: it is.
+// An element of -infinity or near it makes t NaN, being 0 * infinity: the block is added once more, with bounded differences (a look at the
+// least of the elements costs every block as much as a sixteenth of its exponentials).
 template <bool ENTROPY, int N>
-__device__ __forceinline__ void add(Sum& a, const float (&x)[N]) {
-    float most = x[0], least = x[0];
+__device__ __forceinline__ float add(Sum& a, const float (&x)[N]) {
+    float most = x[0];
 #pragma unroll
-    for (int i = 1; i < N; ++i) {
-        most = fmaxf(most, x[i]);
-        if constexpr (ENTROPY) least = fminf(least, x[i]);
-    }
+    for (int i = 1; i < N; ++i) most = fmaxf(most, x[i]);
     if (most > a.m) {
         const float d = fmaxf((a.m - most) * LOG2E, -0x1p20f), e = fast_exp2(d);
         if constexpr (ENTROPY) a.t = (a.t + d * a.s) * e;
         a.s *= e;
         a.m = most;
     }
-    const bool tame = fabsf(a.m) < TAME && (!ENTROPY || least > -FAR);
-    if (__builtin_amdgcn_ballot_w64(!tame) == 0) {
-        // relative to c, which is m log2(e) but for its rounding: that much is put right for the sums
-        const float c = a.m * LOG2E, off = -fmaf(a.m, LOG2E, -c), off_ln = off * LN2;
-        float s = 0.0f, t = 0.0f;
+    // relative to c, which is m log2(e) but for its rounding: that much is put right for the sums
+    const float c = a.m * LOG2E, off = -fmaf(a.m, LOG2E, -c), off_ln = off * LN2;
+    float s = 0.0f, t = 0.0f;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float y = fmaf(x[i], LOG2E, -c), e = fast_exp2(y);
-            s += e;
-            if constexpr (ENTROPY) t = fmaf(y, e, t);
-        }
-        if constexpr (ENTROPY) a.t += t + fmaf(off, s, off_ln * t);
-        a.s += fmaf(s, off_ln, s);
-    } else {
+    for (int i = 0; i < N; ++i) {
+        const float y = fmaf(x[i], LOG2E, -c), e = fast_exp2(y);
+        s += e;
+        if constexpr (ENTROPY) t = fmaf(y, e, t);
+    }
+    if constexpr (ENTROPY) t += fmaf(off, s, off_ln * t);
+    s = fmaf(s, off_ln, s);
+    const bool exact = fabsf(a.m) < TAME && (!ENTROPY || t == t);
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(!exact) != 0, 0) && !exact) {
+        s = t = 0.0f;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float y = (x[i] - a.m) * LOG2E, e = fast_exp2(y);
-            a.s += e;
-            if constexpr (ENTROPY) a.t = fmaf(fmaxf(y, -0x1p20f), e, a.t);
+            s += e;
+            if constexpr (ENTROPY) t = fmaf(fmaxf(y, -0x1p20f), e, t);
         }
     }
+    a.s += s;
+    if constexpr (ENTROPY) a.t += t;
+    return most;
 }
 
 // Elements in the order of the alternatives: larger first, equal ones by place; -0 is 0, and NaN the least.
+__device__ __forceinline__ uint32_t order_of(float x) {           // of a number
+    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
 __device__ __forceinline__ uint64_t rank_of(float x, uint32_t place) {
-    x = x == x ? x + 0.0f : -__builtin_inff();
-    const uint32_t b = __builtin_bit_cast(uint32_t, x);
-    return (uint64_t)(b >> 31 ? ~b : b | 0x80000000u) << 32 | (uint32_t)~place;
+    return (uint64_t)order_of(x == x ? x : -__builtin_inff()) << 32 | (uint32_t)~place;
 }
 __device__ __forceinline__ float value_of(uint64_t rank) {
     const uint32_t b = (uint32_t)(rank >> 32);
@@ -140,12 +149,24 @@ __device__ __forceinline__ float value_of(uint64_t rank) {
 }
 __device__ __forceinline__ uint32_t place_of(uint64_t rank) { return ~(uint32_t)rank; }
 
+// A wave's, or a workgroup's, sums over its threads: the largest m first, then what the others come to beside it.
+__device__ __forceinline__ Sum over_wave(Sum a) {
+    const float m = row_ops::over_lanes<64>(a.m, row_ops::Max{});
+    const float d = fmaxf((a.m - m) * LOG2E, -0x1p20f), e = fast_exp2(d);
+    return {m, row_ops::over_lanes<64>(a.s * e, row_ops::Add{}), row_ops::over_lanes<64>((a.t + d * a.s) * e, row_ops::Add{})};
+}
+
 // What may still be among the alternatives.
 struct Candidates {
-    uint64_t list[KEPT + THREADS * 8];            // what stays, and what the threads add in a turn
+    union {
+        uint64_t list[LIST];
+        uint16_t block[SLOTS][THREADS];       // of the largest of a thread's block, the upper half of its place in their order
+    };
     uint64_t chosen[MAX_TOP];
     uint64_t best[WAVES];
-    int count;
+    int count, blocks;
+    float limit;
+    uint16_t which[MOST_BLOCKS];              // the blocks that reach the limit: thread, and slot times THREADS
 };
 __device__ __forceinline__ uint64_t largest(uint64_t v) {
 #pragma unroll
@@ -155,19 +176,69 @@ __device__ __forceinline__ uint64_t largest(uint64_t v) {
     }
     return v;
 }
+// The top-th largest of a wave's N x 64 keys, or what it has of the bits from `least_bit` on, or a number between that and the next smaller
+// key; 0 where there are fewer.
+template <int N>
+__device__ __forceinline__ uint32_t top_key(const uint32_t (&key)[N], int top, uint32_t least_bit) {
+    uint32_t found = 0;
+    for (uint32_t bit = 0x80000000u; bit >= least_bit && bit; bit >>= 1) {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[k] >= (found | bit)));
+        if (n >= top) found |= bit;
+        if (n == top) break;
+    }
+    return found;
+}
 // c.chosen = the `top` largest of the first `count` of the list, in order, 0 behind the last; all threads call it.  A few by counting how many
-// are larger than each, many by one search for each of the chosen.
+// are larger than each, which one wave does in registers up to 64 of them; where there are more, those are out first whose value alone is too
+// small.  Many, which are ties, by one search for each of the chosen.
 __device__ __forceinline__ void choose(Candidates& c, int count, int top) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (count <= KEPT) {
-        for (int i = threadIdx.x; i < top; i += THREADS)
-            if (i >= count) c.chosen[i] = 0;
-        for (int i = threadIdx.x; i < count; i += THREADS) {
-            const uint64_t mine = c.list[i];
+        if (wave == 0) {                                          // the others leave it their share of the vector unit
+            uint64_t* list = c.list;
+            if (count > 64) {
+                list += KEPT;
+                uint32_t key[KEPT / 64], few[2];
+#pragma unroll
+                for (int k = 0; k < KEPT / 64; ++k) key[k] = lane + 64 * k < count ? (uint32_t)(c.list[lane + 64 * k] >> 32) : 0;
+                few[0] = key[0], few[1] = key[1];
+                const uint32_t least = count <= 128 ? top_key(few, top, 1) : top_key(key, top, 1);
+                int above = 0, ties = 0;
+#pragma unroll
+                for (int k = 0; k < KEPT / 64; ++k) {
+                    above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[k] > least));
+                    ties += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[k] == least));
+                }
+                uint32_t place[KEPT / 64], first = 0;                 // of the ties the first that there is room for
+                if (above + ties > 64) {
+#pragma unroll
+                    for (int k = 0; k < KEPT / 64; ++k) place[k] = key[k] == least && least != 0 ? (uint32_t)c.list[lane + 64 * k] : 0;
+                    first = top_key(place, top - above, 1);
+                }
+                int n = 0;
+#pragma unroll
+                for (int k = 0; k < KEPT / 64; ++k) {
+                    const bool stays = key[k] != 0 && (key[k] > least || (key[k] == least && (first == 0 || place[k] >= first)));
+                    const uint64_t all = __builtin_amdgcn_ballot_w64(stays);
+                    if (stays) list[n + __builtin_popcountll(all & (((uint64_t)1 << lane) - 1))] = c.list[lane + 64 * k];
+                    n += __builtin_popcountll(all);
+                }
+                count = __builtin_amdgcn_readfirstlane(n);            // at most 64: `top` of them where there were ties
+                __builtin_amdgcn_wave_barrier();
+            }
+            if (lane < top && lane >= count) c.chosen[lane] = 0;
+            count = __builtin_amdgcn_readfirstlane(count);
+            const uint64_t mine = lane < count ? list[lane] : 0;
             int front = 0;
-#pragma unroll 8
-            for (int j = 0; j < count; ++j) front += c.list[j] > mine;
-            if (front < top) c.chosen[front] = mine;
+#pragma unroll 4
+            for (int j = 0; j < count; ++j) {
+                const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32 |
+                                       (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
+                front += other > mine;
+            }
+            if (lane < count && front < top) c.chosen[front] = mine;
         }
     } else {
         uint64_t limit = ~(uint64_t)0;
@@ -235,6 +306,18 @@ __global__ __launch_bounds__(lp::THREADS) void token_logprobs_kernel(const T* __
     Sum a{LEAST, 0.0f, 0.0f};
     const int alone = st.single(threadIdx.x);
     const float single[1] = {alone >= 0 ? Elem<T>::one(x[alone]) : -__builtin_inff()};
+    __shared__ typename std::conditional<TOP, float[THREADS], float[1]>::type most;
+    __shared__ typename std::conditional<TOP, Candidates, char>::type c;
+    int blocks = 0;
+    // the maximum of the next block; a thread reads no other's
+    auto keep = [&](float m) {
+        if constexpr (TOP) {
+            uint16_t* at = &c.block[blocks % SLOTS][threadIdx.x];
+            const uint16_t now = (uint16_t)(order_of(m) >> 16);
+            *at = blocks < SLOTS ? now : max(now, *at);
+            ++blocks;
+        }
+    };
     int p = threadIdx.x;
     for (; p + (AT_ONCE - 1) * THREADS < st.pieces; p += AT_ONCE * THREADS) {
         u32x4 v[AT_ONCE];
@@ -248,18 +331,25 @@ __global__ __launch_bounds__(lp::THREADS) void token_logprobs_kernel(const T* __
 #pragma unroll
             for (int i = 0; i < E; ++i) f[u * E + i] = g[i];
         }
-        add<ENTROPY>(a, f);
+        keep(add<ENTROPY>(a, f));
     }
-    for (; p < st.pieces; p += THREADS) {
-        float f[E];
-        Elem<T>::unpack(ld_stream_16<CACHED>(st.piece(p)), f);
-        add<ENTROPY>(a, f);
+    if (p < st.pieces) {
+        float m = LEAST;
+        for (; p < st.pieces; p += THREADS) {
+            float f[E];
+            Elem<T>::unpack(ld_stream_16<CACHED>(st.piece(p)), f);
+            m = fmaxf(m, add<ENTROPY>(a, f));
+        }
+        keep(m);
     }
     if (alone >= 0) add<ENTROPY>(a, single);
     const float mine = a.m;                                       // the largest of this thread's elements
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) a = join(a, Sum{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64)});
+    a = over_wave(a);
     if (lane == 0) sums[wave] = a;
+    if constexpr (TOP) {
+        most[threadIdx.x] = mine;
+        if (threadIdx.x == 0) c.count = c.blocks = 0;
+    }
     __syncthreads();
     a = sums[0];
 #pragma unroll
@@ -270,62 +360,95 @@ __global__ __launch_bounds__(lp::THREADS) void token_logprobs_kernel(const T* __
         else write_row<T, ENTROPY>(out, row, x, target_of(targets, targets64, row), vocab, a, ls);
     }
     if constexpr (TOP) {
-        __shared__ Candidates c;
-        __shared__ float most[THREADS];
-        __shared__ uint8_t who[THREADS];
-        __shared__ int whos;
-        most[threadIdx.x] = mine;
-        if (threadIdx.x == 0) c.count = whos = 0;
-        __syncthreads();
-        // the top-th largest of the threads' largest (or a little less): bit by bit in the order of whole numbers, every wave by itself
-        uint32_t key[WAVES], found = 0;
+        // No element below the top-th largest of the threads' largest is an alternative; nor below that of four threads' together, which is one
+        // key a lane and for small `top` hardly less.  One wave looks for it, by the upper 16 bits of the keys.
+        if (wave == 0) {
+            uint32_t key[WAVES], four[1] = {0};
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) key[w] = (uint32_t)(rank_of(most[w * 64 + lane], 0) >> 32);
-        for (uint32_t bit = 0x80000000u; bit >= (sizeof(T) == 4 ? 1u : 0x10000u); bit >>= 1) {
-            int n = 0;
-#pragma unroll
-            for (int w = 0; w < WAVES; ++w) n += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[w] >= (found | bit)));
-            if (n >= top) found |= bit;
-            if (bit == 1) break;
+            for (int w = 0; w < WAVES; ++w) {
+                key[w] = order_of(most[w * 64 + lane]);
+                four[0] = max(four[0], key[w]);
+            }
+            const float found = value_of((uint64_t)(top <= 24 ? top_key(four, top, 0x10000u) : top_key(key, top, 0x10000u)) << 32);
+            // none where fewer than `top` threads have elements that are numbers
+            if (lane == 0) c.limit = found > LEAST ? found : -__builtin_inff();
         }
-        const float limit = value_of((uint64_t)found << 32);
-        // no limit where fewer than `top` threads have elements that are numbers
-        const bool all = !(limit > LEAST);
-        if (all || mine >= limit) who[atomicAdd(&whos, 1)] = (uint8_t)threadIdx.x;
         __syncthreads();
-        // their elements, a piece a thread in a turn, and the single ones in a last turn
-        const int threads = whos, items = threads * ((st.pieces + THREADS - 1) / THREADS), turns = (items + THREADS - 1) / THREADS;
-        uint64_t least = 0;                                       // only what is larger can still be among the alternatives
-        for (int turn = 0; turn <= turns; ++turn) {
-            if (turn < turns) {
-                const int item = turn * THREADS + threadIdx.x, piece = item < items ? who[item % threads] + item / threads * THREADS : st.pieces;
-                if (piece < st.pieces) {
-                    float f[E];
-                    Elem<T>::unpack(ld_global_16(st.piece(piece)), f);
-#pragma unroll
-                    for (int i = 0; i < E; ++i)
-                        if (all || f[i] >= limit) {
-                            const uint64_t r = rank_of(f[i], st.place(piece) + i);
-                            if (r > least) c.list[atomicAdd(&c.count, 1)] = r;
-                        }
+        const float limit = c.limit;
+        const bool all = limit == -__builtin_inff();
+        if (all || mine >= limit) {
+            const uint32_t least = all ? 0 : order_of(limit) >> 16;
+            for (int k = 0; k < min(blocks, SLOTS); ++k)
+                if (c.block[k][threadIdx.x] >= least) {
+                    const int at = atomicAdd(&c.blocks, 1);
+                    if (at < MOST_BLOCKS) c.which[at] = (uint16_t)(k * THREADS + threadIdx.x);
                 }
-            } else if (alone >= 0 && (all || single[0] >= limit)) {
-                const uint64_t r = rank_of(single[0], alone);
-                if (r > least) c.list[atomicAdd(&c.count, 1)] = r;
+        }
+        __syncthreads();
+        // elements of a piece go to the list, those that reach the limit and are above `least`
+        auto offer = [&](int piece, uint64_t least) {
+            if (piece >= st.pieces) return;
+            float f[E];
+            Elem<T>::unpack(ld_global_16(st.piece(piece)), f);
+            const int place = st.place(piece);
+            uint32_t mine = 0;                                    // a bit for each
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if ((all || f[i] >= limit) && (least == 0 || rank_of(f[i], place + i) > least)) mine |= 1u << i;
+            if (!mine) return;
+            int at = atomicAdd(&c.count, __builtin_popcount(mine));
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (mine >> i & 1) {
+                    if (at < LIST) c.list[at] = rank_of(f[i], place + i);
+                    ++at;
+                }
+        };
+        auto offer_single = [&](uint64_t least) {
+            if (alone < 0 || !(all || single[0] >= limit) || rank_of(single[0], alone) <= least) return;
+            const int at = atomicAdd(&c.count, 1);
+            if (at < LIST) c.list[at] = rank_of(single[0], alone);
+        };
+        // the blocks that reach the limit, a piece a thread
+        const int found = c.blocks;
+        if (found <= MOST_BLOCKS) {
+            for (int i = threadIdx.x; i < found * AT_ONCE; i += THREADS) {
+                const int which = c.which[i / AT_ONCE];
+                for (int p = which % THREADS + (which / THREADS * AT_ONCE + i % AT_ONCE) * THREADS; p < st.pieces; p += SLOTS * AT_ONCE * THREADS) offer(p, 0);
             }
+            offer_single(0);
+        }
+        __syncthreads();
+        int count = c.count;
+        if (count > LIST || found > MOST_BLOCKS) {
+            // Many are as large: all elements once more, TURN threads' pieces in a turn, and whenever there are many the first of them go on.
             __syncthreads();
-            const int count = c.count;
+            if (threadIdx.x == 0) c.count = 0;
             __syncthreads();
-            if (turn == turns || count > KEPT) choose(c, count, top);
-            if (turn < turns && count > KEPT) {                   // many are as large: the first of them go on
-                least = c.chosen[top - 1];
-                if (threadIdx.x < top) c.list[threadIdx.x] = c.chosen[threadIdx.x];
-                if (threadIdx.x == 0) c.count = top;
+            const int turns = (st.pieces + TURN - 1) / TURN;
+            uint64_t least = 0;
+            for (int turn = 0; turn <= turns; ++turn) {
+                if (turn < turns) {
+                    if (threadIdx.x < TURN) offer(turn * TURN + threadIdx.x, least);
+                } else {
+                    offer_single(least);
+                }
                 __syncthreads();
+                count = c.count;
+                __syncthreads();
+                if (turn < turns && count > KEPT) {
+                    choose(c, count, top);
+                    least = c.chosen[top - 1];
+                    if (threadIdx.x < top) c.list[threadIdx.x] = c.chosen[threadIdx.x];
+                    if (threadIdx.x == 0) c.count = top;
+                    __syncthreads();
+                }
             }
         }
+        choose(c, count, top);
         if (cut > 1) {
-            if (threadIdx.x < top) part_tops[(size_t)blockIdx.x * top + threadIdx.x] = c.chosen[threadIdx.x];
+            // the first of all parts, then the second, ...
+            if (threadIdx.x < top) part_tops[(row * top + threadIdx.x) * cut + part] = c.chosen[threadIdx.x];
         } else {
             write_top(out, row, c, top, a, ls);
         }
@@ -346,23 +469,38 @@ __global__ __launch_bounds__(lp::THREADS) void token_logprobs_join_kernel(const 
         const Part q = parts[row * cut + i];
         a = join(a, Sum{q.m, q.s, q.t});
     }
+    uint32_t limit = 0;
+    if constexpr (TOP) {
+        // no alternative is below the top-th largest of each part's first few
+        const int first = min(top, JOINED / cut);
+        uint32_t key[JOINED / 64];
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) a = join(a, Sum{__shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64)});
+        for (int k = 0; k < JOINED / 64; ++k) {
+            const int i = lane + 64 * k;
+            key[k] = i < cut * first ? (uint32_t)(part_tops[row * cut * top + i] >> 32) : 0;
+        }
+        limit = top_key(key, top, 1);
+    }
+    a = over_wave(a);
     const float ls = logf(a.s);
     if (threadIdx.x == 0) write_row<T, ENTROPY>(out, row, x, target_of(targets, targets64, row), vocab, a, ls);
     if constexpr (TOP) {
         __shared__ Candidates c;
-        const int count = cut * top;                              // at most the list's length
-        for (int i = threadIdx.x; i < count; i += THREADS) c.list[i] = part_tops[row * count + i];
+        if (threadIdx.x == 0) c.count = 0;
         __syncthreads();
-        choose(c, count, top);
+        for (int i = threadIdx.x; i < cut * top; i += THREADS) {  // at most as many as the list holds
+            const uint64_t r = part_tops[row * cut * top + i];
+            if (r != 0 && (uint32_t)(r >> 32) >= limit) c.list[atomicAdd(&c.count, 1)] = r;
+        }
+        __syncthreads();
+        choose(c, c.count, top);
         write_top(out, row, c, top, a, ls);
     }
 }
 
 // The gradient: workgroup (row, part of it).  logits and d_logits may be the same memory: a thread writes where it alone has read.
 template <class T, bool CACHED, bool ENTROPY>
-__global__ __launch_bounds__(lp::THREADS) void token_logprobs_bwd_kernel(const T* logits, const void* __restrict__ targets, int targets64,
+__global__ __launch_bounds__(lp::BWD_THREADS) void token_logprobs_bwd_kernel(const T* logits, const void* __restrict__ targets, int targets64,
                                                                          const float* __restrict__ lse, const float* __restrict__ entropy,
                                                                          const float* __restrict__ d_logp, const float* __restrict__ d_entropy,
                                                                          const float* __restrict__ d_lse, T* d_logits, int vocab, size_t width,
@@ -404,19 +542,19 @@ __global__ __launch_bounds__(lp::THREADS) void token_logprobs_bwd_kernel(const T
     auto put = [&](int i) { Elem<T>::put(dx + i, zero ? 0.0f : with_target(slope(Elem<T>::one(x[i])), i == target)); };
     // pieces of 16 bytes where both tensors have them at the same elements
     if ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(d_logits)) % 16 != 0) {
-        for (int i = begin + threadIdx.x; i < end; i += THREADS) put(i);
+        for (int i = begin + threadIdx.x; i < end; i += BWD_THREADS) put(i);
     } else {
         const int alone = st.single(threadIdx.x);
         if (alone >= 0) put(alone);
-        for (int p0 = threadIdx.x; p0 < st.pieces; p0 += AT_ONCE * THREADS) {
-            u32x4 v[AT_ONCE];
+        for (int p0 = threadIdx.x; p0 < st.pieces; p0 += BWD_AT_ONCE * BWD_THREADS) {
+            u32x4 v[BWD_AT_ONCE];
             if (!zero) {
 #pragma unroll
-                for (int u = 0; u < AT_ONCE; ++u) v[u] = ld_stream_16<CACHED>(st.piece(min(p0 + u * THREADS, st.pieces - 1)));
+                for (int u = 0; u < BWD_AT_ONCE; ++u) v[u] = ld_stream_16<CACHED>(st.piece(min(p0 + u * BWD_THREADS, st.pieces - 1)));
             }
 #pragma unroll
-            for (int u = 0; u < AT_ONCE; ++u) {
-                const int p = p0 + u * THREADS;
+            for (int u = 0; u < BWD_AT_ONCE; ++u) {
+                const int p = p0 + u * BWD_THREADS;
                 if (p >= st.pieces) break;
                 float f[E];
                 if (zero) {
@@ -437,7 +575,7 @@ __global__ __launch_bounds__(lp::THREADS) void token_logprobs_bwd_kernel(const T
         }
     }
     if (part == cut - 1)
-        for (size_t i = vocab + threadIdx.x; i < width; i += THREADS) Elem<T>::put(dx + i, 0.0f);
+        for (size_t i = vocab + threadIdx.x; i < width; i += BWD_THREADS) Elem<T>::put(dx + i, 0.0f);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -447,15 +585,15 @@ using namespace lp;
 // the list that joins them.
 struct Cut { int parts, each; };
 Cut cut_of(size_t rows, int vocab, int elem_bytes, int top) {
-    size_t n = 1024 / rows;
+    size_t n = std::min((size_t)1024 / rows, (size_t)JOINED / 2);
     n = std::min(n, (size_t)vocab * elem_bytes / 8192);
-    if (top) n = std::min(n, (size_t)2048 / top);
+    if (top) n = std::min(n, (size_t)LIST / top);
     n = std::max(n, (size_t)1);
     const int each = (int)(((vocab + n - 1) / n + 127) / 128 * 128);
     return {(vocab + each - 1) / each, each};
 }
 // of the gradient: a workgroup's threads go round once
-int bwd_each(int elem_bytes) { return THREADS * AT_ONCE * 16 / elem_bytes; }
+int bwd_each(int elem_bytes) { return BWD_THREADS * BWD_AT_ONCE * 16 / elem_bytes; }
 }  // namespace
 
 bool token_logprobs_fits(size_t rows, int vocab, int bf16) {
@@ -496,11 +634,12 @@ int launch_token_logprobs(const void* logits, const void* targets, int targets64
 int launch_token_logprobs_bwd(const void* logits, const void* targets, int targets64, const float* lse, const float* entropy, const float* d_logp,
                               const float* d_entropy, const float* d_lse, void* d_logits, size_t rows, int vocab, size_t width, int bf16,
                               hipStream_t stream) {
-    const int each = bwd_each(bf16 ? 2 : 4), cut = (vocab + each - 1) / each;
+    const int most = bwd_each(bf16 ? 2 : 4), cut = (vocab + most - 1) / most;
+    const int each = ((vocab + cut - 1) / cut + 63) / 64 * 64;       // of equal parts, at most `most`
     const bool cached = rows * vocab * (bf16 ? 4 : 8) <= kStreamCached;
     auto go = [&](auto elem, auto in_cache, auto with_entropy) {
         using T = decltype(elem);
-        launch_kernel((token_logprobs_bwd_kernel<T, in_cache(), with_entropy()>), dim3((unsigned)(rows * cut)), dim3(THREADS), 0, stream,
+        launch_kernel((token_logprobs_bwd_kernel<T, in_cache(), with_entropy()>), dim3((unsigned)(rows * cut)), dim3(BWD_THREADS), 0, stream,
                       static_cast<const T*>(logits), targets, targets64, lse, entropy, d_logp, d_entropy, d_lse, static_cast<T*>(d_logits), vocab, width, cut,
                       each);
     };
