@@ -532,8 +532,9 @@ int tyr_hip_embedding_bwd(const void* d_out, const void* ids, int ids_dtype, voi
     if (!is_index(ids_dtype)) return TYR_HIP_ERR_UNSUPPORTED;
     if (!aligned_index(ids, ids_dtype) || !aligned16(d_out) || !aligned16(d_table)) return TYR_HIP_ERR_MISALIGNED;
     const int bf16 = dtype == TYR_HIP_BF16;
-    if (!workspace || workspace_bytes < tyr::embedding_bwd_workspace_bytes((size_t)n, (size_t)vocab, (int)d_model, bf16)) return TYR_HIP_ERR_WORKSPACE;
-    if (!aligned16(workspace)) return TYR_HIP_ERR_MISALIGNED;
+    const size_t need = tyr::embedding_bwd_workspace_bytes((size_t)n, (size_t)vocab, (int)d_model, bf16);
+    if (need && (!workspace || workspace_bytes < need)) return TYR_HIP_ERR_WORKSPACE;
+    if (need && !aligned16(workspace)) return TYR_HIP_ERR_MISALIGNED;
     rc = tyr::launch_embedding_bwd(d_out, ids, ids_dtype == TYR_HIP_I64, d_table, (size_t)n, (size_t)vocab, (int)d_model, scale, accumulate, bf16,
                                    workspace, static_cast<hipStream_t>(stream));
     return rc == 0 ? TYR_HIP_OK : TYR_HIP_ERR_LAUNCH;

@@ -601,18 +601,18 @@ PyObject* embedding_bwd(PyObject* const* a) {
     const at::Tensor* into = optional(a[4], "into", g.scalar_type(), 2);
     if (into && (into->size(0) != vocab || into->size(1) != d)) fail("into must be [vocab, d_model]");
     not_empty({&ids, &g}, "embeddingBwd");
+    if (vocab == 0 || vocab > INT32_MAX) check_status(TYR_HIP_ERR_BAD_SHAPE, "embeddingBwd");      // nothing is allocated for it
     const OnDevice on(g, {&ids, into}, truth(a[5]));
     at::Tensor table;
     int rc;
     {
         NoGil nogil;
         const size_t bytes = api.tyr_hip_embedding_bwd_workspace_bytes(ids.numel(), vocab, d, dtype);
-        // a shape that the call refuses is not allocated for
-        if (into) table = *into;
-        else if (bytes) table = empty({vocab, d}, g.scalar_type(), g);
-        const at::Tensor ws = scratch(bytes, g);
-        rc = api.tyr_hip_embedding_bwd(g.data_ptr(), ids.data_ptr(), index, bytes ? table.data_ptr() : ws.data_ptr(), ids.numel(), vocab, d, scale,
-                                       into != nullptr, dtype, ws.data_ptr(), ws.numel(), stream());
+        table = into ? *into : empty({vocab, d}, g.scalar_type(), g);
+        at::Tensor ws;
+        if (bytes) ws = scratch(bytes, g);
+        rc = api.tyr_hip_embedding_bwd(g.data_ptr(), ids.data_ptr(), index, table.data_ptr(), ids.numel(), vocab, d, scale, into != nullptr, dtype,
+                                       bytes ? ws.data_ptr() : nullptr, bytes, stream());
     }
     check_status(rc, "embeddingBwd");
     return wrap(std::move(table));
