@@ -474,7 +474,7 @@ int tyr_hip_embedding(const void* ids, int ids_dtype, const void* table, void* o
  *   workspace : tyr_hip_embedding_bwd_workspace_bytes(...) bytes (0 also for shapes that the call refuses), 16-byte aligned, contents
  *               arbitrary; calls that overlap in time need one each (may be NULL where that is 0)
  * Supported: as the lookup, and n <= 2^30; with pieces of 32 tokens and blocks of 64 16-byte pieces of a row,
- * pieces * blocks < 2^26, pieces / 16 * d_model / 256 < 2^22, and the table is smaller than 512 GiB. */
+ * pieces * blocks + vocab < 2^26 and pieces / 16 * d_model / 256 < 2^22. */
 size_t tyr_hip_embedding_bwd_workspace_bytes(uint64_t n, uint64_t vocab, uint64_t d_model, int dtype);
 int tyr_hip_embedding_bwd(const void* d_out, const void* ids, int ids_dtype, void* d_table, uint64_t n, uint64_t vocab, uint64_t d_model,
                           float scale, int accumulate, int dtype, void* workspace, size_t workspace_bytes, void* stream);

@@ -7,8 +7,8 @@
 //   few tokens       one launch: a workgroup has the tokens of its residue class, finds them among all, adds their rows, and clears the others
 //   up to 2^15       such classes put their pairs (token, place) together, equal tokens side by side; then the sums
 //   more             a radix sort of the pairs, then the sums
-// The table is cleared beside the sort, whose launches leave the memory idle: rows that are summed are written twice, which costs less than to wait
-// for the sort to tell which rows are not.
+// The sort notes which tokens are there, and beside the sums the rows of the others are cleared.  The sort's own launches leave the memory idle:
+// beside them the end of the table is cleared as a whole, where tokens are rare if they are numbered by how frequent they are.
 // The sums: a wave adds the rows of PIECE consecutive pairs, 16 bytes of a row a lane, in f32.  A run of equal tokens no longer than that belongs to
 // the wave of the piece that it begins in; a longer one leaves an f32 row for each piece that it reaches into, and a last launch adds those.
 //
@@ -58,6 +58,7 @@ constexpr int MAX_QUOTIENTS = 1024;       // quotients by CLASSES at most, for b
 constexpr int CHUNK = 1024, CHUNKS = 128; // radix sort: tokens of a turn, workgroups at most
 constexpr int MAX_DIGIT = 9;
 constexpr int CLEARED = 16;               // 16-byte pieces that a thread of 1024 fills with zeros
+constexpr size_t BESIDE = (size_t)48 << 20, BESIDE_PASS = (size_t)20 << 20;      // bytes of the table cleared beside the classes, a launch of the radix sort
 constexpr int HELD = 256;                 // pairs that a wave keeps of its share
 }  // namespace emb
 
@@ -91,13 +92,18 @@ template <class T>
 __device__ __forceinline__ void clear_row(T* row, int row_pieces) {
     for (int p = threadIdx.x & 63; p < row_pieces; p += 64) st_global_16_nt(row + p * emb::Row<T>::E, u32x4{0, 0, 0, 0});
 }
-// Zeros by workgroup w of 1024 threads.
-__device__ __forceinline__ void clear_share(void* table, size_t pieces, uint32_t w) {
-    const size_t first = (size_t)w * (1024 * emb::CLEARED) + threadIdx.x;
+// Zeros: `pieces` of 16 bytes, their share of workgroup w of 1024 threads.
+struct Zeros {
+    void* at;
+    size_t pieces;
+    __device__ __forceinline__ void fill(uint32_t w) const {
+        const size_t first = (size_t)w * (1024 * emb::CLEARED) + threadIdx.x;
 #pragma unroll
-    for (int k = 0; k < emb::CLEARED; ++k)
-        if (first + k * 1024 < pieces) st_global_16_nt(static_cast<char*>(table) + (first + k * 1024) * 16, u32x4{0, 0, 0, 0});
-}
+        for (int k = 0; k < emb::CLEARED; ++k)
+            if (first + k * 1024 < pieces) st_global_16_nt(static_cast<char*>(at) + (first + k * 1024) * 16, u32x4{0, 0, 0, 0});
+    }
+    __host__ uint32_t workgroups() const { return (uint32_t)((pieces + 1024 * emb::CLEARED - 1) / (1024 * emb::CLEARED)); }
+};
 // f32 sums to a row of the table, or to what is there
 template <class T>
 __device__ __forceinline__ void finish(T* to, float (&sum)[emb::Row<T>::E], float scale, bool into) {
@@ -161,15 +167,16 @@ __device__ __forceinline__ void add_scan(uint32_t* place, const uint32_t* total,
 
 // Classes: workgroup c has the tokens that are c modulo CLASSES.  It counts over all ids how many pairs stand in front of its own, those of
 // smaller classes, and how many each wave finds of each quotient in its share of the ids; so every wave knows where its pairs go and puts them
-// there without another's help.  Workgroups behind the classes clear the table.  LDS: count [16][digits], total and front [digits].
+// there without another's help.  there[token] = whether it is.  Workgroups behind the classes clear the end of the table.  LDS:
+// count [16][digits], total and front [digits].
 template <class I>
-__global__ __launch_bounds__(1024, 8) void embedding_gather_kernel(const I* __restrict__ ids, u32x2* __restrict__ pairs, void* __restrict__ table, int n,
-                                                                uint32_t vocab, size_t table_pieces, int bits) {
+__global__ __launch_bounds__(1024, 8) void embedding_gather_kernel(const I* __restrict__ ids, u32x2* __restrict__ pairs, uint8_t* __restrict__ there, int n,
+                                                                   uint32_t vocab, int bits, Zeros zeros) {
     using namespace emb;
     __shared__ u32x2 held[16][HELD];
     __shared__ int mine_of[16], front_of[16];
     extern __shared__ __attribute__((aligned(16))) uint32_t total[];
-    if (blockIdx.x >= CLASSES) return clear_share(table, table_pieces, blockIdx.x - CLASSES);
+    if (blockIdx.x >= CLASSES) return zeros.fill(blockIdx.x - CLASSES);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), digits = 1 << bits;
     uint32_t* const place = total + digits;
     uint32_t* const counts = place + digits;                        // of wave w, two quotients a word
@@ -229,6 +236,7 @@ __global__ __launch_bounds__(1024, 8) void embedding_gather_kernel(const I* __re
             sum += k;
         }
         total[d] = sum;
+        if (d * CLASSES + c < vocab) there[d * CLASSES + c] = sum != 0;
     }
     // places of no pair, behind the last
     if (c == CLASSES - 1)
@@ -377,7 +385,7 @@ __global__ __launch_bounds__(1024) void embedding_few_kernel(const I* __restrict
 }
 
 // More: a radix sort from the low digit up, two launches a digit.  Workgroup w has the tokens [w each, (w + 1) each); those behind
-// clear the table from share `cleared` on.
+// clear memory.  The last launch notes which tokens are there.
 template <class I, bool FIRST>
 struct SortInput {
     const I* ids;
@@ -390,9 +398,12 @@ struct SortInput {
 };
 template <class I, bool FIRST>
 __global__ __launch_bounds__(1024) void embedding_count_kernel(SortInput<I, FIRST> in, uint32_t* __restrict__ hist, int n, int each, int workgroups, int at,
-                                                               int bits, void* __restrict__ table, size_t table_pieces, uint32_t cleared) {
+                                                               int bits, Zeros zeros, Zeros none, uint32_t none_workgroups) {
     __shared__ uint32_t count[1 << emb::MAX_DIGIT];
-    if ((int)blockIdx.x >= workgroups) return clear_share(table, table_pieces, cleared + blockIdx.x - workgroups);
+    if ((int)blockIdx.x >= workgroups) {
+        const uint32_t w = blockIdx.x - workgroups;
+        return w < none_workgroups ? none.fill(w) : zeros.fill(w - none_workgroups);
+    }
     const int digits = 1 << bits, first = blockIdx.x * each, end = min(n, first + each);
     for (int d = threadIdx.x; d < digits; d += 1024) count[d] = 0;
     __syncthreads();
@@ -402,12 +413,12 @@ __global__ __launch_bounds__(1024) void embedding_count_kernel(SortInput<I, FIRS
 }
 template <class I, bool FIRST>
 __global__ __launch_bounds__(1024) void embedding_scatter_kernel(SortInput<I, FIRST> in, const uint32_t* __restrict__ hist, u32x2* __restrict__ out,
-                                                                 int n, int each, int workgroups, int at, int bits, void* __restrict__ table,
-                                                                 size_t table_pieces, uint32_t cleared) {
+                                                                 uint8_t* __restrict__ there, int n, uint32_t vocab, int each, int workgroups, int at,
+                                                                 int bits, Zeros zeros) {
     constexpr int MOST = 1 << emb::MAX_DIGIT;
     __shared__ uint32_t place[MOST], total[MOST];
     __shared__ uint16_t count[16][MOST];
-    if ((int)blockIdx.x >= workgroups) return clear_share(table, table_pieces, cleared + blockIdx.x - workgroups);
+    if ((int)blockIdx.x >= workgroups) return zeros.fill(blockIdx.x - workgroups);
     const int digits = 1 << bits, first = blockIdx.x * each, end = min(n, first + each);
     for (int d = threadIdx.x; d < 16 * digits; d += 1024) count[d >> bits][d & (digits - 1)] = 0;
     // where this workgroup's tokens of a digit go: behind all smaller digits and the same one of the workgroups in front
@@ -432,7 +443,10 @@ __global__ __launch_bounds__(1024) void embedding_scatter_kernel(SortInput<I, FI
         const int i = start + threadIdx.x;
         const u32x2 pair = i < end ? in(i) : u32x2{0, 0};
         const uint32_t to = take_places(place, count, pair.x >> at & (digits - 1), i < end, bits);
-        if (i < end) out[to] = pair;
+        if (i < end) {
+            out[to] = pair;
+            if (there && pair.x < vocab) there[pair.x] = 1;
+        }
     }
 }
 
@@ -478,16 +492,21 @@ struct Window {
 };
 
 // One wave: 64 lanes of 16 bytes of the rows of PIECE consecutive pairs, and of those of a last run that goes on behind them, if it is no longer
-// than PIECE; a run in front that is the wave's before, it leaves out.
+// than PIECE; a run in front that is the wave's before, it leaves out.  Waves behind those of the pieces have a row of the
+// table each, of the first `zero_rows`, and clear it where it has no token.
 template <class T, int PIECE, bool CACHED>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(const u32x2* __restrict__ pairs, const T* __restrict__ d_out, T* __restrict__ table,
                                                             float* __restrict__ part, int n, uint32_t vocab, int row_pieces, int blocks,
-                                                            int tasks, float scale, bool into) {
+                                                            int tasks, const uint8_t* __restrict__ there, int zero_rows, float scale, bool into) {
     using R = emb::Row<T>;
     constexpr int E = R::E;
     const int lane = threadIdx.x & 63, task = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     const size_t d = (size_t)row_pieces * E;
-    if (task >= tasks) return;
+    if (task >= tasks) {
+        const int row = task - tasks;
+        if (row < zero_rows && there[row] == 0) clear_row(table + row * d, row_pieces);
+        return;
+    }
     const int piece = task / blocks, p = (task % blocks) * 64 + lane;
     const int first = piece * PIECE, end = min(n, first + PIECE);
     const Window<PIECE> w(pairs, n, first);
@@ -524,7 +543,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const u32x2* __restr
             finish(table + (size_t)key * d + col, sum, scale, into);
         }
     };
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = 16;
     u32x4 row[AHEAD];
     for (; t < last; t += AHEAD) {
 #pragma unroll
@@ -583,9 +602,9 @@ __global__ __launch_bounds__(1024) void embedding_join_kernel(const u32x2* __res
     if (mine < pieces - 1) {
         const int first = mine * PIECE, end = first + PIECE;
         const Window<PIECE> w(pairs, n, first);
-        // pieces behind this one that begin with the token
-        auto begin_with = [&](int q, uint32_t key) {
-            const size_t at = (size_t)(q + lane) * PIECE;
+        // how many of the pieces q, q + step, ... begin with the token, up to 64
+        auto begin_with = [&](int q, int step, uint32_t key) {
+            const size_t at = ((size_t)q + (size_t)lane * step) * PIECE;
             const uint64_t more = __builtin_amdgcn_ballot_w64(at < (size_t)n && pairs[at < (size_t)n ? at : 0].x == key);
             return ~more ? __builtin_ctzll(~more) : 64;
         };
@@ -593,10 +612,13 @@ __global__ __launch_bounds__(1024) void embedding_join_kernel(const u32x2* __res
         const int here = w.with(key, first, end), more = w.with(key, end, end + PIECE);
         if (key < vocab && here > 0 && here + more > PIECE && !(here == PIECE && first > 0 && w.key(first - 1) == key)) {
             found = key;
-            for (int m = 64; m == 64;) {
-                m = begin_with(last + 1, key);
-                last += m;
-            }
+            last += begin_with(last + 1, 1, key);
+            if (last == mine + 64)                                  // the run's end, 64 times nearer with each look
+                for (int left = pieces - 1 - last; left > 0;) {
+                    const int step = (left + 63) / 64;
+                    last += begin_with(last + step, step, key) * step;
+                    left = min(step - 1, pieces - 1 - last);
+                }
         }
     }
     const bool alone = found != 0xffffffffu && last - mine < ALONE;
@@ -641,8 +663,8 @@ struct Plan {
     int each, workgroups;                 // tokens of a workgroup of the sort
     int piece, pieces, blocks;            // pairs of a piece, pieces, 64-lane blocks of a row
     size_t row_pieces;                    // 16-byte pieces of a row
-    size_t pairs_bytes, hist_bytes, part_bytes;
-    size_t bytes() const { return few ? 0 : (gathered ? 1 : 2) * pairs_bytes + hist_bytes + part_bytes; }
+    size_t pairs_bytes, there_bytes, hist_bytes, part_bytes;
+    size_t bytes() const { return few ? 0 : (gathered ? 1 : 2) * pairs_bytes + there_bytes + hist_bytes + part_bytes; }
 };
 int bits_of(size_t v) {
     int bits = 0;
@@ -672,6 +694,7 @@ Plan plan(size_t n, size_t vocab, size_t d_model, int elem_bytes) {
     p.piece = n / 32 * p.blocks >= 1024 ? 32 : 8;
     p.pieces = (int)((n + p.piece - 1) / p.piece);
     p.pairs_bytes = whole(n * 8);
+    p.there_bytes = whole(vocab);
     p.part_bytes = p.pieces > 1 ? (size_t)p.pieces * 2 * d_model * 4 : 0;
     return p;
 }
@@ -706,8 +729,8 @@ size_t embedding_bwd_workspace_bytes(size_t n, size_t vocab, int d_model, int bf
 bool embedding_bwd_fits(size_t n, size_t vocab, int d_model, int bf16) {
     const Plan p = plan(n, vocab, d_model, bf16 ? 2 : 4);
     // waves of the sums and workgroups of the join
-    const size_t tasks = (size_t)p.pieces * p.blocks, cleared = vocab * p.row_pieces / (1024 * CLEARED);
-    return tasks < ((size_t)1 << 26) && ((size_t)p.pieces + 15) / 16 * ((d_model + 255) / 256) < ((size_t)1 << 22) && cleared < ((size_t)1 << 21);
+    return (size_t)p.pieces * p.blocks + vocab < ((size_t)1 << 26) &&
+           ((size_t)p.pieces + 15) / 16 * ((d_model + 255) / 256) < ((size_t)1 << 22);
 }
 
 int launch_embedding_bwd(const void* d_out, const void* ids, int ids64, void* table, size_t n, size_t vocab, int d_model, float scale, int into,
@@ -734,40 +757,47 @@ int launch_embedding_bwd(const void* d_out, const void* ids, int ids64, void* ta
         other = reinterpret_cast<u32x2*>(at);
         at += p.pairs_bytes;
     }
+    uint8_t* there = reinterpret_cast<uint8_t*>(at);
+    at += p.there_bytes;
     uint32_t* hist = reinterpret_cast<uint32_t*>(at);
     float* part = reinterpret_cast<float*>(at + p.hist_bytes);
+    // the last rows of the table, to be cleared beside the sort
+    size_t rows = vocab;
+    auto last_rows = [&](size_t bytes) {
+        const size_t row = p.row_pieces * 16, n = into ? 0 : std::min(rows, bytes / row);
+        rows -= n;
+        return Zeros{static_cast<char*>(table) + rows * row, n * p.row_pieces};
+    };
     with_types([&](auto, auto index) {
         using I = decltype(index);
         const I* from = static_cast<const I*>(ids);
-        const size_t table_pieces = vocab * p.row_pieces;
-        const uint32_t shares = into ? 0 : (uint32_t)((table_pieces + 1024 * CLEARED - 1) / (1024 * CLEARED));
         if (p.gathered) {
-            launch_kernel(embedding_gather_kernel<I>, dim3(CLASSES + shares), dim3(1024), (size_t)40 << p.bits, stream, from, pairs, table, count,
-                          (uint32_t)vocab, table_pieces, p.bits);
+            const Zeros zeros = last_rows(BESIDE);
+            launch_kernel(embedding_gather_kernel<I>, dim3(CLASSES + zeros.workgroups()), dim3(1024), (size_t)40 << p.bits, stream, from, pairs, there,
+                          count, (uint32_t)vocab, p.bits, zeros);
             return;
         }
-        const uint32_t launches = 2 * p.digits;      // each clears its part
-        for (uint32_t k = 0; k < (uint32_t)p.digits; ++k) {
+        for (int k = 0; k < p.digits; ++k) {
             auto pass = [&](auto first) {
                 const SortInput<I, first()> in{from, pairs, (uint32_t)vocab};
-                const uint32_t a = shares * (2 * k) / launches, b = shares * (2 * k + 1) / launches, c = shares * (2 * k + 2) / launches;
-                launch_kernel((embedding_count_kernel<I, first()>), dim3(p.workgroups + b - a), dim3(1024), 0, stream, in, hist, count, p.each, p.workgroups,
-                              (int)k * p.bits, p.bits, table, table_pieces, a);
-                launch_kernel((embedding_scatter_kernel<I, first()>), dim3(p.workgroups + c - b), dim3(1024), 0, stream, in, hist, other, count, p.each,
-                              p.workgroups, (int)k * p.bits, p.bits, table, table_pieces, b);
+                const Zeros a = last_rows(BESIDE_PASS), b = last_rows(BESIDE_PASS), none{there, k == 0 && !into ? p.there_bytes / 16 : 0};
+                launch_kernel((embedding_count_kernel<I, first()>), dim3(p.workgroups + none.workgroups() + a.workgroups()), dim3(1024), 0, stream, in, hist,
+                              count, p.each, p.workgroups, k * p.bits, p.bits, a, none, none.workgroups());
+                launch_kernel((embedding_scatter_kernel<I, first()>), dim3(p.workgroups + b.workgroups()), dim3(1024), 0, stream, in, hist, other,
+                              k == p.digits - 1 && !into ? there : nullptr, count, (uint32_t)vocab, p.each, p.workgroups, k * p.bits, p.bits, b);
             };
             if (k == 0) pass(std::true_type{}); else pass(std::false_type{});
             std::swap(pairs, other);
         }
     });
     if (hipGetLastError() != hipSuccess) return -1;
-    const int tasks = p.pieces * p.blocks;
+    const int tasks = p.pieces * p.blocks, zeros = into ? 0 : (int)rows;
     const bool cached = n * d_model * (bf16 ? 2 : 4) <= kStreamCached;
     auto sums = [&](auto elem, auto piece) {
         using T = decltype(elem);
         auto go = [&](auto in_cache) {
-            launch_kernel((embedding_sum_kernel<T, piece(), in_cache()>), dim3((tasks + 3) / 4), dim3(256), 0, stream, pairs,
-                          static_cast<const T*>(d_out), static_cast<T*>(table), part, count, (uint32_t)vocab, row_pieces, p.blocks, tasks, scale,
+            launch_kernel((embedding_sum_kernel<T, piece(), in_cache()>), dim3((tasks + zeros + 3) / 4), dim3(256), 0, stream, pairs,
+                          static_cast<const T*>(d_out), static_cast<T*>(table), part, count, (uint32_t)vocab, row_pieces, p.blocks, tasks, there, zeros, scale,
                           into != 0);
         };
         if (cached) go(std::true_type{}); else go(std::false_type{});
