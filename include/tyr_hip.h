@@ -473,8 +473,8 @@ int tyr_hip_embedding(const void* ids, int ids_dtype, const void* table, void* o
  *   d_out : [n, d_model]      d_table : [vocab, d_model], overlaps no input; both of dtype
  *   workspace : tyr_hip_embedding_bwd_workspace_bytes(...) bytes (0 also for shapes that the call refuses), 16-byte aligned, contents
  *               arbitrary; calls that overlap in time need one each (may be NULL where that is 0)
- * Supported: as the lookup, and n <= 2^30; with pieces of 32 tokens and blocks of 64 16-byte pieces of a row,
- * pieces * blocks + vocab < 2^26 and pieces / 16 * d_model / 256 < 2^22. */
+ * Supported: n, vocab and d_model as the lookup's, and n <= 2^30; with blocks of 64 16-byte pieces of a row, and pieces of 32 tokens (of 8
+ * where n / 32 * blocks < 1024), pieces * blocks + vocab < 2^26 and ceil(pieces / 16) * ceil(d_model / 256) < 2^22. */
 size_t tyr_hip_embedding_bwd_workspace_bytes(uint64_t n, uint64_t vocab, uint64_t d_model, int dtype);
 int tyr_hip_embedding_bwd(const void* d_out, const void* ids, int ids_dtype, void* d_table, uint64_t n, uint64_t vocab, uint64_t d_model,
                           float scale, int accumulate, int dtype, void* workspace, size_t workspace_bytes, void* stream);

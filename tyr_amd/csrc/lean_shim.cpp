@@ -766,6 +766,217 @@ lean_object* lean_tyr_gpu_rmsnorm_residual_bwd(uint64_t rows, uint64_t d, b_lean
     }
 }
 
+// ---- layer norm without a residual, and the gradients
+
+// layerNorm {rows d} x weight bias eps stream : IO (T #[rows,d])
+lean_object* lean_tyr_gpu_layernorm(uint64_t rows, uint64_t d, b_lean_obj_arg x, b_lean_obj_arg weight, b_lean_obj_arg bias, double eps,
+                                    uint64_t stream, lean_object* /*world*/) {
+    try {
+        auto x_ = borrowTensor(x), w_ = borrowTensor(weight), b_ = borrowTensor(bias);
+        std::string err;
+        if (!check(x_, "x", torch::kBFloat16, err) || !check(w_, "weight", torch::kBFloat16, err) || !check(b_, "bias", torch::kBFloat16, err))
+            return io_error(err);
+        LaunchStreamScope on_stream(stream, x_);   // outputs and scratch belong to the launch stream
+        auto out = torch::empty_like(x_);
+        const int rc = tyr_hip_layernorm_residual(x_.data_ptr(), nullptr, w_.data_ptr(), b_.data_ptr(), out.data_ptr(), nullptr, rows, d,
+                                                  (float)eps, reinterpret_cast<void*>(stream));
+        if (rc != TYR_HIP_OK) return status_error("layerNorm", rc);
+        return lean_io_result_mk_ok(giveTensor(std::move(out)));
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+static lean_object* layernorm_bwd(const char* what, uint64_t rows, uint64_t d, const torch::Tensor& g, const torch::Tensor* dr,
+                                  const torch::Tensor& h, const torch::Tensor& w, double eps, uint64_t stream) {
+    std::string err;
+    if (!check(g, "dOut", torch::kBFloat16, err) || !check(h, "resid", torch::kBFloat16, err) || !check(w, "weight", torch::kBFloat16, err) ||
+        (dr && !check(*dr, "dResid", torch::kBFloat16, err)))
+        return io_error(err);
+    LaunchStreamScope on_stream(stream, h);   // outputs and scratch belong to the launch stream
+    auto dx = torch::empty_like(h), dw = torch::empty_like(w), db = torch::empty_like(w);
+    const size_t ws_bytes = tyr_hip_layernorm_residual_bwd_workspace_bytes(rows, d);
+    auto ws = torch::empty({(int64_t)(ws_bytes ? ws_bytes : 16)}, h.options().dtype(torch::kUInt8));
+    const int rc = tyr_hip_layernorm_residual_bwd(g.data_ptr(), dr ? dr->data_ptr() : nullptr, h.data_ptr(), w.data_ptr(), dx.data_ptr(),
+                                                  dw.data_ptr(), db.data_ptr(), rows, d, (float)eps, ws.data_ptr(), ws_bytes,
+                                                  reinterpret_cast<void*>(stream));
+    if (rc != TYR_HIP_OK) return status_error(what, rc);
+    return triple_result(std::move(dx), std::move(dw), std::move(db));
+}
+
+// layerNormBwd {rows d} dOut x weight eps stream : IO (dX x dWeight x dBias)
+lean_object* lean_tyr_gpu_layernorm_bwd(uint64_t rows, uint64_t d, b_lean_obj_arg d_out, b_lean_obj_arg x, b_lean_obj_arg weight, double eps,
+                                        uint64_t stream, lean_object* /*world*/) {
+    try {
+        return layernorm_bwd("layerNormBwd", rows, d, borrowTensor(d_out), nullptr, borrowTensor(x), borrowTensor(weight), eps, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+// layerNormResidualBwd {rows d} dOut dResid resid weight eps stream : IO (dX x dWeight x dBias)
+lean_object* lean_tyr_gpu_layernorm_residual_bwd(uint64_t rows, uint64_t d, b_lean_obj_arg d_out, b_lean_obj_arg d_resid,
+                                                 b_lean_obj_arg resid, b_lean_obj_arg weight, double eps, uint64_t stream,
+                                                 lean_object* /*world*/) {
+    try {
+        const auto dr = borrowTensor(d_resid);
+        return layernorm_bwd("layerNormResidualBwd", rows, d, borrowTensor(d_out), &dr, borrowTensor(resid), borrowTensor(weight), eps, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+// ---- from tokens to rows, and from logits to log probabilities
+
+// Contiguous, on the device and of one of two types; `second` says which.
+static bool check_either(const torch::Tensor& t, const char* name, c10::ScalarType a, c10::ScalarType b, int& second, std::string& err) {
+    second = t.scalar_type() == b;
+    return check(t, name, second ? b : a, err);
+}
+static int element_type(const torch::Tensor& t) { return t.scalar_type() == torch::kBFloat16 ? TYR_HIP_BF16 : TYR_HIP_F32; }
+
+// embedding {n vocab d} ids table scale stream : IO (T #[n,d])
+lean_object* lean_tyr_gpu_embedding(uint64_t n, uint64_t vocab, uint64_t d, b_lean_obj_arg ids, b_lean_obj_arg table, double scale,
+                                    uint64_t stream, lean_object* /*world*/) {
+    try {
+        auto i_ = borrowTensor(ids), t_ = borrowTensor(table);
+        std::string err;
+        int wide = 0, low = 0;
+        if (!check_either(i_, "ids", torch::kInt32, torch::kInt64, wide, err) ||
+            !check_either(t_, "table", torch::kFloat32, torch::kBFloat16, low, err))
+            return io_error(err);
+        LaunchStreamScope on_stream(stream, t_);   // outputs and scratch belong to the launch stream
+        auto out = torch::empty({(int64_t)n, (int64_t)d}, t_.options());
+        const int rc = tyr_hip_embedding(i_.data_ptr(), wide ? TYR_HIP_I64 : TYR_HIP_I32, t_.data_ptr(), out.data_ptr(), n, vocab, d,
+                                         (float)scale, element_type(t_), reinterpret_cast<void*>(stream));
+        if (rc != TYR_HIP_OK) return status_error("embedding", rc);
+        return lean_io_result_mk_ok(giveTensor(std::move(out)));
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+static lean_object* embedding_bwd(const char* what, uint64_t n, uint64_t vocab, uint64_t d, const torch::Tensor& g, const torch::Tensor& ids,
+                                  const torch::Tensor* into, double scale, uint64_t stream) {
+    std::string err;
+    int low = 0, wide = 0;
+    if (!check_either(g, "dOut", torch::kFloat32, torch::kBFloat16, low, err) ||
+        !check_either(ids, "ids", torch::kInt32, torch::kInt64, wide, err) || (into && !check(*into, "dTable", g.scalar_type(), err)))
+        return io_error(err);
+    LaunchStreamScope on_stream(stream, g);   // outputs and scratch belong to the launch stream
+    // before the table, whose size a refused call may not give
+    const size_t ws_bytes = tyr_hip_embedding_bwd_workspace_bytes(n, vocab, d, element_type(g));
+    auto ws = torch::empty({(int64_t)(ws_bytes ? ws_bytes : 16)}, g.options().dtype(torch::kUInt8));
+    auto table = into ? *into : torch::empty({(int64_t)vocab, (int64_t)d}, g.options());
+    const int rc = tyr_hip_embedding_bwd(g.data_ptr(), ids.data_ptr(), wide ? TYR_HIP_I64 : TYR_HIP_I32, table.data_ptr(), n, vocab, d,
+                                         (float)scale, into ? 1 : 0, element_type(g), ws.data_ptr(), ws_bytes,
+                                         reinterpret_cast<void*>(stream));
+    if (rc != TYR_HIP_OK) return status_error(what, rc);
+    return lean_io_result_mk_ok(into ? lean_box(0) : giveTensor(std::move(table)));
+}
+
+// embeddingBwd {n vocab d} dOut ids scale stream : IO (T #[vocab,d])
+lean_object* lean_tyr_gpu_embedding_bwd(uint64_t n, uint64_t vocab, uint64_t d, b_lean_obj_arg d_out, b_lean_obj_arg ids, double scale,
+                                        uint64_t stream, lean_object* /*world*/) {
+    try {
+        return embedding_bwd("embeddingBwd", n, vocab, d, borrowTensor(d_out), borrowTensor(ids), nullptr, scale, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+// embeddingBwdInto {n vocab d} dOut ids dTable scale stream : IO Unit
+lean_object* lean_tyr_gpu_embedding_bwd_into(uint64_t n, uint64_t vocab, uint64_t d, b_lean_obj_arg d_out, b_lean_obj_arg ids,
+                                             b_lean_obj_arg d_table, double scale, uint64_t stream, lean_object* /*world*/) {
+    try {
+        const auto into = borrowTensor(d_table);
+        return embedding_bwd("embeddingBwdInto", n, vocab, d, borrowTensor(d_out), borrowTensor(ids), &into, scale, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+// tokenLogprobs {rows width} logits targets vocab top stream : IO (logp x lse x entropy x topLogp x topIds)
+lean_object* lean_tyr_gpu_token_logprobs(uint64_t rows, uint64_t width, b_lean_obj_arg logits, b_lean_obj_arg targets, uint64_t vocab,
+                                         uint64_t top, uint64_t stream, lean_object* /*world*/) {
+    try {
+        auto x_ = borrowTensor(logits), t_ = borrowTensor(targets);
+        std::string err;
+        int low = 0, wide = 0;
+        if (!check_either(x_, "logits", torch::kFloat32, torch::kBFloat16, low, err) ||
+            !check_either(t_, "targets", torch::kInt32, torch::kInt64, wide, err))
+            return io_error(err);
+        if (top > TYR_HIP_TOKEN_LOGPROBS_MAX_TOP) return status_error("tokenLogprobs", TYR_HIP_ERR_UNSUPPORTED);
+        LaunchStreamScope on_stream(stream, x_);   // outputs and scratch belong to the launch stream
+        const auto f32 = x_.options().dtype(torch::kFloat32);
+        auto logp = torch::empty({(int64_t)rows}, f32), lse = torch::empty({(int64_t)rows}, f32), entropy = torch::empty({(int64_t)rows}, f32);
+        auto top_logp = torch::empty({(int64_t)rows, (int64_t)top}, f32);
+        auto top_ids = torch::empty({(int64_t)rows, (int64_t)top}, x_.options().dtype(torch::kInt32));
+        const size_t ws_bytes = tyr_hip_token_logprobs_workspace_bytes(rows, vocab, top, element_type(x_));
+        auto ws = torch::empty({(int64_t)(ws_bytes ? ws_bytes : 16)}, x_.options().dtype(torch::kUInt8));
+        const int rc = tyr_hip_token_logprobs(x_.data_ptr(), t_.data_ptr(), wide ? TYR_HIP_I64 : TYR_HIP_I32, logp.data_ptr<float>(),
+                                              lse.data_ptr<float>(), entropy.data_ptr<float>(), top ? top_logp.data_ptr<float>() : nullptr,
+                                              top ? top_ids.data_ptr<int32_t>() : nullptr, rows, vocab, width, top, element_type(x_),
+                                              ws.data_ptr(), ws_bytes, reinterpret_cast<void*>(stream));
+        if (rc != TYR_HIP_OK) return status_error("tokenLogprobs", rc);
+        lean_object* result = giveTensor(std::move(top_ids));
+        for (torch::Tensor* t : {&top_logp, &entropy, &lse, &logp}) {
+            lean_object* pair = lean_alloc_ctor(0, 2, 0);
+            lean_ctor_set(pair, 0, giveTensor(std::move(*t)));
+            lean_ctor_set(pair, 1, result);
+            result = pair;
+        }
+        return lean_io_result_mk_ok(result);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+static lean_object* token_logprobs_bwd(const char* what, uint64_t rows, uint64_t width, const torch::Tensor& d_logp, const torch::Tensor* d_entropy,
+                                       const torch::Tensor* d_lse, const torch::Tensor& x, const torch::Tensor& targets, const torch::Tensor& lse,
+                                       const torch::Tensor* entropy, uint64_t vocab, uint64_t stream) {
+    std::string err;
+    int low = 0, wide = 0;
+    if (!check(d_logp, "dLogp", torch::kFloat32, err) || (d_entropy && !check(*d_entropy, "dEntropy", torch::kFloat32, err)) ||
+        (d_lse && !check(*d_lse, "dLse", torch::kFloat32, err)) || !check_either(x, "logits", torch::kFloat32, torch::kBFloat16, low, err) ||
+        !check_either(targets, "targets", torch::kInt32, torch::kInt64, wide, err) || !check(lse, "lse", torch::kFloat32, err) ||
+        (entropy && !check(*entropy, "entropy", torch::kFloat32, err)))
+        return io_error(err);
+    LaunchStreamScope on_stream(stream, x);   // outputs and scratch belong to the launch stream
+    auto dx = torch::empty_like(x);
+    const int rc = tyr_hip_token_logprobs_bwd(x.data_ptr(), targets.data_ptr(), wide ? TYR_HIP_I64 : TYR_HIP_I32, lse.data_ptr<float>(),
+                                              entropy ? entropy->data_ptr<float>() : nullptr, d_logp.data_ptr<float>(),
+                                              d_entropy ? d_entropy->data_ptr<float>() : nullptr, d_lse ? d_lse->data_ptr<float>() : nullptr,
+                                              dx.data_ptr(), rows, vocab, width, element_type(x), reinterpret_cast<void*>(stream));
+    if (rc != TYR_HIP_OK) return status_error(what, rc);
+    return lean_io_result_mk_ok(giveTensor(std::move(dx)));
+}
+
+// tokenLogprobsBwd {rows width} dLogp logits targets lse vocab stream : IO (T #[rows,width])
+lean_object* lean_tyr_gpu_token_logprobs_bwd(uint64_t rows, uint64_t width, b_lean_obj_arg d_logp, b_lean_obj_arg logits,
+                                             b_lean_obj_arg targets, b_lean_obj_arg lse, uint64_t vocab, uint64_t stream,
+                                             lean_object* /*world*/) {
+    try {
+        return token_logprobs_bwd("tokenLogprobsBwd", rows, width, borrowTensor(d_logp), nullptr, nullptr, borrowTensor(logits),
+                                  borrowTensor(targets), borrowTensor(lse), nullptr, vocab, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
+// tokenLogprobsEntropyBwd {rows width} dLogp dEntropy dLse logits targets lse entropy vocab stream : IO (T #[rows,width])
+lean_object* lean_tyr_gpu_token_logprobs_entropy_bwd(uint64_t rows, uint64_t width, b_lean_obj_arg d_logp, b_lean_obj_arg d_entropy,
+                                                     b_lean_obj_arg d_lse, b_lean_obj_arg logits, b_lean_obj_arg targets, b_lean_obj_arg lse,
+                                                     b_lean_obj_arg entropy, uint64_t vocab, uint64_t stream, lean_object* /*world*/) {
+    try {
+        const auto dh = borrowTensor(d_entropy), dl = borrowTensor(d_lse), h = borrowTensor(entropy);
+        return token_logprobs_bwd("tokenLogprobsEntropyBwd", rows, width, borrowTensor(d_logp), &dh, &dl, borrowTensor(logits),
+                                  borrowTensor(targets), borrowTensor(lse), &h, vocab, stream);
+    } catch (const std::exception& e) {
+        return io_error(e.what());
+    }
+}
+
 // ---- the cache in pages: bf16, or e4m3 with a factor per kv head
 
 static lean_object* paged_append(const char* what, uint64_t B, uint64_t T, uint64_t Hq, uint64_t Hkv, uint64_t D, uint64_t P, uint64_t ps,

@@ -228,6 +228,57 @@ opaque rmsNormBwd {rows d : UInt64} (dOut x : @& T #[rows, d]) (weight : @& T #[
 opaque rmsNormResidualBwd {rows d : UInt64} (dOut dResid resid : @& T #[rows, d]) (weight : @& T #[d]) (eps : Float)
     (stream : CudaStream) : IO (T #[rows, d] × T #[d])
 
+/-- Layer norm over the last axis, bf16: `(x − mean) · weight / √(var + eps) + bias`, shapes as `fusedLayerNormResidual`. -/
+@[extern "lean_tyr_gpu_layernorm"]
+opaque layerNorm {rows d : UInt64} (x : @& T #[rows, d]) (weight bias : @& T #[d]) (eps : Float) (stream : CudaStream)
+    : IO (T #[rows, d])
+
+/-- Gradients of `layerNorm`: `(dX, dWeight, dBias)`, bf16. -/
+@[extern "lean_tyr_gpu_layernorm_bwd"]
+opaque layerNormBwd {rows d : UInt64} (dOut x : @& T #[rows, d]) (weight : @& T #[d]) (eps : Float) (stream : CudaStream)
+    : IO (T #[rows, d] × T #[d] × T #[d])
+
+/-- Gradients of `fusedLayerNormResidual`: `resid` is the forward's `outResid`, `dResid` the gradient that reaches it from the
+    layers behind. Returns `(dX, dWeight, dBias)`; `dX` is the gradient of `x` and of `residual` alike. -/
+@[extern "lean_tyr_gpu_layernorm_residual_bwd"]
+opaque layerNormResidualBwd {rows d : UInt64} (dOut dResid resid : @& T #[rows, d]) (weight : @& T #[d]) (eps : Float)
+    (stream : CudaStream) : IO (T #[rows, d] × T #[d] × T #[d])
+
+/-- Rows of a table by token: `out[i] = scale · table[ids[i]]`, zeros for a token outside of the table (padding).
+    `ids : int32 | int64 [n]`, `table : f32 | bf16 [vocab, d]`. -/
+@[extern "lean_tyr_gpu_embedding"]
+opaque embedding {n vocab d : UInt64} (ids : @& T #[n]) (table : @& T #[vocab, d]) (scale : Float) (stream : CudaStream)
+    : IO (T #[n, d])
+
+/-- Gradient of `embedding` with respect to the table: row `v` is `scale` times the sum of the rows of `dOut : f32 | bf16` whose
+    token is `v`, zeros where there is none. Summed by sorted tokens, the same bits every time. -/
+@[extern "lean_tyr_gpu_embedding_bwd"]
+opaque embeddingBwd {n vocab d : UInt64} (dOut : @& T #[n, d]) (ids : @& T #[n]) (scale : Float) (stream : CudaStream)
+    : IO (T #[vocab, d])
+
+/-- `embeddingBwd` added to a gradient that is there (tied weights, accumulated batches): `dTable` is changed **in place**, in
+    the rows that have a token. -/
+@[extern "lean_tyr_gpu_embedding_bwd_into"]
+opaque embeddingBwdInto {n vocab d : UInt64} (dOut : @& T #[n, d]) (ids : @& T #[n]) (dTable : @& T #[vocab, d]) (scale : Float)
+    (stream : CudaStream) : IO Unit
+
+/-- Log probabilities of given tokens: `(logp, lse, entropy, topLogp, topIds)` of the first `vocab` columns of
+    `logits : f32 | bf16`, f32 results; `targets : int32 | int64`, `logp = 0` for one outside of `[0, vocab)` (padding). The `top`
+    (up to 64) largest log probabilities stand with their ids (int32) in falling order, equal ones by id. -/
+@[extern "lean_tyr_gpu_token_logprobs"]
+opaque tokenLogprobs {rows width : UInt64} (logits : @& T #[rows, width]) (targets : @& T #[rows]) (vocab top : UInt64)
+    (stream : CudaStream) : IO (T #[rows] × T #[rows] × T #[rows] × T #[rows, top] × T #[rows, top])
+
+/-- Gradient of `tokenLogprobs` with respect to the logits, from `dLogp : f32`; `lse` is the forward's. -/
+@[extern "lean_tyr_gpu_token_logprobs_bwd"]
+opaque tokenLogprobsBwd {rows width : UInt64} (dLogp : @& T #[rows]) (logits : @& T #[rows, width]) (targets lse : @& T #[rows])
+    (vocab : UInt64) (stream : CudaStream) : IO (T #[rows, width])
+
+/-- `tokenLogprobsBwd` with the gradients of `entropy` and `lse` too; both are the forward's. -/
+@[extern "lean_tyr_gpu_token_logprobs_entropy_bwd"]
+opaque tokenLogprobsEntropyBwd {rows width : UInt64} (dLogp dEntropy dLse : @& T #[rows]) (logits : @& T #[rows, width])
+    (targets lse entropy : @& T #[rows]) (vocab : UInt64) (stream : CudaStream) : IO (T #[rows, width])
+
 /-- `decodeRopeAppend` for a cache in pages, and for any number `Tn` of new tokens a sequence. `kPages vPages : bf16
     [P, Hkv, ps, D]` are written **in place**; row `j` of sequence `b` is row `j % ps` of page `pageTable[b, j / ps]` (int32).
     `cos sin : f32 [S, D/2]` is the whole rotary table, `positions : int32 [B]` where each sequence's first new token stands
