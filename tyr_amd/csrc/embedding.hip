@@ -104,19 +104,23 @@ struct Zeros {
     }
     __host__ uint32_t workgroups() const { return (uint32_t)((pieces + 1024 * emb::CLEARED - 1) / (1024 * emb::CLEARED)); }
 };
-// f32 sums to a row of the table, or to what is there
-template <class T>
-__device__ __forceinline__ void finish(T* to, float (&sum)[emb::Row<T>::E], float scale, bool into) {
+// f32 sums to a row of the table, or with what is there of it
+template <class T, bool INTO>
+__device__ __forceinline__ void finish(T* to, float (&sum)[emb::Row<T>::E], float scale, u32x4 there) {
     using R = emb::Row<T>;
 #pragma unroll
     for (int i = 0; i < R::E; ++i) sum[i] *= scale;
-    if (into) {
+    if constexpr (INTO) {
         float old[R::E];
-        R::unpack(ld_global_16(to), old);
+        R::unpack(there, old);
 #pragma unroll
         for (int i = 0; i < R::E; ++i) sum[i] += old[i];
     }
     st_global_16_nt(to, R::pack(sum));
+}
+template <class T>
+__device__ __forceinline__ void finish(T* to, float (&sum)[emb::Row<T>::E], float scale, bool into) {
+    if (into) finish<T, true>(to, sum, scale, ld_global_16(to)); else finish<T, false>(to, sum, scale, u32x4{});
 }
 // Lanes in front that are set.
 __device__ __forceinline__ int before(uint64_t lanes) { return __builtin_popcountll(lanes & (((uint64_t)1 << (threadIdx.x & 63)) - 1)); }
@@ -494,10 +498,10 @@ struct Window {
 // One wave: 64 lanes of 16 bytes of the rows of PIECE consecutive pairs, and of those of a last run that goes on behind them, if it is no longer
 // than PIECE; a run in front that is the wave's before, it leaves out.  Waves behind those of the pieces have a row of the
 // table each, of the first `zero_rows`, and clear it where it has no token.
-template <class T, int PIECE, bool CACHED>
+template <class T, int PIECE, bool CACHED, bool INTO>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(const u32x2* __restrict__ pairs, const T* __restrict__ d_out, T* __restrict__ table,
                                                             float* __restrict__ part, int n, uint32_t vocab, int row_pieces, int blocks,
-                                                            int tasks, const uint8_t* __restrict__ there, int zero_rows, float scale, bool into) {
+                                                            int tasks, const uint8_t* __restrict__ there, int zero_rows, float scale) {
     using R = emb::Row<T>;
     constexpr int E = R::E;
     const int lane = threadIdx.x & 63, task = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -533,6 +537,10 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const u32x2* __restr
     float sum[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) sum[i] = 0.0f;
+    // What is there of a row is asked for with the rows that are added to it.
+    auto old_row = [&](uint32_t key) { return ld_global_16(table + (size_t)min(key, vocab - 1) * d + col); };
+    u32x4 old = {0, 0, 0, 0};
+    if constexpr (INTO) old = old_row(key);
     auto end_run = [&](bool open) {
         if (key >= vocab || !has) return;
         if (from_before || open) {
@@ -540,14 +548,17 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const u32x2* __restr
 #pragma unroll
             for (int i = 0; i < E; i += 4) *reinterpret_cast<f32x4*>(to + i) = f32x4{sum[i], sum[i + 1], sum[i + 2], sum[i + 3]};
         } else {
-            finish(table + (size_t)key * d + col, sum, scale, into);
+            finish<T, INTO>(table + (size_t)key * d + col, sum, scale, old);
         }
     };
-    constexpr int AHEAD = 16;
-    u32x4 row[AHEAD];
+    constexpr int AHEAD = INTO ? 8 : 16;
+    u32x4 row[AHEAD], olds[AHEAD];
     for (; t < last; t += AHEAD) {
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) row[u] = ld_stream_16<CACHED>(d_out + (size_t)w.place(min(t + u, last - 1)) * d + col);
+        for (int u = 0; u < AHEAD; ++u) {
+            row[u] = ld_stream_16<CACHED>(d_out + (size_t)w.place(min(t + u, last - 1)) * d + col);
+            if constexpr (INTO) olds[u] = old_row(w.key(min(t + u, last - 1)));
+        }
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             if (t + u >= last) break;
@@ -555,6 +566,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const u32x2* __restr
             if (k != key) {
                 end_run(false);
                 key = k;
+                if constexpr (INTO) old = olds[u];
                 from_before = false;
 #pragma unroll
                 for (int i = 0; i < E; ++i) sum[i] = 0.0f;
@@ -795,12 +807,12 @@ int launch_embedding_bwd(const void* d_out, const void* ids, int ids64, void* ta
     const bool cached = n * d_model * (bf16 ? 2 : 4) <= kStreamCached;
     auto sums = [&](auto elem, auto piece) {
         using T = decltype(elem);
-        auto go = [&](auto in_cache) {
-            launch_kernel((embedding_sum_kernel<T, piece(), in_cache()>), dim3((tasks + zeros + 3) / 4), dim3(256), 0, stream, pairs,
-                          static_cast<const T*>(d_out), static_cast<T*>(table), part, count, (uint32_t)vocab, row_pieces, p.blocks, tasks, there, zeros, scale,
-                          into != 0);
+        auto go = [&](auto in_cache, auto add) {
+            launch_kernel((embedding_sum_kernel<T, piece(), in_cache(), add()>), dim3((tasks + zeros + 3) / 4), dim3(256), 0, stream, pairs,
+                          static_cast<const T*>(d_out), static_cast<T*>(table), part, count, (uint32_t)vocab, row_pieces, p.blocks, tasks, there, zeros, scale);
         };
-        if (cached) go(std::true_type{}); else go(std::false_type{});
+        if (cached) { if (into) go(std::true_type{}, std::true_type{}); else go(std::true_type{}, std::false_type{}); }
+        else { if (into) go(std::false_type{}, std::true_type{}); else go(std::false_type{}, std::false_type{}); }
         if (p.pieces > 1)
             launch_kernel((embedding_join_kernel<T, piece()>), dim3((p.pieces + 15) / 16 * ((d_model + 255) / 256)), dim3(1024), 0, stream, pairs, part,
                           static_cast<T*>(table), count, (uint32_t)vocab, d_model, (d_model + 255) / 256, p.pieces, scale, into != 0);
