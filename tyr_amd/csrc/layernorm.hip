@@ -164,7 +164,7 @@ __global__ __launch_bounds__(1024) void layernorm_residual_bwd_kernel(
     using namespace row_ops;
     constexpr int LPR = S::LPR, WPR = S::WPR, ROWS = 1024 / (LPR * WPR);
     static_assert(S::P == 1, "a lane holds one piece of a row");
-    constexpr int FEW = WPR > 8 ? 4 : WPR;                         // sums of waves read at a time: registers
+    constexpr int JOINED = WPR <= 2 ? 2 : WPR <= 4 ? 4 : WPR <= 8 ? 8 : 16;      // lanes that add the sums of a row's waves, one of them each
     __shared__ f32x4 part[2][ROWS][WPR];
     extern __shared__ __attribute__((aligned(16))) float sums[];   // [ROWS / 2][2][d_model]
     const int lane = threadIdx.x % LPR, wave = threadIdx.x / 64, wr = wave % WPR;
@@ -174,7 +174,9 @@ __global__ __launch_bounds__(1024) void layernorm_residual_bwd_kernel(
     const int at = has ? 2 * (slot * d_model + pc) : NOWHERE;      // their place in a group of rows
     const float inv_d = 1.0f / (float)d_model;
     auto elements = [&](int i) { return 8.0f * (float)max(0, min(LPR, d_model / 8 - LPR * i)); };      // of wave i of a row
-    const float mine = fmaxf(elements(wr), 1.0f);
+    const float inv_mine = 1.0f / fmaxf(elements(wr), 1.0f);
+    const int other = lane % JOINED;                               // the wave whose sums this lane reads
+    const float others = other < WPR ? elements(other) : 0.0f;
     float w[8], dw[8], db[8];
     unpack8(has ? ld_global_16(weight + pc) : u32x4{0, 0, 0, 0}, w);
 #pragma unroll
@@ -198,10 +200,11 @@ __global__ __launch_bounds__(1024) void layernorm_residual_bwd_kernel(
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum += h[i];
         // of the wave's elements: their mean, and about it the sums of squares, of g w and of g w times the difference
-        float mean = over_lanes<LPR>(sum, Add{}) / mine, sq = 0.0f, gw = 0.0f, gwc = 0.0f;
+        float mean = over_lanes<LPR>(sum, Add{}) * inv_mine, sq = 0.0f, gw = 0.0f, gwc = 0.0f;
+        const float here = has ? mean : 0.0f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float c = has ? h[i] - mean : 0.0f, a = g[i] * w[i];
+            const float c = h[i] - here, a = g[i] * w[i];
             sq += c * c;
             gw += a;
             gwc += a * c;
@@ -213,23 +216,27 @@ __global__ __launch_bounds__(1024) void layernorm_residual_bwd_kernel(
             // two sets of sums in turn: a wave that is already at the next row writes the other one
             if (lane == 0) part[turn][slot][wr] = f32x4{mean, sq, gw, gwc};
             __syncthreads();
-            float total = 0.0f;
-#pragma unroll FEW
-            for (int i = 0; i < WPR; ++i) total += part[turn][slot][i][0] * elements(i);
-            mean = total / (float)d_model;
-            sq = gw = gwc = 0.0f;
-#pragma unroll FEW
-            for (int i = 0; i < WPR; ++i) {
-                const f32x4 q = part[turn][slot][i];
+            if constexpr (WPR == 2) {
+                const f32x4 q0 = part[turn][slot][0], q1 = part[turn][slot][1];
+                const float n0 = elements(0), n1 = elements(1);
+                mean = (q0[0] * n0 + q1[0] * n1) * inv_d;
+                const float d0 = q0[0] - mean, d1 = q1[0] - mean;
+                sq = q0[1] + n0 * d0 * d0 + (q1[1] + n1 * d1 * d1);
+                gw = q0[2] + q1[2];
+                gwc = q0[3] + q0[2] * d0 + (q1[3] + q1[2] * d1);
+            } else {                                                 // a wave's sums a lane, not all of them in every lane: 4096 x 5120 54.9 -> 41.2 us
+                const f32x4 q = part[turn][slot][min(other, WPR - 1)];
+                const bool real = WPR == JOINED || other < WPR;
+                mean = over_lanes<JOINED>(q[0] * others, Add{}) * inv_d;
                 const float d = q[0] - mean;
-                sq += q[1] + elements(i) * d * d;
-                gw += q[2];
-                gwc += q[3] + q[2] * d;
+                sq = over_lanes<JOINED>(real ? q[1] + others * d * d : 0.0f, Add{});
+                gw = over_lanes<JOINED>(real ? q[2] : 0.0f, Add{});
+                gwc = over_lanes<JOINED>(real ? q[3] + q[2] * d : 0.0f, Add{});
             }
             turn ^= 1;
         }
         const bool real = first + slot < rows;
-        const float var = sq / (float)d_model + eps;
+        const float var = sq * inv_d + eps;
         float rho = real ? rsqrtf(var) : 0.0f;
         float rho_x = rho;                                           // of dx; the other is that of h as it stands in registers
         float c = gwc * inv_d * rho * rho * rho;                     // in this order: rho^3 alone leaves f32 for rows of 1e13 or 1e-13
@@ -375,7 +382,7 @@ constexpr size_t ALONE = 2;                                          // so many 
 template <class S>
 size_t bwd_parts(size_t rows) {
     constexpr int ROWS = 1024 / (S::LPR * S::WPR);
-    const size_t groups = (rows + ROWS - 1) / ROWS, most = groups <= ALONE ? 1 : S::WPR == 10 && rows >= 4096 ? 512 : 256;
+    const size_t groups = (rows + ROWS - 1) / ROWS, most = groups <= ALONE ? 1 : 256;
     return groups < most ? groups : most;
 }
 }  // namespace
