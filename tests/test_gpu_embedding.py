@@ -2,7 +2,8 @@
 
 Tolerances.  The lookup is one f32 product, rounded once more: its bits are known.  A row of the gradient of c tokens is a sum in f32 of 32 rows
 at most in turn, of 1/8 of the pieces of 8 or 32 tokens that the token reaches into, and of 8: fewer than 64 + c/64 roundings of 2^-24 of the
-terms' sizes (a factor and an addition to what was there among them), and one of the result: 2^-8 (bf16), 2^-24 (f32)."""
+terms' sizes (a factor and an addition to what was there among them), and one of the result: 2^-8 (bf16), 2^-24 (f32).  Few tokens are up to 128
+rows in turn, the k-th rounding of which is one of k/128 of the sizes: 64 and what is in the other term."""
 import pytest
 import torch
 
@@ -117,6 +118,33 @@ def test_a_frequent_token_among_rare_ones():
                 _check(tyr_amd.embedding_bwd(g, ids, n + 40), g, ids, n + 40, 1.0, None)
 
 
+@pytest.mark.parametrize("n,vocab,d,dtype", [(3000, 40001, 1024, "bf16"), (300, 50, 1 << 19, "f32"), (33000, 60001, 1024, "f32"), (300, 270000, 512, "bf16")])
+def test_tables_larger_than_what_is_cleared_beside_the_sort(n, vocab, d, dtype):
+    """The rows without a token that the sums' launch clears, and those before it; the memory held NaN."""
+    import tyr_amd
+    g, ids = _rows(n, 512, TYPES[dtype], 15).repeat(1, d // 512), _ids("text", n, vocab)
+    for index in (ids, vocab - 1 - ids):                        # tokens are frequent at the beginning of the table, or at its end
+        held = torch.full((vocab, d), float("nan"), dtype=TYPES[dtype], device="cuda")
+        del held
+        got = tyr_amd.embedding_bwd(g, index, vocab, scale=0.75)
+        _check(got, g, index, vocab, 0.75, None)
+        assert torch.equal(got, tyr_amd.embedding_bwd(g, index, vocab, scale=0.75))
+        del got
+
+
+def test_runs_over_many_pieces_end_anywhere():
+    import tyr_amd
+    n = 32000
+    for runs in ((515, 17, 600, 1, 4096, 9, 2050, 24000), (31000, 5, 700), (8 * 64, 8 * 65 - 3, 8 * 66 + 1, 8 * 129, 8 * 193 + 5, 25000), (1, 32 * 65 - 1, 2, 32 * 200, 32 * 513)):
+        ids = torch.repeat_interleave(torch.arange(len(runs)), torch.tensor(runs))[:n].to("cuda")
+        ids = ids[torch.randperm(len(ids), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda")]
+        for d in (64, 2048):                                     # pieces of 8, of 32
+            g = _rows(len(ids), d, torch.bfloat16, 16)
+            base = _rows(9, d, torch.bfloat16, 17)
+            _check(tyr_amd.embedding_bwd(g, ids, 9), g, ids, 9, 1.0, None)
+            _check(tyr_amd.embedding_bwd(g, ids, 9, into=base.clone()), g, ids, 9, 1.0, base)
+
+
 def test_gradient_against_differences():
     """The lookup is linear: its difference quotient in the table is exact in float64."""
     import tyr_amd
@@ -157,6 +185,8 @@ def test_refusals():
             (lambda: tyr_amd.embedding_bwd(g, i[:3], 10), "dOut must have the shape"), (lambda: tyr_amd.embedding_bwd(g, i, 0), "status -2"),
             (lambda: tyr_amd.embedding_bwd(g, i, -1), "vocab must not be negative"), (lambda: tyr_amd.embedding_bwd(g, i, 2 ** 40), "status -2"),
             (lambda: tyr_amd.embedding_bwd(g, i, 10, into=t[:9]), "into must be"), (lambda: tyr_amd.embedding_bwd(g, i, 10, into=t.float()), "into must have dtype"),
-            (lambda: tyr_amd.embedding_bwd(g[:, :60].contiguous(), i, 10), "status -3")]:
+            (lambda: tyr_amd.embedding_bwd(g[:, :60].contiguous(), i, 10), "status -3"), (lambda: tyr_amd.embedding_bwd(g, i, 1 << 26), "status -2"),
+            (lambda: tyr_amd.embedding_bwd(g, i, 4, into=g), "into must not overlap dOut"),
+            (lambda: tyr_amd.embedding_bwd(t[2:6], i, 4, into=t[5:9]), "into must not overlap dOut")]:
         with pytest.raises(tyr_amd.TyrGpuError, match=message):
             call()

@@ -601,7 +601,11 @@ PyObject* embedding_bwd(PyObject* const* a) {
     const at::Tensor* into = optional(a[4], "into", g.scalar_type(), 2);
     if (into && (into->size(0) != vocab || into->size(1) != d)) fail("into must be [vocab, d_model]");
     not_empty({&ids, &g}, "embeddingBwd");
-    if (vocab == 0 || vocab > INT32_MAX) check_status(TYR_HIP_ERR_BAD_SHAPE, "embeddingBwd");      // nothing is allocated for it
+    if (vocab == 0 || vocab >= (int64_t)1 << 26) check_status(TYR_HIP_ERR_BAD_SHAPE, "embeddingBwd");      // nothing is allocated for it
+    if (into) {
+        const char *to = (const char*)into->data_ptr(), *from = (const char*)g.data_ptr();
+        if (to < from + g.nbytes() && from < to + into->nbytes()) fail("into must not overlap dOut");
+    }
     const OnDevice on(g, {&ids, into}, truth(a[5]));
     at::Tensor table;
     int rc;
