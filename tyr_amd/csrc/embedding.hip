@@ -5,7 +5,7 @@
 //
 // The gradient is summed by sorted tokens: no atomic additions of floating point, the same bits every time.  Three ways:
 //   few tokens       one launch: a workgroup has the tokens of its residue class, finds them among all, adds their rows, and clears the others
-//   up to 2^15       such classes put their pairs (token, place) together, equal tokens side by side; then the sums
+//   up to 24576      such classes put their pairs (token, place) together, equal tokens side by side; then the sums
 //   more             a radix sort of the pairs, then the sums
 // The sort notes which tokens are there, and beside the sums the rows of the others are cleared.  The sort's own launches leave the memory idle:
 // beside them the end of the table is cleared as a whole, where tokens are rare if they are numbered by how frequent they are.
@@ -52,13 +52,18 @@ __device__ __forceinline__ uint32_t key_of(int32_t id) { return (uint32_t)id; }
 __device__ __forceinline__ uint32_t key_of(int64_t id) { return (uint64_t)id >> 31 ? 0xffffffffu : (uint32_t)id; }
 
 constexpr int CLASSES = 256;              // residue classes of tokens, a workgroup each
-constexpr int FEW = 2048;                 // tokens times 64-lane blocks of a row, of one launch
-constexpr int GATHERED = 1 << 15;         // tokens at most that classes put together
+// Tokens times 64-lane blocks of a row, of one launch.  900 tokens of 1024 bf16 15.1 us so (half of them one token 24.6) and 20.6 (21.9) as the next
+// form; 1800 17.7 (35.2) so and 20.9 (23.4).
+constexpr int FEW = 2048;
+// Tokens at most that classes put together.  20000 28.8 us so (half of them one token 50.3) and 36.1 (48.5) by the radix sort; 30000 34.5 (67.0), 41.8 (57.8).
+constexpr int GATHERED = 3 << 13;
 constexpr int MAX_QUOTIENTS = 1024;       // quotients by CLASSES at most, for both
 constexpr int CHUNK = 1024, CHUNKS = 128; // radix sort: tokens of a turn, workgroups at most
 constexpr int MAX_DIGIT = 9;
 constexpr int CLEARED = 16;               // 16-byte pieces that a thread of 1024 fills with zeros
-constexpr size_t BESIDE = (size_t)48 << 20, BESIDE_PASS = (size_t)20 << 20;      // bytes of the table cleared beside the classes, a launch of the radix sort
+// Bytes of the table cleared beside the classes, beside a launch of the radix sort.  24500 tokens of a 65536 x 2048 bf16 table 74 us, without 80;
+// 32768 89.0, with 20 MB 91.0, without 100.
+constexpr size_t BESIDE = (size_t)48 << 20, BESIDE_PASS = (size_t)32 << 20;
 constexpr int HELD = 256;                 // pairs that a wave keeps of its share
 }  // namespace emb
 
@@ -251,11 +256,12 @@ __global__ __launch_bounds__(1024, 8) void embedding_gather_kernel(const I* __re
     auto put = [&](u32x2 pair, bool own) {
         uint64_t same = __builtin_amdgcn_ballot_w64(own);
         if (!same) return;
-        const uint32_t d = own ? pair.x / CLASSES : 0;
-        for (int b = 0; b < bits; ++b) {
-            const uint64_t set = __builtin_amdgcn_ballot_w64(d >> b & 1);
-            same &= d >> b & 1 ? set : ~set;
-        }
+        const uint32_t d = own ? pair.x / CLASSES : 0, first = __builtin_amdgcn_readlane(d, __builtin_ctzll(same));
+        if (__builtin_amdgcn_ballot_w64(own && d != first))
+            for (int b = 0; b < bits; ++b) {
+                const uint64_t set = __builtin_amdgcn_ballot_w64(d >> b & 1);
+                same &= d >> b & 1 ? set : ~set;
+            }
         const int rank = before(same);
         const uint32_t at = count[d];
         if (own) {
@@ -537,7 +543,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const u32x2* __restr
     float sum[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) sum[i] = 0.0f;
-    // What is there of a row is asked for with the rows that are added to it.
+    // What is there of a row is asked for with the rows that are added to it: 16384 different tokens of 1024 f32 48 us; at the end of each run 58.
     auto old_row = [&](uint32_t key) { return ld_global_16(table + (size_t)min(key, vocab - 1) * d + col); };
     u32x4 old = {0, 0, 0, 0};
     if constexpr (INTO) old = old_row(key);
@@ -551,7 +557,7 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(const u32x2* __restr
             finish<T, INTO>(table + (size_t)key * d + col, sum, scale, old);
         }
     };
-    constexpr int AHEAD = INTO ? 8 : 16;
+    constexpr int AHEAD = INTO ? 8 : 16;      // 32768 tokens of 65536 x 2048 bf16 91 us with 16, 97 with 8; with 8 in turns of two sets 89, but f32 5 % more
     u32x4 row[AHEAD], olds[AHEAD];
     for (; t < last; t += AHEAD) {
 #pragma unroll
@@ -702,7 +708,8 @@ Plan plan(size_t n, size_t vocab, size_t d_model, int elem_bytes) {
         p.workgroups = (int)((n + p.each - 1) / p.each);
         p.hist_bytes = whole((size_t)p.workgroups * ((size_t)4 << p.bits));
     }
-    // long pieces where they leave a wave for every SIMD
+    // long pieces where they leave a wave for every SIMD.  Where they leave two: 8192 tokens of 2048 bf16 for a whole table 44.6 us, with pieces of 8
+    // 49.1, added to a gradient 29.8 and 27.6; all one token 35.6 and 42.1.
     p.piece = n / 32 * p.blocks >= 1024 ? 32 : 8;
     p.pieces = (int)((n + p.piece - 1) / p.piece);
     p.pairs_bytes = whole(n * 8);
