@@ -67,7 +67,8 @@ constexpr size_t BESIDE = (size_t)48 << 20, BESIDE_PASS = (size_t)32 << 20;
 constexpr int HELD = 256;                 // pairs that a wave keeps of its share
 }  // namespace emb
 
-// 2^shift threads a row, 256 >> shift rows a workgroup.
+// 2^shift threads a row, 256 >> shift rows a workgroup.  16384 rows of 65536 x 2048 bf16 16.3 us: 67 MB written past the caches and 26 MB of
+// distinct rows read, 5.7 TB/s.
 template <class T, class I>
 __global__ __launch_bounds__(256) void embedding_kernel(const I* __restrict__ ids, const T* __restrict__ table, T* __restrict__ out, size_t n,
                                                         uint32_t vocab, int pieces, int shift, float scale) {
@@ -177,7 +178,7 @@ __device__ __forceinline__ void add_scan(uint32_t* place, const uint32_t* total,
 // Classes: workgroup c has the tokens that are c modulo CLASSES.  It counts over all ids how many pairs stand in front of its own, those of
 // smaller classes, and how many each wave finds of each quotient in its share of the ids; so every wave knows where its pairs go and puts them
 // there without another's help.  there[token] = whether it is.  Workgroups behind the classes clear the end of the table.  LDS:
-// count [16][digits], total and front [digits].
+// count [16][digits], total and front [digits].  16384 tokens 9.1 us, which is latency: ids, counts, a scan.
 template <class I>
 __global__ __launch_bounds__(1024, 8) void embedding_gather_kernel(const I* __restrict__ ids, u32x2* __restrict__ pairs, uint8_t* __restrict__ there, int n,
                                                                    uint32_t vocab, int bits, Zeros zeros) {
@@ -278,7 +279,8 @@ __global__ __launch_bounds__(1024, 8) void embedding_gather_kernel(const I* __re
 }
 
 // Few tokens, all in one launch.  A workgroup keeps its class's pairs in LDS and clears the rows of the others.  Tokens that are there up to
-// LIGHT times are summed by one group of waves that covers a row; more frequent ones by all groups, joined through LDS.
+// LIGHT times are summed by one group of waves that covers a row; more frequent ones by all groups, joined through LDS.  900 tokens of a
+// 32768 x 1024 bf16 table 13.9 us, 67 MB of them zeros: 4.9 TB/s with 3 us of looking for the tokens.
 template <class T, class I>
 __global__ __launch_bounds__(1024) void embedding_few_kernel(const I* __restrict__ ids, const T* __restrict__ d_out, T* __restrict__ table, int n,
                                                              uint32_t vocab, int row_pieces, int blocks, float scale, bool into) {
@@ -395,7 +397,7 @@ __global__ __launch_bounds__(1024) void embedding_few_kernel(const I* __restrict
 }
 
 // More: a radix sort from the low digit up, two launches a digit.  Workgroup w has the tokens [w each, (w + 1) each); those behind
-// clear memory.  The last launch notes which tokens are there.
+// clear memory.  The last launch notes which tokens are there.  32768 tokens in four launches 28.7 us, 128 MB cleared beside them.
 template <class I, bool FIRST>
 struct SortInput {
     const I* ids;
@@ -504,6 +506,7 @@ struct Window {
 // One wave: 64 lanes of 16 bytes of the rows of PIECE consecutive pairs, and of those of a last run that goes on behind them, if it is no longer
 // than PIECE; a run in front that is the wave's before, it leaves out.  Waves behind those of the pieces have a row of the
 // table each, of the first `zero_rows`, and clear it where it has no token.
+// 32768 tokens of 2048 bf16, 126 MB read and 142 written, 52 us: 5.3 TB/s (with the zeros first 57, in turn with the sums 60).
 template <class T, int PIECE, bool CACHED, bool INTO>
 __global__ __launch_bounds__(256) void embedding_sum_kernel(const u32x2* __restrict__ pairs, const T* __restrict__ d_out, T* __restrict__ table,
                                                             float* __restrict__ part, int n, uint32_t vocab, int row_pieces, int blocks,
@@ -602,7 +605,7 @@ __device__ __forceinline__ void finish_four(float* to, f32x4 sum, float scale, b
 }
 
 // Long runs: a workgroup looks through 16 pieces, a wave each, for those where one begins, and adds the rows that they left, 256 columns of them:
-// the wave itself up to ALONE rows, all waves in turn more of them.
+// the wave itself up to ALONE rows, all waves in turn more of them.  6 us, of which the search is most.
 template <class T, int PIECE>
 __global__ __launch_bounds__(1024) void embedding_join_kernel(const u32x2* __restrict__ pairs, const float* __restrict__ part, T* __restrict__ table,
                                                               int n, uint32_t vocab, int d_model, int blocks, int pieces, float scale, bool into) {
