@@ -191,54 +191,18 @@ __device__ __forceinline__ uint32_t top_key(const uint32_t (&key)[N], int top, u
     return found;
 }
 // c.chosen = the `top` largest of the first `count` of the list, in order, 0 behind the last; all threads call it.  A few by counting how many
-// are larger than each, which one wave does in registers up to 64 of them; where there are more, those are out first whose value alone is too
-// small.  Many, which are ties, by one search for each of the chosen.
+// are larger than each; many, which are ties, by one search for each of the chosen.
 __device__ __forceinline__ void choose(Candidates& c, int count, int top) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (count <= KEPT) {
-        if (wave == 0) {                                          // the others leave it their share of the vector unit
-            uint64_t* list = c.list;
-            if (count > 64) {
-                list += KEPT;
-                uint32_t key[KEPT / 64], few[2];
-#pragma unroll
-                for (int k = 0; k < KEPT / 64; ++k) key[k] = lane + 64 * k < count ? (uint32_t)(c.list[lane + 64 * k] >> 32) : 0;
-                few[0] = key[0], few[1] = key[1];
-                const uint32_t least = count <= 128 ? top_key(few, top, 1) : top_key(key, top, 1);
-                int above = 0, ties = 0;
-#pragma unroll
-                for (int k = 0; k < KEPT / 64; ++k) {
-                    above += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[k] > least));
-                    ties += __builtin_popcountll(__builtin_amdgcn_ballot_w64(key[k] == least));
-                }
-                uint32_t place[KEPT / 64], first = 0;                 // of the ties the first that there is room for
-                if (above + ties > 64) {
-#pragma unroll
-                    for (int k = 0; k < KEPT / 64; ++k) place[k] = key[k] == least && least != 0 ? (uint32_t)c.list[lane + 64 * k] : 0;
-                    first = top_key(place, top - above, 1);
-                }
-                int n = 0;
-#pragma unroll
-                for (int k = 0; k < KEPT / 64; ++k) {
-                    const bool stays = key[k] != 0 && (key[k] > least || (key[k] == least && (first == 0 || place[k] >= first)));
-                    const uint64_t all = __builtin_amdgcn_ballot_w64(stays);
-                    if (stays) list[n + __builtin_popcountll(all & (((uint64_t)1 << lane) - 1))] = c.list[lane + 64 * k];
-                    n += __builtin_popcountll(all);
-                }
-                count = __builtin_amdgcn_readfirstlane(n);            // at most 64: `top` of them where there were ties
-                __builtin_amdgcn_wave_barrier();
-            }
-            if (lane < top && lane >= count) c.chosen[lane] = 0;
-            count = __builtin_amdgcn_readfirstlane(count);
-            const uint64_t mine = lane < count ? list[lane] : 0;
+        if ((int)threadIdx.x < top && (int)threadIdx.x >= count) c.chosen[threadIdx.x] = 0;
+        for (int first = wave * 64; first < count; first += THREADS) {
+            const bool has = first + lane < count;
+            const uint64_t mine = has ? c.list[first + lane] : 0;
             int front = 0;
-#pragma unroll 4
-            for (int j = 0; j < count; ++j) {
-                const uint64_t other = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(mine >> 32), j) << 32 |
-                                       (uint32_t)__builtin_amdgcn_readlane((int)mine, j);
-                front += other > mine;
-            }
-            if (lane < count && front < top) c.chosen[front] = mine;
+#pragma unroll 8
+            for (int j = 0; j < count; ++j) front += c.list[j] > mine;
+            if (has && front < top) c.chosen[front] = mine;
         }
     } else {
         uint64_t limit = ~(uint64_t)0;
