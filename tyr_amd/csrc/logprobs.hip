@@ -434,17 +434,26 @@ __global__ __launch_bounds__(lp::THREADS) void token_logprobs_join_kernel(const 
         const Part q = parts[row * cut + i];
         a = join(a, Sum{q.m, q.s, q.t});
     }
+    // No alternative is below the top-th largest of each part's first few: one key a lane, or four.  128 and fewer are all put
+    // in order (160 12.1 us with a limit, 12.4 without; 32 12.9 and 11.4).
+    constexpr uint32_t LEAST_BIT = sizeof(T) == 2 ? 0x10000 : 1;
+    const bool all = cut * top <= THREADS / 2;
     uint32_t limit = 0;
+    uint64_t mine = 0;
     if constexpr (TOP) {
-        // no alternative is below the top-th largest of each part's first few
-        const int first = min(top, JOINED / cut);
-        uint32_t key[JOINED / 64];
+        const uint64_t* ranks = part_tops + row * cut * top;
+        auto key_of = [&](int i, int first) { return i < cut * first ? (uint32_t)(ranks[i] >> 32) : 0; };
+        if (all) {
+            if ((int)threadIdx.x < cut * top) mine = ranks[threadIdx.x];
+        } else if (top <= 24 && cut <= 32) {
+            const uint32_t key[1] = {key_of(lane, min(top, 64 / cut))};
+            limit = top_key(key, top, LEAST_BIT);
+        } else {
+            uint32_t key[JOINED / 64];
 #pragma unroll
-        for (int k = 0; k < JOINED / 64; ++k) {
-            const int i = lane + 64 * k;
-            key[k] = i < cut * first ? (uint32_t)(part_tops[row * cut * top + i] >> 32) : 0;
+            for (int k = 0; k < JOINED / 64; ++k) key[k] = key_of(lane + 64 * k, min(top, JOINED / cut));
+            limit = top_key(key, top, LEAST_BIT);
         }
-        limit = top_key(key, top, 1);
     }
     a = over_wave(a);
     const float ls = logf(a.s);
@@ -453,12 +462,16 @@ __global__ __launch_bounds__(lp::THREADS) void token_logprobs_join_kernel(const 
         __shared__ Candidates c;
         if (threadIdx.x == 0) c.count = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < cut * top; i += THREADS) {  // at most as many as the list holds
-            const uint64_t r = part_tops[row * cut * top + i];
-            if (r != 0 && (uint32_t)(r >> 32) >= limit) c.list[atomicAdd(&c.count, 1)] = r;
+        if (all) {
+            c.list[threadIdx.x] = mine;                           // 0, no element, is behind all of them
+        } else {
+            for (int i = threadIdx.x; i < cut * top; i += THREADS) {  // at most as many as the list holds
+                const uint64_t r = part_tops[row * cut * top + i];
+                if (r != 0 && (uint32_t)(r >> 32) >= limit) c.list[atomicAdd(&c.count, 1)] = r;
+            }
         }
         __syncthreads();
-        choose(c, c.count, top);
+        choose(c, all ? cut * top : c.count, top);
         write_top(out, row, c, top, a, ls);
     }
 }
