@@ -91,6 +91,21 @@ def test_alternatives_of_ties_and_sorted_rows(rows, vocab, dtype, kind):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,vocab", [(1, 40000), (2, 131072), (20, 70001), (1, 400000)])
+def test_alternatives_of_rows_in_parts(rows, vocab, dtype):
+    """As many from each part, all from one of them, and ties across them, around the numbers where another way is taken."""
+    import tyr_amd
+    i = torch.arange(vocab, device="cuda", dtype=torch.float32)
+    spread, equal, dense = -((i * 7919) % 8191), torch.full_like(i, 2.0), _logits(1, vocab, torch.float32, scale=2.0 ** -9)[0] + 10.0
+    together = torch.where((i > vocab - 300) & (i < vocab - 200), 20.0 - (i % 13), spread)
+    for x in (spread, together, equal, dense):
+        x = x.to(TYPES[dtype]).expand(rows, vocab).contiguous()
+        t = torch.arange(rows, device="cuda") * 5
+        for top in (2, 4, 8, 15, 24, 25, 40):
+            _check(tyr_amd.token_logprobs(x, t, top=top), x, t, vocab, top)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("vocab", [3, 70, 3001, 40007])
 def test_masked_and_extreme_rows(vocab, dtype):
     import tyr_amd
