@@ -507,8 +507,8 @@ int tyr_hip_token_logprobs(const void* logits, const void* targets, int targets_
  *   logits, targets : the forward's      lse, entropy : its results (entropy only with d_entropy)
  *   d_logp, d_entropy, d_lse : f32 [rows], NULL = zeros; d_logp of a target outside of [0, vocab) counts as zero
  *   d_logits : as logits; may be logits itself (fastest where both begin at the same place of 16 bytes)
- * A row whose gradients are all zero, or whose lse is -infinity, gets zeros whatever else it holds.  p has the precision of lse:
- * |lse| 2^-24 of its size. */
+ * A row whose gradients are all zero, or whose lse is -infinity, gets zeros whatever else it holds; entropy is not looked at where d_entropy
+ * is 0.  p has the precision of lse: |lse| 2^-24 of its size. */
 int tyr_hip_token_logprobs_bwd(const void* logits, const void* targets, int targets_dtype, const float* lse, const float* entropy,
                                const float* d_logp, const float* d_entropy, const float* d_lse, void* d_logits, uint64_t rows,
                                uint64_t vocab, uint64_t width, int dtype, void* stream);

@@ -497,9 +497,9 @@ __global__ __launch_bounds__(lp::BWD_THREADS) void token_logprobs_bwd_kernel(con
     const int target = has_target ? (int)given : -1;
     const float g = has_target ? d_logp[row] : 0.0f, gh = ENTROPY ? d_entropy[row] : 0.0f, l = lse[row];
     float k = (d_lse ? d_lse[row] : 0.0f) - g, kh = -gh * LN2;    // dx = p (k + kh log2 p)
-    if constexpr (ENTROPY) k -= gh * entropy[row];
     // a row without a gradient, or without a logit above -infinity
     const bool zero = (g == 0.0f && k == 0.0f && gh == 0.0f) || l == -__builtin_inff();
+    if constexpr (ENTROPY) k -= gh != 0.0f ? gh * entropy[row] : 0.0f;      // an entropy without a gradient may be NaN
     // dx = e (k + kh y) with e = 2^y; y is relative to c, which is lse log2(e) but for its rounding: that much goes into k and kh
     const bool tame = fabsf(l) < 0x1p20f;
     const float c = l * LOG2E;
