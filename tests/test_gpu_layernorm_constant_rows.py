@@ -52,3 +52,31 @@ def test_rows_of_any_width(d):
     values = [3.0, -0.1, 99840.0, -1.5e7, 1.1e18, 1.7e9, 2.0 ** 30 * 1.9921875]
     _check_forward(values, d, 1e-5)
     _check_gradients(values, d, 1e-5)
+
+
+@pytest.mark.parametrize("eps", [1e-5, 1e-25, 1e-38, 1e-40])
+@pytest.mark.parametrize("d", WIDTHS)
+def test_rows_beyond_f32(d, eps):
+    """Their sum is, or their squares, or eps beside them."""
+    values = [3.0, 2.0 ** 90 * 1.25, -(2.0 ** 118 * 1.171875), 2.0 ** 126 * 1.9, -3.38e38, 2.0 ** -90 * 1.4, 2.0 ** -130 * 1.25, 0.0]
+    _check_forward(values, d, eps)
+    _check_gradients(values, d, eps)
+
+
+@pytest.mark.parametrize("d", [104, 1000, 4096])
+def test_one_such_row_among_others(d):
+    """It does not reach the gradients of the weights, and the other rows are what they are without it."""
+    import tyr_amd
+    gen = torch.Generator(device="cuda").manual_seed(d)
+    x, g = (torch.randn(50, d, generator=gen, device="cuda").bfloat16() for _ in range(2))
+    w, b = _weights(d)
+    g[17] = 0.0                                                  # row 17 adds nothing to dw, whatever it holds
+    out, _ = tyr_amd.layernorm_residual(x, None, w, b)
+    dx, dw, db = tyr_amd.layernorm_residual_bwd(g, x, w)
+    other = [i for i in range(50) if i != 17]
+    for value in (2.0 ** 126, -3.38e38, 2.0 ** 90 * 1.25, 2.0 ** 15 * 1.546875):
+        x[17] = value
+        out2, _ = tyr_amd.layernorm_residual(x, None, w, b)
+        assert torch.equal(out2[17], b) and torch.equal(out2[other], out[other])
+        dx2, dw2, db2 = tyr_amd.layernorm_residual_bwd(g, x, w)
+        assert not bool(dx2[17].any()) and torch.equal(dx2[other], dx[other]) and torch.equal(dw2, dw) and torch.equal(db2, db)

@@ -132,7 +132,8 @@ __global__ __launch_bounds__(S::THREADS) void layernorm_residual_kernel(
             for (int i = 0; i < 8; ++i) { const float c = f[i] * k - mean; sq += c * c; }
         }
         sq = over_lanes<LPR>(sq, Add{});
-        inv_std = rsqrtf(sq / (float)d_model + eps * k * k);
+        const float scaled = sq / (float)d_model + eps * k * k;
+        inv_std = scaled < 0x1p-126f && eps > 0.0f ? 1.0f : rsqrtf(scaled);      // equal elements, n = 0: eps k^2 has left f32, eps is not 0
         each<P>([&](auto p) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[p][i] *= k;
@@ -279,8 +280,13 @@ __global__ __launch_bounds__(1024) void layernorm_residual_bwd_kernel(
             sq = over_lanes<LPR>(sq, Add{});
             gw = over_lanes<LPR>(gw, Add{});
             gwc = over_lanes<LPR>(gwc, Add{});
-            rho = rsqrtf(sq / (float)d_model + eps * k * k);
+            const float scaled = sq / (float)d_model + eps * k * k;
+            rho = rsqrtf(scaled);
             rho_x = rho * k;
+            if (scaled < 0x1p-126f && eps > 0.0f) {                  // equal elements, n = 0: eps k^2 has left f32, eps is not 0
+                rho = 1.0f;
+                rho_x = 1.0f / sqrtf(eps);
+            }
             c = gwc * inv_d * rho * rho * rho * k;
 #pragma unroll
             for (int i = 0; i < 8; ++i) h[i] *= k;                   // what underflows is nothing beside the row's largest
