@@ -297,6 +297,7 @@ int tyr_hip_rope_fwd(const void* x, const float* cos, const float* sin, void* y,
  * the gradients.
  *
  *   x, residual, out, out_resid : bf16 [rows, d_model]      weight, bias : bf16 [d_model]
+ *   out and out_resid may be x or residual themselves (not both the same one); otherwise they overlap no input
  * Supported: a launch of fewer than 2^32 threads: rows * (elements of a row, rounded up to 64 * 2^n) < 2^35, twice that above 512.
  */
 int tyr_hip_layernorm_residual(const void* x, const void* residual, const void* weight,
