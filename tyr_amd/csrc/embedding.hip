@@ -711,8 +711,10 @@ Plan plan(size_t n, size_t vocab, size_t d_model, int elem_bytes) {
         p.workgroups = (int)((n + p.each - 1) / p.each);
         p.hist_bytes = whole((size_t)p.workgroups * ((size_t)4 << p.bits));
     }
-    // long pieces where they leave a wave for every SIMD.  Where they leave two: 8192 tokens of 2048 bf16 for a whole table 44.6 us, with pieces of 8
-    // 49.1, added to a gradient 29.8 and 27.6; all one token 35.6 and 42.1.
+    // Long pieces where they leave a wave for every SIMD, short ones where they do not, one rule for a whole table and for sums that are added to one.
+    // 8192 tokens of 2048 bf16, one wave: a whole table 45.6 us so and 49.8 with pieces of 8 (all one token 51.8 and 62.7), added 29.9 and
+    // 27.8 (33.3 and 40.0); 16384 added 41.4 and 44.4 (49.1 and 65.3).  4096, which leave half of the SIMDs without: a whole table 46.0 so and
+    // 44.1 with pieces of 32 (49.2 and 44.3), added 22.3 and 28.0 (27.1 and 24.4).
     p.piece = n / 32 * p.blocks >= 1024 ? 32 : 8;
     p.pieces = (int)((n + p.piece - 1) / p.piece);
     p.pairs_bytes = whole(n * 8);

@@ -22,7 +22,7 @@ namespace tyr {
 
 // WPR waves per row; a lane holds P <= 2 pieces (8 bf16) of it, lane, lane + LPR * WPR, so that all loads of a row, weights
 // included, are under way at once and many waves share the chip (one wave per row, up to 16 pieces a lane: 2222 x 4096
-// 16.8 us, 300 x 8192 17; so 13.1 and 7.1).  65536 x 1024 without a residual 43.7 us, 6.1 TB/s.
+// 16.8 us, 300 x 8192 17; so 13.1 and 7.1).  65536 x 1024 without a residual 43.8 us, 6.1 TB/s.
 template <class S, bool CACHED, bool RESIDUAL, bool BIAS>
 __global__ __launch_bounds__(S::THREADS) void layernorm_residual_kernel(
     const uint16_t* __restrict__ x, const uint16_t* __restrict__ res, const uint16_t* __restrict__ weight,
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(S::THREADS) void layernorm_residual_kernel(
 // Gradients.  Workgroups of 16 waves (or as many of them as whole rows need): as many row slots as fit, slot s of workgroup i takes the rows
 // ROWS (i + k gridDim.x) + s, the next one's loads under way while it works on one, and keeps dw and dbias of its rows in registers.  The slots
 // are added through LDS at the end, half of them to the other half at a time, and the workgroup writes one row of part [gridDim.x][2][d_model].
-// 65536 x 1024 with d_resid 84.8 us, 6.3 TB/s, and 4 for the parts; 2000 x 4096 13.6 and 3.  Wide rows are nearly bound by the vector units (a row of
+// 65536 x 1024 with d_resid 89 us (the least of 40 launches 86), 6.0 TB/s, and 5 for the parts; 2000 x 4096 15.1 (13.7) and 3 to 5.  Wide rows are nearly bound by the vector units (a row of
 // 5120 takes each of its ten waves some 260 instructions): 20000 x 5120 155 us, 5.3 TB/s.  Two and three rows ahead 2 to 60 % slower (registers).
 template <class S, bool CACHED, bool RESID>
 __global__ __launch_bounds__(1024) void layernorm_residual_bwd_kernel(

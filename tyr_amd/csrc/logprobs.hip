@@ -8,7 +8,7 @@
 // One pass over the row: every lane keeps m, s and t of its own elements and scales them when its m grows; they are joined at the end, in f32.
 // The alternatives need no second pass: the `top`-th largest of the lanes' m is no larger than the `top`-th largest element.  Every lane keeps
 // the maxima of its blocks of 64 bytes, too, and only the blocks that reach that limit are read once more (all of such a lane's elements:
-// each 16 bytes of them another cache line, with 20 alternatives nearly the whole row again, 4096 x 50001 108 us, 82 so).
+// each 16 bytes of them another cache line, with 20 alternatives nearly the whole row again, 4096 x 50001 108 us, 80 so).
 //
 // Bound by HBM (bf16: and nearly by the vector units, 7 to 9 instructions an element, of which the exponential counts as four).
 //
@@ -254,8 +254,8 @@ __device__ __forceinline__ int64_t target_of(const void* targets, int is64, size
 }
 }  // namespace lp
 
-// Workgroup (row, part of it).  Rows of one part are finished here, others leave a Part and their alternatives.  4096 x 50001 bf16 with entropy
-// and 5 alternatives 74.5 us, 5.5 TB/s; 32 x 131072 with 20 8.6 us, 4.3 of them without alternatives.
+// Workgroup (row, part of it).  Rows of one part are finished here, others leave a Part and their alternatives.  A pass over 4096 x 50001 bf16
+// with entropy and 5 alternatives 75 us, 5.5 TB/s; 32 x 131072 with 20 8.6 us, 4.3 of them without alternatives.
 template <class T, bool CACHED, bool ENTROPY, bool TOP>
 __global__ __launch_bounds__(lp::THREADS) void token_logprobs_kernel(const T* __restrict__ logits, const void* __restrict__ targets, int targets64,
                                                                      lp::Out out, lp::Part* __restrict__ parts, uint64_t* __restrict__ part_tops,
@@ -326,7 +326,9 @@ __global__ __launch_bounds__(lp::THREADS) void token_logprobs_kernel(const T* __
     }
     if constexpr (TOP) {
         // No element below the top-th largest of the threads' largest is an alternative; nor below that of four threads' together, which is one
-        // key a lane and for small `top` hardly less.  One wave looks for it, by the upper 16 bits of the keys.
+        // key a lane and for small `top` hardly less.  One wave looks for it, by the upper 16 bits of the keys.  One key a lane is faster for few rows
+        // (32 x 131072, top 8 13.9 us and by four 14.6, 20 15.7 and 16.4, 28 16.6 and 17.1), and slower for many from some 28 alternatives on, the
+        // more so the nearer they are to the 64 keys (4096 x 50001, 28 82.3 and 81.5, 48 94.1 and 86.1, 64 613 and 91).
         if (wave == 0) {
             uint32_t key[WAVES], four[1] = {0};
 #pragma unroll
@@ -435,7 +437,8 @@ __global__ __launch_bounds__(lp::THREADS) void token_logprobs_join_kernel(const 
         a = join(a, Sum{q.m, q.s, q.t});
     }
     // No alternative is below the top-th largest of each part's first few: one key a lane, or four.  128 and fewer are all put
-    // in order (160 12.1 us with a limit, 12.4 without; 32 12.9 and 11.4).
+    // in order (160 12.1 us with a limit, 12.4 without; 32 12.9 and 11.4).  One key a lane where that is two of each part or more and `top` is far
+    // below 64: 32 x 131072 of 32 parts, top 16 14.9 us so and 15.1 by four, 20 15.6 and 15.9, 24 15.8 and 16.0.
     constexpr uint32_t LEAST_BIT = sizeof(T) == 2 ? 0x10000 : 1;
     const bool all = cut * top <= THREADS / 2;
     uint32_t limit = 0;
@@ -476,8 +479,8 @@ __global__ __launch_bounds__(lp::THREADS) void token_logprobs_join_kernel(const 
     }
 }
 
-// The gradient: workgroup (row, part of it).  logits and d_logits may be the same memory: a thread writes where it alone has read.  4096 x 50001
-// bf16 128 us, 6.4 TB/s; 777 x 50001 f32 with entropy 51.6, 6.0 TB/s.
+// The gradient: workgroup (row, part of it).  logits and d_logits may be the same memory: a thread writes where it alone has read.  A pass
+// over 4096 x 50001 bf16 130 us, 6.3 TB/s; 777 x 50001 f32 with entropy 52.7, 5.9 TB/s.
 template <class T, bool CACHED, bool ENTROPY>
 __global__ __launch_bounds__(lp::BWD_THREADS) void token_logprobs_bwd_kernel(const T* logits, const void* __restrict__ targets, int targets64,
                                                                          const float* __restrict__ lse, const float* __restrict__ entropy,
